@@ -12,6 +12,8 @@ from . import _build
 OK = 0
 S_TABLE_FULL = 1
 S_WAIT_TIMEOUT = 2
+S_BAD_OFFSETS = 3
+S_BAD_INDEX = 4
 F16, BF16, F32_TF32, F32_IEEE = 0, 1, 2, 3
 
 _P = c_void_p
@@ -87,6 +89,13 @@ _PROTOTYPES = {
     "fgb_sparse_conv_dgrad": (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int64, c_int64, c_int, c_int, c_int, c_int, _P, c_int64, _P, _P]),
     "fgb_sparse_conv_wgrad": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int, _P, c_int64, _P, _P]),
     "fgb_sparse_conv_workspace_bytes": (c_int64, [c_int, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int]),
+    "fgb_sample_offsets": (c_int, [_P, c_int64, c_int64, _P, _P, _P]),
+    "fgb_group_norm_workspace_bytes": (c_int64, [_P]),
+    "fgb_group_norm_forward": (c_int, [_P, _P]),
+    "fgb_group_norm_backward": (c_int, [_P, _P]),
+    "fgb_embedding_forward": (c_int, [_P, _P]),
+    "fgb_embedding_workspace_bytes": (c_int64, [_P]),
+    "fgb_embedding_backward": (c_int, [_P, _P]),
     "fgb_noalloc_max_channels": (c_int, []),
     "fgb_subm_conv_bias_grad_noalloc": (c_int, [_P, _P, _P, c_int64, c_int, c_int, _P]),
 }

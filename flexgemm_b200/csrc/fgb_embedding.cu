@@ -1,0 +1,365 @@
+// Embedding: rows of a table by index, scaled; the gradient of the table by sorted indices.
+//
+//   out[i] = scale * table[t_i]          grad[v] = scale * sum over i with t_i = v of g[i]
+//
+// The gradient sorts the positions by index (stable, fgb_sort.cu) and walks the sorted list in chunks of fixed length: a
+// group of threads adds the rows of one chunk, one run of equal indices after the other, in fp32.  A run that ends where
+// it began, in one chunk, is final; the two runs of a chunk that reach beyond its ends leave their sums in a slab, and a
+// second kernel adds a run's pieces up.  Nothing is added atomically, so the order of every sum is fixed, and an index
+// that every other position holds costs no more than a spread one.
+#include <algorithm>
+
+#include "fgb_common.cuh"
+#include "fgb_device.cuh"
+#include "fgb_rows.cuh"
+
+namespace fgb {
+
+constexpr int kEmbThreads = 256;
+constexpr int kEmbRows = 4;      // rows in flight per thread of the lookup
+
+__device__ __forceinline__ int64_t index_at(const void* p, int wide, uint32_t i) {
+  return wide ? __ldg(static_cast<const int64_t*>(p) + i) : __ldg(static_cast<const int32_t*>(p) + i);
+}
+
+// ------------------------------------------------------------------ lookup
+template <typename T, int kVec, bool kScaled>
+__global__ void __launch_bounds__(kEmbThreads) embedding_kernel(const void* __restrict__ indices, int wide, const T* __restrict__ table, T* __restrict__ out,
+                                                                uint32_t n, uint32_t rows, int C, float scale, int32_t* status, int32_t* mirror) {
+  using Ch = Channels<T, kVec>;
+  chain_release();
+  chain_wait();
+  const int packs = C / kVec, width = min(kEmbThreads, packs), lanes = kEmbThreads / width;
+  const int cx = threadIdx.x % width, ry = threadIdx.x / width;
+  if (ry >= lanes) return;
+  for (uint32_t r0 = blockIdx.x * (lanes * kEmbRows); r0 < n; r0 += gridDim.x * (lanes * kEmbRows)) {
+    int64_t idx[kEmbRows];
+#pragma unroll
+    for (int u = 0; u < kEmbRows; ++u) {
+      const uint32_t r = r0 + u * lanes + ry;
+      idx[u] = r < n ? index_at(indices, wide, r) : 0;
+    }
+    for (int c = cx; c < packs; c += width) {
+      typename Ch::Raw raw[kEmbRows];
+#pragma unroll
+      for (int u = 0; u < kEmbRows; ++u) {
+        raw[u] = typename Ch::Raw{};
+        if (idx[u] >= 0 && idx[u] < int64_t(rows)) raw[u] = Ch::load(table + size_t(idx[u]) * C + c * kVec);
+      }
+#pragma unroll
+      for (int u = 0; u < kEmbRows; ++u) {
+        const uint32_t r = r0 + u * lanes + ry;
+        if (r >= n) continue;
+        if constexpr (kScaled) {
+          float f[kVec];
+          Ch::unpack(raw[u], f);
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) f[i] *= scale;
+          raw[u] = Ch::pack(f);
+        }
+        Ch::store(out + size_t(r) * C + c * kVec, raw[u]);
+      }
+    }
+    if (cx == 0) {
+#pragma unroll
+      for (int u = 0; u < kEmbRows; ++u) {
+        if (idx[u] < 0 || idx[u] >= int64_t(rows)) {
+          report(status, FGB_S_BAD_INDEX);
+          mirror_code(mirror, FGB_S_BAD_INDEX);
+        }
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ gradient
+// Sort keys: the index, or `rows` for a position that adds nothing (padding, out of range), which sorts behind all others.
+// Also clears the gradient (rows of indices that no position holds stay zero) and the counter of cut runs.
+__global__ void __launch_bounds__(kEmbThreads) embedding_keys_kernel(const void* __restrict__ indices, int wide, uint32_t n, uint32_t rows, int64_t padding,
+                                                                     int32_t* __restrict__ keys, uint16_t* __restrict__ grad, uint64_t grad_halves,
+                                                                     uint32_t* cut_count, int32_t* status, int32_t* mirror) {
+  chain_release();
+  chain_wait();
+  const uint32_t t = blockIdx.x * kEmbThreads + threadIdx.x, total = gridDim.x * kEmbThreads;
+  if (t == 0) *cut_count = 0u;
+  for (uint32_t i = t; i < n; i += total) {
+    const int64_t v = index_at(indices, wide, i);
+    const bool in = v >= 0 && v < int64_t(rows);
+    if (!in) {
+      report(status, FGB_S_BAD_INDEX);
+      mirror_code(mirror, FGB_S_BAD_INDEX);
+    }
+    keys[i] = static_cast<int32_t>(in && v != padding ? static_cast<uint32_t>(v) : rows);
+  }
+  const uint64_t whole = grad_halves / 8;
+  for (uint64_t i = t; i < whole; i += total) reinterpret_cast<uint4*>(grad)[i] = make_uint4(0, 0, 0, 0);
+  if (t < grad_halves - whole * 8) grad[whole * 8 + t] = 0;
+}
+
+struct EmbGrad {
+  const void* g;
+  void* grad;
+  const int32_t* keys;      // by position
+  const int64_t* order;     // positions by key
+  float* slab;              // [chunks][2][C]: the sum of the chunk's run that began before it, and of the one that goes on behind it
+  uint32_t* cut;            // [1 + chunks]: number of runs that go on behind the chunk they begin in, and those chunks
+  uint32_t n, rows, chunk, chunks;
+  int C;
+  float scale;
+};
+
+template <typename T, int kVec>
+__global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const EmbGrad p) {
+  using Ch = Channels<T, kVec>;
+  extern __shared__ uint32_t s_mem[];
+  chain_release();
+  const int packs = p.C / kVec, width = min(kEmbThreads, packs), lanes = kEmbThreads / width;
+  const int cx = threadIdx.x % width, ry = threadIdx.x / width;
+  const uint32_t per_cta = lanes * p.chunk;
+  uint32_t* s_key = s_mem + 1;               // keys of the CTA's positions, one before and one behind them
+  uint32_t* s_pos = s_mem + per_cta + 2;
+  chain_wait();
+  const uint32_t base = blockIdx.x * per_cta;  // < n
+  const uint32_t none = 0xFFFFFFFFu;
+  for (uint32_t i = threadIdx.x; i < per_cta + 2u; i += kEmbThreads) {
+    const uint32_t at = base + i - 1u;  // wraps to 2^32 - 1 ahead of the first
+    uint32_t key = none, pos = 0;
+    if (at < p.n) {
+      pos = static_cast<uint32_t>(__ldg(&p.order[at]));
+      pos = min(pos, p.n - 1u);  // the order is void after a sort that gave up
+      key = static_cast<uint32_t>(__ldg(&p.keys[pos]));
+    }
+    s_mem[i] = key;
+    if (i >= 1u && i <= per_cta) s_pos[i - 1u] = pos;
+  }
+  __syncthreads();
+  if (ry >= lanes) return;
+  const uint32_t b = ry * p.chunk, e = min(b + p.chunk, p.n > base ? p.n - base : 0u);
+  if (b >= e) return;
+  const uint32_t q = blockIdx.x * lanes + ry;  // chunk
+  const T* g = static_cast<const T*>(p.g);
+  T* grad = static_cast<T*>(p.grad);
+  for (int c = cx; c < packs; c += width) {
+    float acc[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) acc[i] = 0.f;
+    uint32_t key = s_key[b];
+    bool open = static_cast<int32_t>(s_key[int(b) - 1]) == static_cast<int32_t>(key);  // the run began in an earlier chunk
+    auto flush = [&](bool goes_on) {
+      if (key >= p.rows) return;
+      if (open || goes_on) {
+        float* to = p.slab + (size_t(q) * 2 + (open ? 0 : 1)) * p.C + c * kVec;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) to[i] = acc[i];
+        if (!open && c == 0) p.cut[1u + atomicAdd(p.cut, 1u)] = q;  // the list's order decides which CTA adds a run up, never a result
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) acc[i] *= p.scale;
+        Ch::store(grad + size_t(key) * p.C + c * kVec, Ch::pack(acc));
+      }
+    };
+    auto add = [&](uint32_t i, const typename Ch::Raw& raw) {
+      const uint32_t k = s_key[i];
+      if (k != key) {
+        flush(false);
+        open = false;
+        key = k;
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) acc[v] = 0.f;
+      }
+      float f[kVec];
+      Ch::unpack(raw, f);
+#pragma unroll
+      for (int v = 0; v < kVec; ++v) acc[v] += f[v];
+    };
+    uint32_t i = b;
+    constexpr int kUnroll = 8;
+    for (; i + kUnroll <= e; i += kUnroll) {
+      typename Ch::Raw raw[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) raw[u] = Ch::load(g + size_t(s_pos[i + u]) * p.C + c * kVec);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) add(i + u, raw[u]);
+    }
+    for (; i < e; ++i) add(i, Ch::load(g + size_t(s_pos[i]) * p.C + c * kVec));
+    flush(s_key[e] == key);
+  }
+}
+
+// The runs that lie in more than one chunk.  A CTA takes 32 channels of a run: its 32 groups of eight threads add every
+// 32nd piece, and their sums are added in order.
+constexpr int kJoinCols = 32;
+template <typename T>
+__global__ void __launch_bounds__(kEmbThreads) embedding_join_kernel(const EmbGrad p) {
+  __shared__ float s_sum[32][kJoinCols + 1];
+  chain_release();
+  chain_wait();
+  const uint32_t slices = static_cast<uint32_t>((p.C + kJoinCols - 1) / kJoinCols);
+  const uint32_t work = *p.cut * slices;
+  const int cx = threadIdx.x & 7, ry = threadIdx.x >> 3;
+  for (uint32_t w = blockIdx.x; w < work; w += gridDim.x) {
+    const uint32_t q = p.cut[1u + w / slices];
+    const int c0 = static_cast<int>(w % slices) * kJoinCols + cx * 4;
+    const uint32_t end = min((q + 1u) * p.chunk, p.n);  // > end of the chunk the run begins in
+    auto key_at = [&](uint32_t i) { return p.keys[min(static_cast<uint32_t>(p.order[i]), p.n - 1u)]; };
+    const int32_t key = key_at(end - 1u);
+    uint32_t lo = end, hi = p.n;  // the run's end: positions below lo hold the key, those from hi on do not
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo) / 2u;
+      if (key_at(mid) == key) lo = mid + 1u;
+      else hi = mid;
+    }
+    const uint32_t last = (lo - 1u) / p.chunk;  // chunk that holds the run's last position
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t k = q + ry; k <= last; k += 32u) {
+      const float* from = p.slab + (size_t(k) * 2 + (k == q ? 1 : 0)) * p.C + c0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c0 + i < p.C) acc[i] += from[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s_sum[ry][cx * 4 + i] = acc[i];
+    __syncthreads();
+    if (threadIdx.x < kJoinCols) {
+      const int c = static_cast<int>(w % slices) * kJoinCols + threadIdx.x;
+      if (c < p.C && key >= 0 && static_cast<uint32_t>(key) < p.rows) {
+        float v = 0.f;
+        for (int i = 0; i < 32; ++i) v += s_sum[i][threadIdx.x];
+        static_cast<T*>(p.grad)[size_t(key) * p.C + c] = static_cast<T>(v * p.scale);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------ host side
+struct EmbPlan {
+  int vec, lanes;
+  uint32_t chunk, chunks;
+  size_t keys_off, order_off, sort_off, sort_bytes, slab_off, cut_off, bytes;
+};
+static int emb_plan(const fgb_embedding_call& c, EmbPlan& p) {
+  p.vec = row_pack(c.c, elem_bytes(c.dtype));
+  const int packs = c.c / p.vec, width = std::min(packs, kEmbThreads);
+  p.lanes = kEmbThreads / width;
+  // long chunks leave little in the slab, short ones make more of them: some 1000 threads for every SM before chunks grow
+  int64_t chunk = 8;
+  while (chunk < 64 && c.n / (2 * chunk) * width >= int64_t(device_sm_count()) * 1024) chunk *= 2;
+  p.chunk = static_cast<uint32_t>(chunk);
+  p.chunks = static_cast<uint32_t>(ceil_div(c.n, chunk));
+  const int64_t sort = fgb_pp_sorted_idx_workspace_bytes(c.n);
+  if (sort < 0) return static_cast<int>(sort);
+  p.sort_bytes = static_cast<size_t>(sort);
+  p.keys_off = 0;
+  p.order_off = align256(c.n * 4);
+  p.sort_off = p.order_off + align256(c.n * 8);
+  p.slab_off = p.sort_off + align256(sort);
+  p.cut_off = p.slab_off + align256(int64_t(p.chunks) * 2 * c.c * 4);
+  p.bytes = p.cut_off + align256((int64_t(p.chunks) + 1) * 4);
+  return FGB_OK;
+}
+
+static int emb_check(const fgb_embedding_call* c) {
+  if (c == nullptr) return FGB_E_NULL;
+  if (c->dtype != FGB_F16 && c->dtype != FGB_BF16 && c->dtype != FGB_F32_TF32 && c->dtype != FGB_F32_IEEE) return FGB_E_DTYPE;
+  if (c->index_bits != 32 && c->index_bits != 64) return FGB_E_DTYPE;
+  if (c->n < 0 || c->n >= (int64_t(1) << 30) || c->rows < 1 || c->rows >= (int64_t(1) << 31) - 1 || c->c < 1 || c->c > 65536) return FGB_E_SIZE;
+  return FGB_OK;
+}
+
+template <typename T, int kVec>
+static cudaError_t emb_forward(const fgb_embedding_call& c, cudaStream_t s) {
+  const int width = std::min(c.c / kVec, kEmbThreads), lanes = kEmbThreads / width;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ceil_div(c.n, lanes * kEmbRows), int64_t(device_sm_count()) * 64));
+  const uint32_t n = static_cast<uint32_t>(c.n), rows = static_cast<uint32_t>(c.rows);
+  const T* table = static_cast<const T*>(c.table);
+  T* out = static_cast<T*>(c.out);
+  int32_t* mirror = status_mirror(c.status);
+  const int wide = c.index_bits == 64;
+  return c.scale == 1.f ? launch_chained(embedding_kernel<T, kVec, false>, dim3(grid), dim3(kEmbThreads), 0, s, c.indices, wide, table, out, n, rows, c.c,
+                                         c.scale, c.status, mirror)
+                        : launch_chained(embedding_kernel<T, kVec, true>, dim3(grid), dim3(kEmbThreads), 0, s, c.indices, wide, table, out, n, rows, c.c,
+                                         c.scale, c.status, mirror);
+}
+
+template <typename T, int kVec>
+static cudaError_t emb_sum(const EmbGrad& a, const EmbPlan& p, cudaStream_t s) {
+  const uint32_t per_cta = p.lanes * p.chunk;
+  const size_t smem = (2 * size_t(per_cta) + 2) * 4;
+  static PerDeviceTable configured;
+  if (ensure_dynamic_smem(configured, embedding_sum_kernel<T, kVec>, smem) != FGB_OK) return cudaErrorInvalidConfiguration;
+  LaunchErrors chain;
+  chain.add(launch_chained(embedding_sum_kernel<T, kVec>, dim3(static_cast<unsigned>(ceil_div(a.n, per_cta))), dim3(kEmbThreads), smem, s, a));
+  chain.add(launch_chained(embedding_join_kernel<T>, dim3(device_sm_count() * 4), dim3(kEmbThreads), 0, s, a));
+  return chain.first;
+}
+
+#define FGB_BY_PACK(T, vec, call)                                                       \
+  ((vec) * sizeof(T) == 16  ? call<T, 16 / sizeof(T)>                                   \
+   : (vec) * sizeof(T) == 8 ? call<T, 8 / sizeof(T)>                                    \
+   : (vec) == 2             ? call<T, 2>                                                \
+                            : call<T, 1>)
+
+}  // namespace fgb
+
+extern "C" int fgb_embedding_forward(const fgb_embedding_call* c, void* stream) {
+  using namespace fgb;
+  const int rc = emb_check(c);
+  if (rc != FGB_OK) return rc;
+  if (c->n == 0) return FGB_OK;
+  if (!c->indices || !c->table || !c->out) return FGB_E_NULL;
+  if ((reinterpret_cast<uintptr_t>(c->table) | reinterpret_cast<uintptr_t>(c->out)) & 15) return FGB_E_ALIGN;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int vec = row_pack(c->c, elem_bytes(c->dtype));
+  cudaError_t e;
+  if (c->dtype == FGB_F16) e = FGB_BY_PACK(__half, vec, emb_forward)(*c, s);
+  else if (c->dtype == FGB_BF16) e = FGB_BY_PACK(__nv_bfloat16, vec, emb_forward)(*c, s);
+  else e = FGB_BY_PACK(float, vec, emb_forward)(*c, s);
+  return e != cudaSuccess ? cuda_status(e) : launch_status();
+}
+
+extern "C" int64_t fgb_embedding_workspace_bytes(const fgb_embedding_call* c) {
+  using namespace fgb;
+  int rc = emb_check(c);
+  EmbPlan p;
+  if (rc == FGB_OK) rc = emb_plan(*c, p);
+  return rc != FGB_OK ? rc : static_cast<int64_t>(p.bytes);
+}
+
+extern "C" int fgb_embedding_backward(const fgb_embedding_call* c, void* stream) {
+  using namespace fgb;
+  int rc = emb_check(c);
+  if (rc != FGB_OK) return rc;
+  if (!c->grad_table || !c->workspace || (c->n > 0 && (!c->indices || !c->grad_out))) return FGB_E_NULL;
+  if ((reinterpret_cast<uintptr_t>(c->grad_out) | reinterpret_cast<uintptr_t>(c->grad_table)) & 15) return FGB_E_ALIGN;
+  if (reinterpret_cast<uintptr_t>(c->workspace) & 255) return FGB_E_ALIGN;
+  EmbPlan p;
+  rc = emb_plan(*c, p);
+  if (rc != FGB_OK) return rc;
+  if (c->workspace_bytes < static_cast<int64_t>(p.bytes)) return FGB_E_WORKSPACE;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(c->workspace);
+  int32_t* keys = reinterpret_cast<int32_t*>(ws + p.keys_off);
+  int64_t* order = reinterpret_cast<int64_t*>(ws + p.order_off);
+  uint32_t* cut = reinterpret_cast<uint32_t*>(ws + p.cut_off);
+  const uint32_t n = static_cast<uint32_t>(c->n), rows = static_cast<uint32_t>(c->rows);
+  const uint64_t halves = uint64_t(c->rows) * c->c * (elem_bytes(c->dtype) / 2);
+  const int64_t units = std::max<int64_t>(c->n, static_cast<int64_t>(halves / 8));
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(ceil_div(units, kEmbThreads), 1), int64_t(device_sm_count()) * 8));
+  cudaError_t e = launch_chained(embedding_keys_kernel, dim3(grid), dim3(kEmbThreads), 0, s, c->indices, c->index_bits == 64, n, rows, c->padding_idx, keys,
+                                 static_cast<uint16_t*>(c->grad_table), halves, cut, c->status, status_mirror(c->status));
+  if (e != cudaSuccess) return cuda_status(e);
+  if (n == 0) return launch_status();
+  int key_bits = 1;
+  while (key_bits < 31 && (rows >> key_bits) != 0u) ++key_bits;  // the largest key is `rows`
+  rc = fgb_pp_sorted_idx(keys, c->n, key_bits, order, ws + p.sort_off, static_cast<int64_t>(p.sort_bytes), c->status, stream);
+  if (rc != FGB_OK) return rc;
+  EmbGrad a{};
+  a.g = c->grad_out, a.grad = c->grad_table, a.keys = keys, a.order = order;
+  a.slab = reinterpret_cast<float*>(ws + p.slab_off), a.cut = cut;
+  a.n = n, a.rows = rows, a.chunk = p.chunk, a.chunks = p.chunks, a.C = c->c, a.scale = c->scale;
+  if (c->dtype == FGB_F16) e = FGB_BY_PACK(__half, p.vec, emb_sum)(a, p, s);
+  else if (c->dtype == FGB_BF16) e = FGB_BY_PACK(__nv_bfloat16, p.vec, emb_sum)(a, p, s);
+  else e = FGB_BY_PACK(float, p.vec, emb_sum)(a, p, s);
+  return e != cudaSuccess ? cuda_status(e) : launch_status();
+}

@@ -23,6 +23,7 @@
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -48,7 +49,9 @@ using torch::autograd::variable_list;
   X(fgb_bias_grad_workspace_bytes) X(fgb_subm_conv_bias_grad) X(fgb_subm_cache_scratch_bytes)                         \
   X(fgb_subm_cache_build) X(fgb_pp_valid_signal) X(fgb_hash_table_bytes)                                    \
   X(fgb_strided_grid_bytes) X(fgb_strided_mark) X(fgb_strided_build_bytes) X(fgb_strided_build)                       \
-  X(fgb_grid_sample_fused) X(fgb_indice_weighted_sum_grad_full_bytes) X(fgb_indice_weighted_sum_grad)
+  X(fgb_grid_sample_fused) X(fgb_indice_weighted_sum_grad_full_bytes) X(fgb_indice_weighted_sum_grad)                 \
+  X(fgb_sample_offsets) X(fgb_group_norm_workspace_bytes) X(fgb_group_norm_forward) X(fgb_group_norm_backward)        \
+  X(fgb_embedding_forward) X(fgb_embedding_workspace_bytes) X(fgb_embedding_backward)
 struct Api {
 #define X(f) decltype(&::f) f = nullptr;
   FGB_TORCH_API(X)
@@ -97,6 +100,8 @@ DeviceState& device_state(c10::DeviceIndex d) {
 [[noreturn]] void throw_soft_error(int code) {
   const char* what = code == FGB_S_TABLE_FULL     ? "hash table full (raise the hashmap ratio)"
                      : code == FGB_S_WAIT_TIMEOUT ? "a bounded barrier wait ran out inside a kernel"
+                     : code == FGB_S_BAD_OFFSETS  ? "row offsets or batch indices that do not ascend, or leave the rows"
+                     : code == FGB_S_BAD_INDEX    ? "an embedding index beyond the table"
                                                   : nullptr;
   throw std::runtime_error("flexgemm_b200 device-side error: " + (what != nullptr ? std::string(what) : "code " + std::to_string(code)));
 }
@@ -1150,6 +1155,255 @@ PyObject* py_sample_grad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   FGB_END
 }
 
+// ------------------------------------------------------------------ layers on ragged rows
+// Gradients that these nodes return have no history: differentiating them a second time is an error, not a silent zero.
+variable_list without_second_derivative(variable_list&& grads, const char* name) {
+  if (!at::GradMode::is_enabled()) return std::move(grads);
+  const std::string msg = std::string(name) + " has no second derivative";
+  for (Tensor& g : grads)
+    if (g.defined()) g.set_requires_grad(true);
+  return (*std::make_shared<torch::autograd::DelayedError>(msg, static_cast<int64_t>(grads.size())))(std::move(grads));
+}
+bool aligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0; }
+// [rows, ..., C] features as the kernels take them
+bool rows_arg_ok(const Tensor& t) {
+  return t.defined() && t.is_cuda() && t.layout() == at::kStrided && t.dim() >= 2 && t.numel() > 0 && t.is_contiguous() && aligned(t) &&
+         !t.is_neg() && dtype_code(t.scalar_type(), false) >= 0 && !has_tangent(t);
+}
+bool offsets_arg_ok(const Tensor& t, const Tensor& rows) {
+  return t.defined() && t.device() == rows.device() && t.dim() == 1 && t.size(0) >= 2 && t.is_contiguous() &&
+         (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong);
+}
+// gradient of an output: in the output's layout and type
+Tensor grad_rows(const Tensor& g, at::ScalarType dtype) {
+  Tensor r = (g.scalar_type() == dtype ? g : g.to(dtype)).contiguous();
+  return aligned(r) ? r : r.clone();
+}
+
+// --- group norm
+struct NormShape {
+  int64_t n = 0, samples = 0, groups = 0;
+  int act = 0;
+  float eps = 0.f;
+};
+fgb_group_norm_call norm_call(const Tensor& x, const Tensor& offsets, const Tensor& weight, const Tensor& bias, const Tensor& mean, const Tensor& rstd,
+                              const NormShape& k, DeviceState& ds) {
+  fgb_group_norm_call c{};
+  c.x = ptr(x);
+  c.offsets = offsets.defined() ? offsets.const_data_ptr() : nullptr;
+  c.offsets_bits = !offsets.defined() ? 0 : offsets.scalar_type() == at::kLong ? 64 : 32;
+  c.weight = weight.defined() ? ptr(weight) : nullptr, c.bias = bias.defined() ? ptr(bias) : nullptr;
+  c.mean = static_cast<float*>(mean.data_ptr()), c.rstd = static_cast<float*>(rstd.data_ptr());
+  c.n = k.n, c.samples = k.samples;
+  c.c = static_cast<int32_t>(x.size(-1)), c.groups = static_cast<int32_t>(k.groups);
+  c.dtype = dtype_code(x.scalar_type(), false);
+  c.param_dtype = weight.defined() ? dtype_code(weight.scalar_type(), false) : bias.defined() ? dtype_code(bias.scalar_type(), false) : c.dtype;
+  c.act = k.act, c.eps = k.eps;
+  c.status = static_cast<int32_t*>(ds.status.data_ptr());
+  return c;
+}
+
+struct GroupNormBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable x_, weight_, bias_, offsets_, mean_, rstd_;
+  NormShape shape;
+  std::string name() const override { return "SparseGroupNormBackward"; }
+  void release_variables() override {
+    for (auto* v : {&x_, &weight_, &bias_, &offsets_, &mean_, &rstd_}) v->reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(3);
+    if (!grads[0].defined()) return out;
+    const Tensor x = x_.unpack(), weight = weight_.unpack(), bias = bias_.unpack(), offsets = offsets_.unpack();
+    const Tensor mean = mean_.unpack(), rstd = rstd_.unpack();
+    const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1) && weight.defined(),
+               need_b = task_should_compute_output(2) && bias.defined();
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      c10::cuda::CUDAGuard guard(x.device());
+      const auto stream = c10::cuda::getCurrentCUDAStream(x.device().index());
+      DeviceState& ds = device_state(x.device().index());
+      poll(ds, stream);
+      const Tensor g = grad_rows(grads[0], x.scalar_type());
+      fgb_group_norm_call c = norm_call(x, offsets, weight, bias, mean, rstd, shape, ds);
+      c.grad_out = ptr(g);
+      if (need_x) out[0] = new_tensor(x.sizes(), x.scalar_type(), x.device()), c.out = out[0].data_ptr();
+      if (need_w) out[1] = new_tensor(weight.sizes(), weight.scalar_type(), x.device()), c.grad_weight = out[1].data_ptr();
+      if (need_b) out[2] = new_tensor(bias.sizes(), bias.scalar_type(), x.device()), c.grad_bias = out[2].data_ptr();
+      c.workspace_bytes = check_bytes(api.fgb_group_norm_workspace_bytes(&c), "fgb_group_norm_workspace_bytes");
+      const c10::DataPtr ws = scratch(c.workspace_bytes);
+      c.workspace = ws.get();
+      if (need_x || need_w || need_b) check(api.fgb_group_norm_backward(&c, stream), "fgb_group_norm_backward");
+    }
+    return without_second_derivative(std::move(out), "sparse_group_norm");
+  }
+};
+
+// (feats, offsets or None, groups, weight, bias, eps, silu) -> out or None
+PyObject* py_group_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  FGB_TRY
+  TORCH_CHECK(n_args == 7, "group_norm takes 7 arguments");
+  const Tensor x = tensor_arg(a[0]), offsets = tensor_arg(a[1]), weight = tensor_arg(a[3]), bias = tensor_arg(a[4]);
+  NormShape k;
+  k.groups = PyLong_AsLongLong(a[2]);
+  k.eps = static_cast<float>(PyFloat_AsDouble(a[5]));
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  k.act = PyObject_IsTrue(a[6]) == 1 ? FGB_ACT_SILU : FGB_ACT_NONE;
+  if (!rows_arg_ok(x) || (a[1] != Py_None && (x.dim() != 2 || !offsets_arg_ok(offsets, x)))) Py_RETURN_NONE;
+  const int64_t C = x.size(-1);
+  k.n = x.numel() / C;
+  k.samples = a[1] != Py_None ? offsets.size(0) - 1 : x.dim() == 2 ? 1 : x.size(0);
+  if (k.groups < 1 || C % k.groups != 0 || C > 65536 || k.n >= (int64_t(1) << 31) || k.samples >= (int64_t(1) << 24) || !(k.eps >= 0.f)) Py_RETURN_NONE;
+  for (int i : {3, 4}) {
+    const Tensor& t = i == 3 ? weight : bias;
+    if (a[i] == Py_None) continue;
+    if (!t.defined() || t.device() != x.device() || t.dim() != 1 || t.size(0) != C || !t.is_contiguous() || t.is_neg() || has_tangent(t) ||
+        (t.scalar_type() != x.scalar_type() && t.scalar_type() != at::kFloat))
+      Py_RETURN_NONE;
+  }
+  if (weight.defined() && bias.defined() && weight.scalar_type() != bias.scalar_type()) Py_RETURN_NONE;
+  const bool want_grad = torch::autograd::compute_requires_grad(x, weight, bias);
+  c10::cuda::CUDAGuard guard(x.device());
+  const auto stream = c10::cuda::getCurrentCUDAStream(x.device().index());
+  DeviceState& ds = device_state(x.device().index());
+  poll(ds, stream);
+  Tensor out, mean, rstd;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = new_tensor(x.sizes(), x.scalar_type(), x.device());
+    mean = new_tensor({k.samples, k.groups}, at::kFloat, x.device());
+    rstd = new_tensor({k.samples, k.groups}, at::kFloat, x.device());
+    fgb_group_norm_call c = norm_call(x, offsets, weight, bias, mean, rstd, k, ds);
+    c.out = out.data_ptr();
+    c.workspace_bytes = check_bytes(api.fgb_group_norm_workspace_bytes(&c), "fgb_group_norm_workspace_bytes");
+    const c10::DataPtr ws = scratch(c.workspace_bytes);
+    c.workspace = ws.get();
+    check(api.fgb_group_norm_forward(&c, stream), "fgb_group_norm_forward");
+  }
+  if (want_grad) {
+    std::shared_ptr<GroupNormBackward> node(new GroupNormBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, weight, bias));
+    using torch::autograd::SavedVariable;
+    node->x_ = SavedVariable(x, false);
+    if (weight.defined()) node->weight_ = SavedVariable(weight, false);
+    if (bias.defined()) node->bias_ = SavedVariable(bias, false);
+    if (offsets.defined()) node->offsets_ = SavedVariable(offsets, false);
+    node->mean_ = SavedVariable(mean, false), node->rstd_ = SavedVariable(rstd, false);
+    node->shape = k;
+    torch::autograd::set_history(out, node);
+  }
+  return THPVariable_Wrap(out);
+  FGB_END
+}
+
+// (coords [N, 4], batch) -> offsets [batch + 1] or None
+PyObject* py_sample_offsets(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  FGB_TRY
+  TORCH_CHECK(n_args == 2, "sample_offsets takes 2 arguments");
+  const Tensor coords = tensor_arg(a[0]);
+  const int64_t batch = PyLong_AsLongLong(a[1]);
+  if (batch == -1 && PyErr_Occurred()) return nullptr;
+  if (!coords.defined() || !coords.is_cuda() || coords.scalar_type() != at::kInt || coords.dim() != 2 || coords.size(1) != 4 || !coords.is_contiguous() ||
+      (coords.numel() > 0 && !aligned(coords)) || batch < 1 || batch >= (int64_t(1) << 24))
+    Py_RETURN_NONE;
+  c10::cuda::CUDAGuard guard(coords.device());
+  const auto stream = c10::cuda::getCurrentCUDAStream(coords.device().index());
+  DeviceState& ds = device_state(coords.device().index());
+  poll(ds, stream);
+  Tensor out = new_tensor({batch + 1}, at::kInt, coords.device());
+  check(api.fgb_sample_offsets(cptr<int32_t>(coords), coords.size(0), batch, static_cast<int32_t*>(out.data_ptr()),
+                               static_cast<int32_t*>(ds.status.data_ptr()), stream),
+        "fgb_sample_offsets");
+  return THPVariable_Wrap(out);
+  FGB_END
+}
+
+// --- embedding
+fgb_embedding_call embedding_call(const Tensor& indices, int64_t rows, int64_t C, at::ScalarType dtype, float scale, int64_t padding, DeviceState& ds) {
+  fgb_embedding_call c{};
+  c.indices = ptr(indices);
+  c.n = indices.numel(), c.rows = rows, c.c = static_cast<int32_t>(C);
+  c.index_bits = indices.scalar_type() == at::kLong ? 64 : 32;
+  c.padding_idx = padding, c.scale = scale, c.dtype = dtype_code(dtype, false);
+  c.status = static_cast<int32_t*>(ds.status.data_ptr());
+  return c;
+}
+
+struct EmbeddingBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable indices_;
+  std::vector<int64_t> table;
+  at::ScalarType dtype = at::kFloat;
+  float scale = 1.f;
+  int64_t padding = -1;
+  std::string name() const override { return "SparseEmbeddingBackward"; }
+  void release_variables() override { indices_.reset_data(); }
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(1);
+    if (!grads[0].defined() || !task_should_compute_output(0)) return out;
+    const Tensor indices = indices_.unpack();
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      c10::cuda::CUDAGuard guard(indices.device());
+      const auto stream = c10::cuda::getCurrentCUDAStream(indices.device().index());
+      DeviceState& ds = device_state(indices.device().index());
+      poll(ds, stream);
+      const Tensor g = grad_rows(grads[0], dtype);
+      out[0] = new_tensor(table, dtype, indices.device());
+      fgb_embedding_call c = embedding_call(indices, table[0], table[1], dtype, scale, padding, ds);
+      c.grad_out = ptr(g), c.grad_table = out[0].data_ptr();
+      c.workspace_bytes = check_bytes(api.fgb_embedding_workspace_bytes(&c), "fgb_embedding_workspace_bytes");
+      const c10::DataPtr ws = scratch(c.workspace_bytes);
+      c.workspace = ws.get();
+      check(api.fgb_embedding_backward(&c, stream), "fgb_embedding_backward");
+    }
+    return without_second_derivative(std::move(out), "sparse_embedding");
+  }
+};
+
+// (indices, table, scale, padding index or -1) -> [*indices, C] or None
+PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  FGB_TRY
+  TORCH_CHECK(n_args == 4, "embedding takes 4 arguments");
+  const Tensor indices = tensor_arg(a[0]), table = tensor_arg(a[1]);
+  const float scale = static_cast<float>(PyFloat_AsDouble(a[2]));
+  const int64_t padding = PyLong_AsLongLong(a[3]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  if (!rows_arg_ok(table) || table.dim() != 2 || table.size(1) > 65536 || table.size(0) >= (int64_t(1) << 31) - 1 || !indices.defined() ||
+      indices.device() != table.device() || (indices.scalar_type() != at::kInt && indices.scalar_type() != at::kLong) || !indices.is_contiguous() ||
+      indices.numel() == 0 || indices.numel() >= (int64_t(1) << 30) || padding < -1 || padding >= table.size(0))
+    Py_RETURN_NONE;
+  const bool want_grad = torch::autograd::compute_requires_grad(table);
+  c10::cuda::CUDAGuard guard(table.device());
+  const auto stream = c10::cuda::getCurrentCUDAStream(table.device().index());
+  DeviceState& ds = device_state(table.device().index());
+  poll(ds, stream);
+  std::vector<int64_t> size(indices.sizes().begin(), indices.sizes().end());
+  size.push_back(table.size(1));
+  Tensor out;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = new_tensor(size, table.scalar_type(), table.device());
+    fgb_embedding_call c = embedding_call(indices, table.size(0), table.size(1), table.scalar_type(), scale, padding, ds);
+    c.table = ptr(table), c.out = out.data_ptr();
+    check(api.fgb_embedding_forward(&c, stream), "fgb_embedding_forward");
+  }
+  if (want_grad) {
+    std::shared_ptr<EmbeddingBackward> node(new EmbeddingBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(table));
+    node->indices_ = torch::autograd::SavedVariable(indices, false);
+    node->table = table.sizes().vec(), node->dtype = table.scalar_type();
+    node->scale = scale, node->padding = padding;
+    torch::autograd::set_history(out, node);
+  }
+  return THPVariable_Wrap(out);
+  FGB_END
+}
+
 PyObject* py_status_word(PyObject*, PyObject* index) {
   FGB_TRY
   return THPVariable_Wrap(device_state(static_cast<c10::DeviceIndex>(PyLong_AsLong(index))).status);
@@ -1204,6 +1458,9 @@ PyMethodDef methods[] = {
     {"strided_conv", FAST(py_strided_conv), "strided conv"},
     {"grid_sample", FAST(py_grid_sample), "sparse grid sample"},
     {"sample_grad", FAST(py_sample_grad), "gradient of a weighted gather"},
+    {"group_norm", FAST(py_group_norm), "group norm with an activation on ragged rows"},
+    {"sample_offsets", FAST(py_sample_offsets), "row ranges of the samples of coordinate rows"},
+    {"embedding", FAST(py_embedding), "scaled rows of a table"},
     {"status_word", py_status_word, METH_O, "device status word"},
     {"poll", py_poll, METH_O, "raise a soft error that the device has reported"},
     {"clear_mirror", py_clear_mirror, METH_O, "forget the host copy of the status word"},

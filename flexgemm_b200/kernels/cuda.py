@@ -286,7 +286,9 @@ def fetch_meta_async(meta: torch.Tensor):
 def raise_for_status(code: int) -> None:
     if code != 0:
         what = {_cabi.S_TABLE_FULL: "hash table full (raise the hashmap ratio)",
-                _cabi.S_WAIT_TIMEOUT: "a bounded barrier wait ran out inside a kernel"}.get(code, f"code {code}")
+                _cabi.S_WAIT_TIMEOUT: "a bounded barrier wait ran out inside a kernel",
+                _cabi.S_BAD_OFFSETS: "row offsets or batch indices that do not ascend, or leave the rows",
+                _cabi.S_BAD_INDEX: "an embedding index beyond the table"}.get(code, f"code {code}")
         raise RuntimeError(f"flexgemm_b200 device-side error: {what}")
 
 

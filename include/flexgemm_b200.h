@@ -39,6 +39,8 @@ extern "C" {
 /* device-side status codes (written to *status) */
 #define FGB_S_TABLE_FULL 1    /* hash insert found no free slot        */
 #define FGB_S_WAIT_TIMEOUT 2  /* a bounded barrier wait ran out        */
+#define FGB_S_BAD_OFFSETS 3   /* row ranges or batch indices that do not ascend, or leave the rows */
+#define FGB_S_BAD_INDEX 4     /* an index beyond the table             */
 
 /* element types of features / weights */
 #define FGB_F16 0
@@ -712,6 +714,77 @@ int fgb_wgrad_call_run(const fgb_wgrad_call* call, void* stream);
  * 16-byte pieces are padded on the way into the conv calls and cut on the way
  * out.)  Widths must be multiples of 2. */
 int fgb_resize_rows(const void* src, void* dst, int64_t rows_in, int64_t rows_out, int64_t width_in, int64_t width_out, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Layers on ragged rows (no counterpart in the reference)
+ *
+ * Rows [n, C] of `samples` samples (or experts): those of sample s are
+ * offsets[s] .. offsets[s + 1] - 1, with `samples` + 1 ascending entries in
+ * [0, n] on the device.  Rows before the first or behind the last of these
+ * ranges belong to no sample: outputs and gradients have zeros there, and what
+ * the inputs hold there counts for nothing.  Offsets that do not ascend or
+ * leave the rows record FGB_S_BAD_OFFSETS; the results are void then.
+ * --------------------------------------------------------------------- */
+
+/* offsets [batch + 1] (int32) of the samples of coordinate rows (b, x, y, z)
+ * that are grouped by ascending b, as the convolutions take and give them.
+ * coords: int32 [n, 4], 16-byte aligned. */
+int fgb_sample_offsets(const int32_t* coords, int64_t n, int64_t batch, int32_t* offsets, int32_t* status, void* stream);
+
+/* Group norm, channels last: with mean m and variance v over the rows of a
+ * sample and the c / groups channels of a group,
+ *   y = act((x - m) / sqrt(v + eps) * weight + bias).
+ * Sums and statistics are fp32 or wider; y is rounded once. */
+typedef struct fgb_group_norm_call {
+  const void* x;          /* [n, c], 16-byte aligned like every [n, c] here */
+  const void* grad_out;   /* backward: [n, c] */
+  void* out;              /* forward: y; backward: the gradient of x, or null */
+  const void* offsets;    /* [samples + 1]; unused with offsets_bits = 0 */
+  const void* weight;     /* [c] or null (ones) */
+  const void* bias;       /* [c] or null (zeros) */
+  float* mean;            /* [samples, groups]: written by the forward call, read by the backward one */
+  float* rstd;            /* [samples, groups]: 1 / sqrt(v + eps), likewise */
+  void* grad_weight;      /* backward: [c] or null */
+  void* grad_bias;        /* backward: [c] or null */
+  int64_t n, samples;     /* n < 2^31, samples < 2^24 */
+  int32_t offsets_bits;   /* 32, 64, or 0: `samples` ranges of n / samples rows */
+  int32_t c, groups;
+  int32_t dtype;          /* of x, y and their gradients */
+  int32_t param_dtype;    /* of weight, bias and their gradients: dtype, or FGB_F32_IEEE */
+  int32_t act;            /* FGB_ACT_* */
+  float eps;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status;
+} fgb_group_norm_call;
+int64_t fgb_group_norm_workspace_bytes(const fgb_group_norm_call* call);
+int fgb_group_norm_forward(const fgb_group_norm_call* call, void* stream);
+int fgb_group_norm_backward(const fgb_group_norm_call* call, void* stream);
+
+/* Embedding: out[i] = scale * table[indices[i]] (fp32 product, rounded once).
+ * Gradient: grad_table[v] = scale * sum of grad_out[i] over the i with
+ * indices[i] = v, for v != padding_idx (zero there; -1: no padding index); the
+ * rows of an index are added in fp32 in the order of i, cut at fixed places, so
+ * the result does not depend on the run.  An index outside [0, rows) gives a
+ * row of zeros, adds nothing, and records FGB_S_BAD_INDEX. */
+typedef struct fgb_embedding_call {
+  const void* indices;    /* [n], index_bits wide */
+  const void* table;      /* forward: [rows, c] */
+  void* out;              /* forward: [n, c] */
+  const void* grad_out;   /* backward: [n, c] */
+  void* grad_table;       /* backward: [rows, c] */
+  int64_t n, rows;        /* n < 2^30, rows < 2^31 */
+  int64_t padding_idx;
+  int32_t index_bits;     /* 32 or 64 */
+  int32_t c, dtype;
+  float scale;
+  void* workspace;        /* backward only */
+  int64_t workspace_bytes;
+  int32_t* status;
+} fgb_embedding_call;
+int fgb_embedding_forward(const fgb_embedding_call* call, void* stream);
+int64_t fgb_embedding_workspace_bytes(const fgb_embedding_call* call);
+int fgb_embedding_backward(const fgb_embedding_call* call, void* stream);
 
 /* ------------------------------------------------------------------------
  * Pipeline microbenchmark (no counterpart in the reference)

@@ -1,0 +1,155 @@
+"""CPU-side checks of the layers on ragged rows: their oracle against torch's autograd, and what the calls and the C entry
+points refuse before anything is launched."""
+import ctypes
+
+import pytest
+import torch
+
+from flexgemm_b200 import _build, _cabi
+from oracle import rows_oracle as orc
+
+
+@pytest.fixture(scope="module")
+def lib():
+    _build.build()
+    return _cabi.lib()
+
+
+def test_oracle_group_norm_is_torchs():
+    g = torch.Generator().manual_seed(1)
+    x, dy = (torch.randn(31, 12, generator=g, dtype=torch.float64) for _ in range(2))
+    w, b = (torch.randn(12, generator=g, dtype=torch.float64) for _ in range(2))
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    parts = [torch.nn.functional.silu(torch.nn.functional.group_norm(leaves[0][lo:hi].T.unsqueeze(0), 3, leaves[1], leaves[2], 1e-3)[0].T)
+             for lo, hi in ((0, 9), (9, 31))]
+    y = torch.cat(parts)
+    grads = torch.autograd.grad(y, leaves, dy)
+    ref = orc.group_norm(x, [(0, 9), (9, 9), (9, 31)], 3, w, b, 1e-3, True, dy)
+    for got, want in ((ref["y"], y), (ref["dx"], grads[0]), (ref["dw"], grads[1]), (ref["db"], grads[2])):
+        assert torch.allclose(got, want, rtol=1e-10, atol=1e-12)
+
+
+def test_oracle_embedding_is_torchs():
+    g = torch.Generator().manual_seed(2)
+    idx = torch.randint(0, 7, (40,), generator=g)
+    table = torch.randn(7, 5, generator=g, dtype=torch.float64).requires_grad_(True)
+    dy = torch.randn(40, 5, generator=g, dtype=torch.float64)
+    out = torch.nn.functional.embedding(idx, table, padding_idx=3) * 2.5
+    (want,) = torch.autograd.grad(out, [table], dy)
+    assert torch.equal(orc.embedding(idx, table.detach(), 2.5), out.detach())
+    got, size = orc.embedding_grad(idx, dy, 7, 2.5, padding=3)
+    assert torch.allclose(got, want, rtol=1e-12, atol=1e-12) and (size >= got.abs() - 1e-12).all()
+
+
+def test_group_norm_refuses(lib):
+    from flexgemm_b200.ops.group_norm import sparse_group_norm
+    x, off = torch.randn(10, 8), torch.tensor([0, 4, 10])
+    with pytest.raises(NotImplementedError):
+        sparse_group_norm(x, off, 4)
+    for bad in (0, 3, -2, 2.0, None):
+        with pytest.raises(ValueError):
+            sparse_group_norm(x, off, bad)
+    with pytest.raises(ValueError):
+        sparse_group_norm(x, off, 4, activation="gelu")
+    for eps in (-1e-5, float("nan")):
+        with pytest.raises(ValueError):
+            sparse_group_norm(x, off, 4, eps=eps)
+    for shape in ((8,), (2, 5, 8)):
+        with pytest.raises(AssertionError):
+            sparse_group_norm(torch.randn(shape), off, 4)
+    with pytest.raises(TypeError):
+        sparse_group_norm(x.double(), off, 4)
+    with pytest.raises(TypeError):
+        sparse_group_norm(x, off.float(), 4)
+    for bad in (torch.tensor([0]), torch.zeros(2, 2, dtype=torch.int64)):
+        with pytest.raises(AssertionError):
+            sparse_group_norm(x, bad, 4)
+    for bad in (torch.ones(7), torch.ones(1, 8)):
+        with pytest.raises(AssertionError):
+            sparse_group_norm(x, off, 4, bad)
+        with pytest.raises(AssertionError):
+            sparse_group_norm(x, off, 4, None, bad)
+    with pytest.raises(TypeError):
+        sparse_group_norm(x, off, 4, torch.ones(8).half())
+    with pytest.raises(TypeError):
+        sparse_group_norm(x.half(), off, 4, torch.ones(8).half(), torch.ones(8))
+
+
+def test_embedding_refuses(lib):
+    from flexgemm_b200.ops.embedding import sparse_embedding
+    table, idx = torch.randn(10, 8), torch.tensor([1, 2])
+    with pytest.raises(NotImplementedError):
+        sparse_embedding(idx, table)
+    with pytest.raises(AssertionError):
+        sparse_embedding(idx, table[0])
+    for bad in (idx.float(), idx.to(torch.int16), idx.bool()):
+        with pytest.raises(TypeError):
+            sparse_embedding(bad, table)
+    with pytest.raises(TypeError):
+        sparse_embedding(idx, table.double())
+    for bad in (10, -1, -11):
+        with pytest.raises(ValueError):
+            sparse_embedding(idx, table, padding_idx=bad)
+    for bad in (torch.randn(0, 8), torch.randn(3, 0)):
+        with pytest.raises(ValueError):
+            sparse_embedding(idx, bad)
+
+
+def test_sample_offsets_refuses(lib):
+    from flexgemm_b200.ops.utils import sample_offsets
+    c = torch.zeros(5, 4, dtype=torch.int32)
+    with pytest.raises(NotImplementedError):
+        sample_offsets(c, 1)
+    with pytest.raises(AssertionError):
+        sample_offsets(c[:, :3], 1)
+    for bad in (0, -1, 2 ** 24):
+        with pytest.raises(ValueError):
+            sample_offsets(c, bad)
+
+
+class NormCall(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in ("x", "grad_out", "out", "offsets", "weight", "bias", "mean", "rstd", "grad_weight", "grad_bias")] + \
+               [("n", ctypes.c_int64), ("samples", ctypes.c_int64)] + \
+               [(k, ctypes.c_int32) for k in ("offsets_bits", "c", "groups", "dtype", "param_dtype", "act")] + \
+               [("eps", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("status", ctypes.c_void_p)]
+
+
+def test_group_norm_entry_points_refuse(lib):
+    """Pointers are numbers here: every call is refused before a launch."""
+    good = dict(x=1 << 20, out=1 << 21, offsets=1 << 22, mean=1 << 23, rstd=1 << 23, n=100, samples=3, offsets_bits=32, c=64, groups=8,
+                dtype=_cabi.F16, param_dtype=_cabi.F16, act=0, eps=1e-5, workspace=1 << 24, workspace_bytes=1 << 40)
+
+    def rc(fn=lib.fgb_group_norm_forward, **kw):
+        call = NormCall(**{**good, **kw})
+        return fn(ctypes.byref(call), None)
+    assert lib.fgb_group_norm_workspace_bytes(ctypes.byref(NormCall(**good))) > 0
+    assert lib.fgb_group_norm_workspace_bytes(None) == -1 and lib.fgb_group_norm_forward(None, None) == -1
+    for kw, code in ((dict(dtype=9), -3), (dict(param_dtype=_cabi.BF16), -3), (dict(act=7), -3), (dict(offsets_bits=16), -3), (dict(n=-1), -2),
+                     (dict(n=1 << 31), -2), (dict(samples=0), -2), (dict(samples=1 << 24), -2), (dict(groups=7), -2), (dict(c=0), -2),
+                     (dict(offsets_bits=0), -2), (dict(samples=(1 << 24) - 1, c=65536, groups=65536), -2), (dict(offsets=None), -1), (dict(x=None), -1), (dict(out=None), -1),
+                     (dict(mean=None), -1), (dict(workspace=None), -1), (dict(x=(1 << 20) + 8), -4), (dict(workspace=(1 << 24) + 16), -4), (dict(workspace_bytes=10), -5)):
+        assert rc(**kw) == code, kw
+    assert rc(lib.fgb_group_norm_backward) == -1   # no grad_out
+
+
+class EmbeddingCall(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in ("indices", "table", "out", "grad_out", "grad_table")] + \
+               [(k, ctypes.c_int64) for k in ("n", "rows", "padding_idx")] + [(k, ctypes.c_int32) for k in ("index_bits", "c", "dtype")] + \
+               [("scale", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("status", ctypes.c_void_p)]
+
+
+def test_embedding_entry_points_refuse(lib):
+    good = dict(indices=1 << 20, table=1 << 21, out=1 << 22, grad_out=1 << 22, grad_table=1 << 23, n=100, rows=30, padding_idx=-1, index_bits=32, c=64,
+                dtype=_cabi.BF16, scale=1.0, workspace=1 << 24, workspace_bytes=1 << 40)
+
+    def rc(fn, **kw):
+        return fn(ctypes.byref(EmbeddingCall(**{**good, **kw})), None)
+    assert lib.fgb_embedding_workspace_bytes(ctypes.byref(EmbeddingCall(**good))) > 0
+    for fn in (lib.fgb_embedding_forward, lib.fgb_embedding_backward):
+        assert fn(None, None) == -1
+        for kw, code in ((dict(dtype=5), -3), (dict(index_bits=8), -3), (dict(n=1 << 30), -2), (dict(n=-1), -2), (dict(rows=0), -2), (dict(c=0), -2),
+                         (dict(rows=2 ** 31 - 1), -2), (dict(indices=None), -1)):
+            assert rc(fn, **kw) == code, kw
+    assert rc(lib.fgb_embedding_forward, table=None) == -1 and rc(lib.fgb_embedding_forward, out=(1 << 22) + 2) == -4
+    assert rc(lib.fgb_embedding_backward, grad_out=None) == -1 and rc(lib.fgb_embedding_backward, workspace_bytes=64) == -5
+    assert rc(lib.fgb_embedding_backward, workspace=(1 << 24) + 8) == -4 and rc(lib.fgb_embedding_forward, n=0) == 0
