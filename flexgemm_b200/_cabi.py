@@ -96,6 +96,10 @@ _PROTOTYPES = {
     "fgb_embedding_forward": (c_int, [_P, _P]),
     "fgb_embedding_workspace_bytes": (c_int64, [_P]),
     "fgb_embedding_backward": (c_int, [_P, _P]),
+    "fgb_grouped_linear_max_groups": (c_int, []),
+    "fgb_grouped_linear_workspace_bytes": (c_int64, [_P, c_int]),
+    "fgb_grouped_linear_forward": (c_int, [_P, _P]),
+    "fgb_grouped_linear_backward": (c_int, [_P, _P]),
     "fgb_noalloc_max_channels": (c_int, []),
     "fgb_subm_conv_bias_grad_noalloc": (c_int, [_P, _P, _P, c_int64, c_int, c_int, _P]),
 }

@@ -767,6 +767,21 @@ int make_rows_tmap(CUtensorMap* map, const void* rows, int64_t n_rows, int row_e
   });
 }
 
+// 3-D map over 16-bit elements [d2][d1][d0] (d0 a multiple of 8); box = b0 x b1 x 1, 128B swizzle
+int make_rows_tmap_3d(CUtensorMap* map, const void* base, int dtype16, uint64_t d0, uint64_t d1, uint64_t d2, uint32_t b0, uint32_t b1) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return FGB_E_DRIVER;
+  const CUtensorMapDataType dt = dtype16 == FGB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  cuuint64_t dims[3] = {d0, d1, d2};
+  cuuint64_t strides[2] = {d0 * 2, d0 * d1 * 2};
+  cuuint32_t box[3] = {b0, b1, 1u};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return encode_tmap([&] {
+    return fn(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
+}
+
 // Output channels per work item: all of them in steps of 32 up to 256, else as many equal column tiles as 256-wide ones
 // would make, in steps of 64 (the epilogue writes 64 columns of a 16-bit type at a time).  The width sets the weight
 // bytes and the MMA time of a stage: powers of two ran C = 136 like 256 and C = 312 like 512.

@@ -51,7 +51,9 @@ using torch::autograd::variable_list;
   X(fgb_strided_grid_bytes) X(fgb_strided_mark) X(fgb_strided_build_bytes) X(fgb_strided_build)                       \
   X(fgb_grid_sample_fused) X(fgb_indice_weighted_sum_grad_full_bytes) X(fgb_indice_weighted_sum_grad)                 \
   X(fgb_sample_offsets) X(fgb_group_norm_workspace_bytes) X(fgb_group_norm_forward) X(fgb_group_norm_backward)        \
-  X(fgb_embedding_forward) X(fgb_embedding_workspace_bytes) X(fgb_embedding_backward)
+  X(fgb_embedding_forward) X(fgb_embedding_workspace_bytes) X(fgb_embedding_backward)                                 \
+  X(fgb_grouped_linear_max_groups) X(fgb_grouped_linear_workspace_bytes) X(fgb_grouped_linear_forward)                \
+  X(fgb_grouped_linear_backward)
 struct Api {
 #define X(f) decltype(&::f) f = nullptr;
   FGB_TORCH_API(X)
@@ -1404,6 +1406,95 @@ PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   FGB_END
 }
 
+// --- products grouped by row ranges
+fgb_grouped_linear_call grouped_call(const Tensor& x, const Tensor& offsets, const Tensor& weight, int dtype, DeviceState& ds) {
+  fgb_grouped_linear_call c{};
+  c.x = ptr(x), c.weight = ptr(weight), c.offsets = offsets.const_data_ptr();
+  c.offsets_bits = offsets.scalar_type() == at::kLong ? 64 : 32;
+  c.n = x.size(0), c.groups = weight.size(0);
+  c.ci = static_cast<int32_t>(weight.size(2)), c.co = static_cast<int32_t>(weight.size(1));
+  c.dtype = dtype;
+  c.status = static_cast<int32_t*>(ds.status.data_ptr());
+  return c;
+}
+
+struct GroupedLinearBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable x_, offsets_, weight_;
+  bool bias = false;
+  std::string name() const override { return "SparseGroupedLinearBackward"; }
+  void release_variables() override {
+    for (auto* v : {&x_, &offsets_, &weight_}) v->reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(3);
+    if (!grads[0].defined()) return out;
+    const Tensor x = x_.unpack(), offsets = offsets_.unpack(), weight = weight_.unpack();
+    const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1), need_b = bias && task_should_compute_output(2);
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      c10::cuda::CUDAGuard guard(x.device());
+      const auto stream = c10::cuda::getCurrentCUDAStream(x.device().index());
+      DeviceState& ds = device_state(x.device().index());
+      poll(ds, stream);
+      const at::ScalarType t = x.scalar_type();
+      const Tensor g = grad_rows(grads[0], t);
+      fgb_grouped_linear_call c = grouped_call(x, offsets, weight, dtype_code(t, *g_allow_tf32 != 0), ds);
+      c.grad_out = ptr(g);
+      Tensor gw;  // the bias gradient comes out of the weight gradient's pass
+      if (need_x) out[0] = new_tensor(x.sizes(), t, x.device()), c.grad_x = out[0].data_ptr();
+      if (need_w || need_b) gw = new_tensor(weight.sizes(), t, x.device()), c.grad_weight = gw.data_ptr();
+      if (need_b) out[2] = new_tensor({weight.size(0), weight.size(1)}, t, x.device()), c.grad_bias = out[2].data_ptr();
+      if (need_w) out[1] = gw;
+      c.workspace_bytes = check_bytes(api.fgb_grouped_linear_workspace_bytes(&c, 1), "fgb_grouped_linear_workspace_bytes");
+      const c10::DataPtr ws = scratch(c.workspace_bytes);
+      c.workspace = ws.get();
+      check(api.fgb_grouped_linear_backward(&c, stream), "fgb_grouped_linear_backward");
+    }
+    return without_second_derivative(std::move(out), "sparse_grouped_linear");
+  }
+};
+
+// (feats, offsets, weight, bias, tf32) -> [N, Co] or None
+PyObject* py_grouped_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  FGB_TRY
+  TORCH_CHECK(n_args == 5, "grouped_linear takes 5 arguments");
+  const Tensor x = tensor_arg(a[0]), offsets = tensor_arg(a[1]), weight = tensor_arg(a[2]), bias = tensor_arg(a[3]);
+  if (!rows_arg_ok(x) || x.dim() != 2 || !rows_arg_ok(weight) || weight.dim() != 3 || weight.device() != x.device() ||
+      weight.scalar_type() != x.scalar_type() || weight.size(2) != x.size(1) || weight.size(1) > 65536 || weight.size(2) > 65536 ||
+      weight.size(0) > api.fgb_grouped_linear_max_groups() || x.size(0) >= (int64_t(1) << 31) - 256 || !offsets_arg_ok(offsets, x) ||
+      offsets.size(0) != weight.size(0) + 1)
+    Py_RETURN_NONE;
+  if (a[3] != Py_None && (!bias.defined() || bias.device() != x.device() || bias.scalar_type() != x.scalar_type() || bias.dim() != 2 ||
+                          bias.size(0) != weight.size(0) || bias.size(1) != weight.size(1) || !bias.is_contiguous() || bias.is_neg() || has_tangent(bias)))
+    Py_RETURN_NONE;
+  const bool want_grad = torch::autograd::compute_requires_grad(x, weight, bias);
+  c10::cuda::CUDAGuard guard(x.device());
+  const auto stream = c10::cuda::getCurrentCUDAStream(x.device().index());
+  DeviceState& ds = device_state(x.device().index());
+  poll(ds, stream);
+  Tensor out;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = new_tensor({x.size(0), weight.size(1)}, x.scalar_type(), x.device());
+    fgb_grouped_linear_call c = grouped_call(x, offsets, weight, dtype_code(x.scalar_type(), PyObject_IsTrue(a[4]) == 1), ds);
+    c.bias = bias.defined() ? ptr(bias) : nullptr, c.out = out.data_ptr();
+    c.workspace_bytes = check_bytes(api.fgb_grouped_linear_workspace_bytes(&c, 0), "fgb_grouped_linear_workspace_bytes");
+    const c10::DataPtr ws = scratch(c.workspace_bytes);
+    c.workspace = ws.get();
+    check(api.fgb_grouped_linear_forward(&c, stream), "fgb_grouped_linear_forward");
+  }
+  if (want_grad) {
+    std::shared_ptr<GroupedLinearBackward> node(new GroupedLinearBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, weight, bias));
+    using torch::autograd::SavedVariable;
+    node->x_ = SavedVariable(x, false), node->offsets_ = SavedVariable(offsets, false), node->weight_ = SavedVariable(weight, false);
+    node->bias = bias.defined();
+    torch::autograd::set_history(out, node);
+  }
+  return THPVariable_Wrap(out);
+  FGB_END
+}
+
 PyObject* py_status_word(PyObject*, PyObject* index) {
   FGB_TRY
   return THPVariable_Wrap(device_state(static_cast<c10::DeviceIndex>(PyLong_AsLong(index))).status);
@@ -1460,6 +1551,7 @@ PyMethodDef methods[] = {
     {"sample_grad", FAST(py_sample_grad), "gradient of a weighted gather"},
     {"group_norm", FAST(py_group_norm), "group norm with an activation on ragged rows"},
     {"sample_offsets", FAST(py_sample_offsets), "row ranges of the samples of coordinate rows"},
+    {"grouped_linear", FAST(py_grouped_linear), "products grouped by row ranges"},
     {"embedding", FAST(py_embedding), "scaled rows of a table"},
     {"status_word", py_status_word, METH_O, "device status word"},
     {"poll", py_poll, METH_O, "raise a soft error that the device has reported"},

@@ -67,8 +67,8 @@ def sparse_group_norm(feats: torch.Tensor, offsets: Optional[torch.Tensor], num_
         raise ValueError("at most 2^31 - 1 rows and 2^24 - 1 samples are supported")
     if feats.numel() == 0:
         return utils.zeros_with_history((tuple(feats.shape), feats.dtype, feats.device), feats, weight, bias)
-    out = _native.ext().group_norm(utils.kernel_layout(feats), offsets, num_groups, weight.contiguous() if weight is not None else None,
-                                   bias.contiguous() if bias is not None else None, float(eps), silu)
+    out = _native.ext().group_norm(utils.kernel_layout(feats), offsets, num_groups, weight.contiguous().resolve_neg() if weight is not None else None,
+                                   bias.contiguous().resolve_neg() if bias is not None else None, float(eps), silu)
     if out is None:
         raise ValueError("sparse_group_norm: arguments that the kernels do not take")
     return out

@@ -786,6 +786,38 @@ int fgb_embedding_forward(const fgb_embedding_call* call, void* stream);
 int64_t fgb_embedding_workspace_bytes(const fgb_embedding_call* call);
 int fgb_embedding_backward(const fgb_embedding_call* call, void* stream);
 
+/* Products grouped by row ranges: with `groups` ranges (offsets as above) and a
+ * matrix [co, ci] for each,
+ *   forward   out[r] = weight[g] x[r] + bias[g]           for the rows r of group g
+ *   backward  grad_x[r] = weight[g]^T grad_out[r]
+ *             grad_weight[g] = sum_r grad_out[r] x[r]^T,   grad_bias[g] = sum_r grad_out[r]
+ * fp32 accumulation, the bias added in fp32, one rounding.  fp32 data is
+ * multiplied as sums of bf16 planes: FGB_F32_IEEE six products (errors of some
+ * 2^-22 of a product), FGB_F32_TF32 three (2^-17); an infinity among fp32
+ * operands gives NaN.  Gradients that are null are not computed; grad_bias needs
+ * grad_weight.  groups <= fgb_grouped_linear_max_groups(). */
+typedef struct fgb_grouped_linear_call {
+  const void* x;           /* [n, ci] */
+  const void* weight;      /* [groups, co, ci] */
+  const void* bias;        /* [groups, co] or null */
+  const void* grad_out;    /* backward: [n, co] */
+  void* out;               /* forward: [n, co] */
+  void* grad_x;            /* backward: [n, ci] or null */
+  void* grad_weight;       /* backward: [groups, co, ci] or null */
+  void* grad_bias;         /* backward: [groups, co] or null */
+  const void* offsets;     /* [groups + 1] */
+  int64_t n, groups;
+  int32_t offsets_bits;    /* 32 or 64 */
+  int32_t ci, co, dtype;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status;
+} fgb_grouped_linear_call;
+int fgb_grouped_linear_max_groups(void);
+int64_t fgb_grouped_linear_workspace_bytes(const fgb_grouped_linear_call* call, int backward);
+int fgb_grouped_linear_forward(const fgb_grouped_linear_call* call, void* stream);
+int fgb_grouped_linear_backward(const fgb_grouped_linear_call* call, void* stream);
+
 /* ------------------------------------------------------------------------
  * Pipeline microbenchmark (no counterpart in the reference)
  * --------------------------------------------------------------------- */

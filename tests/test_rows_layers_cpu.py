@@ -153,3 +153,58 @@ def test_embedding_entry_points_refuse(lib):
     assert rc(lib.fgb_embedding_forward, table=None) == -1 and rc(lib.fgb_embedding_forward, out=(1 << 22) + 2) == -4
     assert rc(lib.fgb_embedding_backward, grad_out=None) == -1 and rc(lib.fgb_embedding_backward, workspace_bytes=64) == -5
     assert rc(lib.fgb_embedding_backward, workspace=(1 << 24) + 8) == -4 and rc(lib.fgb_embedding_forward, n=0) == 0
+
+
+def test_oracle_grouped_linear_is_torchs():
+    g = torch.Generator().manual_seed(3)
+    x, dy = torch.randn(20, 6, generator=g, dtype=torch.float64), torch.randn(20, 4, generator=g, dtype=torch.float64)
+    w, b = torch.randn(3, 4, 6, generator=g, dtype=torch.float64), torch.randn(3, 4, generator=g, dtype=torch.float64)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    y = torch.cat([torch.nn.functional.linear(leaves[0][lo:hi], leaves[1][i], leaves[2][i]) for i, (lo, hi) in enumerate(((0, 13), (13, 13), (13, 20)))])
+    grads = torch.autograd.grad(y, leaves, dy)
+    ref = orc.grouped_linear(x, [(0, 13), (13, 13), (13, 20)], w, b, dy)
+    for got, want in ((ref["y"], y), (ref["dx"], grads[0]), (ref["dw"], grads[1]), (ref["db"], grads[2])):
+        assert torch.allclose(got, want, rtol=1e-11, atol=1e-12)
+
+
+def test_grouped_linear_refuses(lib):
+    from flexgemm_b200.ops.grouped_linear import sparse_grouped_linear
+    x, off, w, b = torch.randn(10, 8), torch.tensor([0, 4, 10]), torch.randn(2, 5, 8), torch.randn(2, 5)
+    with pytest.raises(NotImplementedError):
+        sparse_grouped_linear(x, off, w, b)
+    for args in ((x[0], off, w), (x, off, w[0]), (x[:, :7], off, w), (x, off[:2], w), (x, off.view(1, 3), w), (x, off, w, b[:, :4]), (x, off, w, b[0])):
+        with pytest.raises(AssertionError):
+            sparse_grouped_linear(*args)
+    for args in ((x.double(), off, w.double()), (x, off.float(), w), (x, off, w.half()), (x, off, w, b.half())):
+        with pytest.raises(TypeError):
+            sparse_grouped_linear(*args)
+    most = lib.fgb_grouped_linear_max_groups()
+    with pytest.raises(ValueError):
+        sparse_grouped_linear(x, torch.zeros(most + 2, dtype=torch.int32), torch.zeros(most + 1, 1, 8))
+
+
+class GroupedCall(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in ("x", "weight", "bias", "grad_out", "out", "grad_x", "grad_weight", "grad_bias", "offsets")] + \
+               [("n", ctypes.c_int64), ("groups", ctypes.c_int64)] + [(k, ctypes.c_int32) for k in ("offsets_bits", "ci", "co", "dtype")] + \
+               [("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("status", ctypes.c_void_p)]
+
+
+def test_grouped_linear_entry_points_refuse(lib):
+    good = dict(x=1 << 20, weight=1 << 21, out=1 << 22, grad_out=1 << 22, grad_x=1 << 23, grad_weight=1 << 23, offsets=1 << 24, n=1000, groups=3,
+                offsets_bits=32, ci=64, co=72, dtype=_cabi.F16, workspace=1 << 25, workspace_bytes=1 << 40)
+
+    def rc(fn, **kw):
+        return fn(ctypes.byref(GroupedCall(**{**good, **kw})), None)
+    for backward in (0, 1):
+        for dtype in range(4):
+            assert lib.fgb_grouped_linear_workspace_bytes(ctypes.byref(GroupedCall(**{**good, "dtype": dtype})), backward) > 0
+        assert lib.fgb_grouped_linear_workspace_bytes(None, backward) == -1
+    for fn in (lib.fgb_grouped_linear_forward, lib.fgb_grouped_linear_backward):
+        assert fn(None, None) == -1
+        for kw, code in ((dict(dtype=4), -3), (dict(offsets_bits=0), -3), (dict(n=-1), -2), (dict(n=1 << 31), -2), (dict(groups=0), -2), (dict(groups=1 << 20), -2),
+                         (dict(ci=0), -2), (dict(co=1 << 17), -2), (dict(n=(1 << 31) - 300, ci=65536, co=65536, dtype=_cabi.F32_IEEE), -2), (dict(offsets=None), -1),
+                         (dict(weight=None), -1), (dict(workspace=None), -1), (dict(x=(1 << 20) + 2), -4), (dict(weight=(1 << 21) + 8), -4),
+                         (dict(workspace=(1 << 25) + 64), -4), (dict(workspace_bytes=100), -5)):
+            assert rc(fn, **kw) == code, (fn.__name__, kw)
+    assert rc(lib.fgb_grouped_linear_forward, out=None) == -1 and rc(lib.fgb_grouped_linear_forward, n=0) == 0
+    assert rc(lib.fgb_grouped_linear_backward, grad_out=None) == -1 and rc(lib.fgb_grouped_linear_backward, grad_weight=None, grad_bias=1 << 23) == -1
