@@ -67,28 +67,32 @@ template <bool kExact>
 __device__ __forceinline__ float activate(float z, int act) {
   return act == FGB_ACT_SILU ? (z == -INFINITY ? 0.f : z * sigmoid<kExact>(z)) : z;
 }
-// dy * act'(z)
+// dy * act'(z).  Every rounding is named: the kernels that call it have to agree on the last bit, so that q - mean(q) is zero
+// where a mean is of one value.
 template <bool kExact>
 __device__ __forceinline__ float activate_grad(float dy, float z, int act) {
   if (act != FGB_ACT_SILU) return dy;
   const float s = sigmoid<kExact>(z);
-  return dy * (s * (1.f + z * (1.f - s)));
+  return __fmul_rn(dy, __fmul_rn(s, fmaf(z, __fsub_rn(1.f, s), 1.f)));
 }
 
 // What a thread keeps of its kVec channels for one sample
 template <int kVec>
 struct ChannelParams {
-  float mean[kVec], a[kVec], b[kVec];  // z = (x - mean) a + b
+  float mean[kVec], r[kVec], w[kVec], b[kVec];
   __device__ __forceinline__ void load(const NormArgs& p, uint32_t s, int c0) {
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       const int c = c0 + i;
       const size_t g = size_t(s) * p.G + c / p.cpg;
       mean[i] = p.mean[g];
-      a[i] = p.rstd[g] * (p.w != nullptr ? load_param(p.w, p.param_dtype, c) : 1.f);
+      r[i] = p.rstd[g];
+      w[i] = p.w != nullptr ? load_param(p.w, p.param_dtype, c) : 1.f;
       b[i] = p.b != nullptr ? load_param(p.b, p.param_dtype, c) : 0.f;
     }
   }
+  __device__ __forceinline__ float h(float x, int i) const { return __fmul_rn(__fsub_rn(x, mean[i]), r[i]); }
+  __device__ __forceinline__ float z(float h, int i) const { return fmaf(h, w[i], b[i]); }
 };
 
 // ------------------------------------------------------------------ 1. sums
@@ -143,19 +147,16 @@ __global__ void __launch_bounds__(kNormThreads) norm_sums_kernel(const NormArgs 
       } else {
         ChannelParams<kVec> k;
         k.load(p, s, c0);
-        float rs[kVec];
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) rs[i] = p.rstd[size_t(s) * p.G + (c0 + i) / p.cpg];
         auto add = [&](const typename Ch::Raw& raw, const typename Ch::Raw& raw_dy) {
           float v[kVec], g[kVec];
           Ch::unpack(raw, v);
           Ch::unpack(raw_dy, g);
 #pragma unroll
           for (int i = 0; i < kVec; ++i) {
-            const float d = v[i] - k.mean[i];
-            const float dz = activate_grad<kExact>(g[i], fmaf(d, k.a[i], k.b[i]), p.act);
+            const float h = k.h(v[i], i);
+            const float dz = activate_grad<kExact>(g[i], k.z(h, i), p.act);
             sum0[i] += dz;
-            sum1[i] = fmaf(dz, d * rs[i], sum1[i]);
+            sum1[i] = fmaf(dz, h, sum1[i]);
           }
         };
         uint32_t r = lo + ry;
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(const NormArgs
         float v[kVec];
         Ch::unpack(raw, v);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) v[i] = activate<kExact>(fmaf(v[i] - k.mean[i], k.a[i], k.b[i]), p.act);
+        for (int i = 0; i < kVec; ++i) v[i] = activate<kExact>(k.z(k.h(v[i], i), i), p.act);
         Ch::store(out + size_t(r) * p.C, Ch::pack(v));
       };
       uint32_t r = lo + ry;
@@ -340,11 +341,11 @@ __global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(const NormArgs
       }
       for (; r < hi; r += lanes) one(Ch::load(x + size_t(r) * p.C), r);
     } else {
-      float rs[kVec], m1[kVec], m2[kVec];
+      float m1[kVec], m2[kVec];
 #pragma unroll
       for (int i = 0; i < kVec; ++i) {
         const size_t g = size_t(s) * p.G + (c0 + i) / p.cpg;
-        rs[i] = p.rstd[g], m1[i] = p.joined[g * 2] * rs[i], m2[i] = p.joined[g * 2 + 1] * rs[i] * rs[i];
+        m1[i] = p.joined[g * 2], m2[i] = p.joined[g * 2 + 1];
       }
       auto one = [&](const typename Ch::Raw& raw, const typename Ch::Raw& raw_dy, uint32_t r) {
         float v[kVec], g[kVec];
@@ -352,9 +353,9 @@ __global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(const NormArgs
         Ch::unpack(raw_dy, g);
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
-          const float d = v[i] - k.mean[i];
-          const float dz = activate_grad<kExact>(g[i], fmaf(d, k.a[i], k.b[i]), p.act);
-          v[i] = fmaf(dz, k.a[i], -fmaf(d, m2[i], m1[i]));  // r (dz w - m1 - h m2) with h = d r
+          const float h = k.h(v[i], i);
+          const float q = __fmul_rn(activate_grad<kExact>(g[i], k.z(h, i), p.act), k.w[i]);
+          v[i] = k.r[i] * fmaf(-h, m2[i], __fsub_rn(q, m1[i]));
         }
         Ch::store(out + size_t(r) * p.C, Ch::pack(v));
       };

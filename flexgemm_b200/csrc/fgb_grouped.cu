@@ -23,7 +23,10 @@
 //
 // fp32 operands are written as sums of bf16 planes (hi + mid + lo, 8 bits each) and multiplied plane by plane: six products
 // (all whose weight is 2^-16 and more) for accurate fp32, three (2^-8 and more) where TF32 is allowed.  bf16 has
-// fp32's range, so no scaling is needed, and the rate is that of the same number of products at TF32's half rate and width.
+// fp32's range, so no scaling is needed, and six of them cost what three TF32 products do (half the rate, twice the bytes).
+// The tensor cores cut what they add to an accumulator at its last bit instead of rounding: over a long k that is a bias
+// (2e-8 of the sum for every 16 k; 1e-5 where k was 10^5).  So fp32 leaves the accumulator after each block of 64 k, the small
+// products first, the large one last, and the storing warps add the blocks up in registers, rounding to nearest.
 #include <algorithm>
 #include <type_traits>
 
@@ -56,7 +59,7 @@ struct GroupedArgs {
   uint32_t p_planes, q_planes;  // their planes, four bits a term
   int p_mn, q_mn;       // operand is MN-major
   int stages, q_bytes, acc_sets, acc_stride;
-  uint32_t min_range, max_range;  // iterations of a range; 0, 0: a range is a tile
+  uint32_t min_range;   // iterations that a range has at least; 0: a range is a tile
   uint32_t idesc, idesc_ones;
   uint32_t one_pair;    // two ones of the operand type
   const void* bias;     // [groups, nout] or null
@@ -121,9 +124,8 @@ __device__ __forceinline__ void plan_groups(const GroupedArgs& p, uint32_t* firs
 // iterations of a range
 template <int kMode>
 __device__ __forceinline__ uint32_t range_length(const GroupedArgs& p, uint32_t total, uint32_t ctas) {
-  if (p.max_range == 0u) return static_cast<uint32_t>(p.k_blocks * p.terms);  // a tile
-  const uint32_t even = (total + ctas - 1u) / ctas;
-  return min(max(even, p.min_range), p.max_range);
+  if (p.min_range == 0u) return static_cast<uint32_t>(p.k_blocks * p.terms);  // a tile
+  return max((total + ctas - 1u) / ctas, p.min_range);
 }
 
 // A tile, or the part of one that a range holds
@@ -189,57 +191,52 @@ __device__ __forceinline__ void store_value(T* p, float v) {
   else *p = static_cast<T>(v);
 }
 
-// The columns [0, columns) of the warp's 32 accumulator rows to out[row * ld + col] (row < rows, col < cols): 32 columns at a
-// time, every second 32 of them (`group` 0 or 1).  64 bytes of each row go through the warp's staging buffer (32 rows of
-// 64 bytes, 16-byte pieces XORed with half the row), so that a store instruction writes whole sectors of eight rows.
+// 32 columns of the warp's 32 accumulator rows to out[row * ld + c0 + i] (row < rows, c0 + i < cols).  64 bytes of each row
+// at a time go through the warp's staging buffer (32 rows of 64 bytes, 16-byte pieces XORed with half the row), so that a
+// store instruction writes whole sectors of eight rows.
 template <typename T>
-__device__ __forceinline__ void store_tile(uint32_t tmem, uint8_t* stage, float* s_bias, int lane, int group, int columns, T* out, int64_t ld, int rows, int cols,
-                                           int vec_ok, const void* bias, int bias_dtype) {
+__device__ __forceinline__ void store_columns(uint32_t (&acc)[32], uint8_t* stage, float* s_bias, int lane, int c0, T* out, int64_t ld, int rows, int cols,
+                                              int vec_ok, const void* bias, int bias_dtype) {
   constexpr int kPiece = 16 / sizeof(T), kCols = 4 * kPiece;  // columns of a piece, and of 64 bytes
   uint8_t* mine = stage + lane * 64;
-  for (int c0 = group * 32; c0 < columns; c0 += 64) {
-    uint32_t acc[32];
-    tmem_ld_32x32(tmem + c0, acc);
-    if (bias != nullptr) s_bias[lane] = c0 + lane < cols ? load_param(bias, bias_dtype, c0 + lane) : 0.f;
+  if (bias != nullptr) {
+    s_bias[lane] = c0 + lane < cols ? load_param(bias, bias_dtype, c0 + lane) : 0.f;
     __syncwarp();
-    tmem_ld_wait();
-    if (bias != nullptr) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float4 b = reinterpret_cast<const float4*>(s_bias)[i];
-        acc[4 * i] = __float_as_uint(__uint_as_float(acc[4 * i]) + b.x), acc[4 * i + 1] = __float_as_uint(__uint_as_float(acc[4 * i + 1]) + b.y);
-        acc[4 * i + 2] = __float_as_uint(__uint_as_float(acc[4 * i + 2]) + b.z), acc[4 * i + 3] = __float_as_uint(__uint_as_float(acc[4 * i + 3]) + b.w);
-      }
+    for (int i = 0; i < 8; ++i) {
+      const float4 b = reinterpret_cast<const float4*>(s_bias)[i];
+      acc[4 * i] = __float_as_uint(__uint_as_float(acc[4 * i]) + b.x), acc[4 * i + 1] = __float_as_uint(__uint_as_float(acc[4 * i + 1]) + b.y);
+      acc[4 * i + 2] = __float_as_uint(__uint_as_float(acc[4 * i + 2]) + b.z), acc[4 * i + 3] = __float_as_uint(__uint_as_float(acc[4 * i + 3]) + b.w);
     }
+  }
 #pragma unroll
-    for (int h = 0; h < 32 / kCols; ++h) {
+  for (int h = 0; h < 32 / kCols; ++h) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float f[kPiece];
+    for (int g = 0; g < 4; ++g) {
+      float f[kPiece];
 #pragma unroll
-        for (int i = 0; i < kPiece; ++i) f[i] = __uint_as_float(acc[h * kCols + g * kPiece + i]);
-        *reinterpret_cast<uint4*>(mine + ((g ^ ((lane >> 1) & 3)) << 4)) = Channels<T, kPiece>::pack(f);
-      }
-      __syncwarp();
-      const int piece = lane & 3, col = c0 + h * kCols + piece * kPiece;
+      for (int i = 0; i < kPiece; ++i) f[i] = __uint_as_float(acc[h * kCols + g * kPiece + i]);
+      *reinterpret_cast<uint4*>(mine + ((g ^ ((lane >> 1) & 3)) << 4)) = Channels<T, kPiece>::pack(f);
+    }
+    __syncwarp();
+    const int piece = lane & 3, col = c0 + h * kCols + piece * kPiece;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = i * 8 + (lane >> 2);
-        const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
-        if (row < rows && col < cols) {
-          T* to = out + int64_t(row) * ld + col;
-          if (vec_ok) {
-            *reinterpret_cast<uint4*>(to) = v;
-          } else {
-            const T* t = reinterpret_cast<const T*>(&v);
+    for (int i = 0; i < 4; ++i) {
+      const int row = i * 8 + (lane >> 2);
+      const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
+      if (row < rows && col < cols) {
+        T* to = out + int64_t(row) * ld + col;
+        if (vec_ok) {
+          *reinterpret_cast<uint4*>(to) = v;
+        } else {
+          const T* t = reinterpret_cast<const T*>(&v);
 #pragma unroll
-            for (int e = 0; e < kPiece; ++e)
-              if (col + e < cols) to[e] = t[e];
-          }
+          for (int e = 0; e < kPiece; ++e)
+            if (col + e < cols) to[e] = t[e];
         }
       }
-      __syncwarp();
     }
+    __syncwarp();
   }
 }
 
@@ -268,6 +265,8 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile uint32_t* abort_flag = &ctl->abort_flag;
   constexpr int kParamDtype = std::is_same<T, __half>::value ? FGB_F16 : std::is_same<T, __nv_bfloat16>::value ? FGB_BF16 : FGB_F32_IEEE;
+  constexpr bool kBlocks = std::is_same<T, float>::value;  // the accumulator is emptied after every block of 64 k
+  constexpr int kSums = kMode == kFew ? 1 : 3;             // blocks of 32 columns that a storing warp adds up
 
   chain_release();
   if (tid == 0) {
@@ -353,13 +352,15 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
     const uint32_t p_lbo = kMode == kWeight || p.p_mn ? 8192u : 16u, q_lbo = kMode == kWeight || p.q_mn ? 8192u : 16u;
     const uint64_t d_ones = make_smem_desc(smem_u32(ones), 16, 1024);
     while (walk.next(it)) {
-      mbar_wait(&ctl->acc_empty[set], set_ph ^ 1, abort_flag);
-      tc_fence_after_sync();
-      const uint32_t acc = tmem_base + set * p.acc_stride;
       const bool with_ones = kMode == kWeight && p.db != nullptr && n_tile_of(it) == 0u;
       uint32_t kb = it.from / p.terms, term = it.from - kb * p.terms;
-      uint32_t any = 0, any_ones = 0;
+      uint32_t any = 0, any_ones = 0, acc = 0;
       for (uint32_t i = it.from; i < it.to; ++i) {
+        if (any == 0u) {  // a new accumulator
+          mbar_wait(&ctl->acc_empty[set], set_ph ^ 1, abort_flag);
+          tc_fence_after_sync();
+          acc = tmem_base + set * p.acc_stride;
+        }
         mbar_wait(&ctl->full[s], ph, abort_flag);
         __syncwarp();
         tc_fence_after_sync();
@@ -376,7 +377,7 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
           fence_proxy_async_smem();
           __syncwarp();
         }
-        const bool ones_now = with_ones && ((p.q_planes >> (4 * term)) & 15u) == 0u;
+        const bool ones_now = with_ones && ((p.q_planes >> (4 * term)) & 15u) == 0u;  // once for each plane of dy
         if (elect_one()) {
           const uint64_t dp = make_smem_desc(base, p_lbo, 1024), dq = make_smem_desc(base + kGrPBytes, q_lbo, 1024);
 #pragma unroll
@@ -393,10 +394,13 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
         any_ones |= ones_now ? 1u : 0u;
         if (++term == static_cast<uint32_t>(p.terms)) term = 0, ++kb;
         if (++s == static_cast<uint32_t>(p.stages)) s = 0, ph ^= 1;
+        if (i + 1u == it.to || (kBlocks && term == 0u)) {  // the accumulator is done: the tile's last, or the block's
+          if (elect_one()) umma_commit(&ctl->acc_full[set]);
+          __syncwarp();
+          if (++set == static_cast<uint32_t>(p.acc_sets)) set = 0, set_ph ^= 1;
+          any = any_ones = 0u;
+        }
       }
-      if (elect_one()) umma_commit(&ctl->acc_full[set]);
-      __syncwarp();
-      if (++set == static_cast<uint32_t>(p.acc_sets)) set = 0, set_ph ^= 1;
     }
   } else {
     // ------------------------------------------------------------------ stores
@@ -404,56 +408,109 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
     uint8_t* stage = store + warp * 2048;
     float* bias_buf = s_bias + warp * 64;
     uint32_t set = 0, set_ph = 0;
-    while (walk.next(it)) {
+    // this warp's columns are [32 group, 32 group + 32) of every 64: at most 3 x 32 of them in fp32
+    uint32_t sum[kBlocks ? kSums : 1][32];
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    auto wait_full = [&]() {
       mbar_wait(&ctl->acc_full[set], set_ph, abort_flag);
       tc_fence_after_sync();
-      const uint32_t tmem = tmem_base + set * p.acc_stride + (static_cast<uint32_t>(quarter * 32) << 16);
-      const int m0 = static_cast<int>(m_tile_of(it)) * 128 + quarter * 32, n0 = static_cast<int>(n_tile_of(it)) * p.bn;
-      const bool whole = it.from == 0u && it.to == it.whole;
-      // a piece of a tile: the first slot of its range for one that began before it, else the second
-      float* piece = whole ? nullptr : p.slab + (size_t(it.range) * 2 + (it.from == 0u ? 1 : 0)) * 128 * p.acc_stride;
-      if (*abort_flag) {
-        // nothing that was waited for is there: the status word says so
-      } else if constexpr (kMode == kFew) {
-        const int rows = static_cast<int>(it.hi - it.lo) - n0;  // rows of the tile, and more
-        const int m = m0 + lane;
-        const float b = whole && p.bias != nullptr && m < p.m_extent ? load_param(p.bias, kParamDtype, int64_t(it.group) * p.m_extent + m) : 0.f;
-        T* out = static_cast<T*>(p.out) + int64_t(it.lo + n0) * p.out_ld + m;
-        for (int c0 = group * 32; c0 < p.bn; c0 += 64) {
-          uint32_t acc[32];
-          tmem_ld_32x32(tmem + c0, acc);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int r = c0 + i;
-            if (r >= p.bn) break;
-            if (piece != nullptr) piece[r * 128 + quarter * 32 + lane] = __uint_as_float(acc[i]);
-            else if (r < rows && m < p.m_extent) store_value(out + int64_t(r) * p.out_ld, __uint_as_float(acc[i]) + b);
-          }
-        }
-      } else if (piece != nullptr) {
-        store_tile<float>(tmem, stage, bias_buf, lane, group, p.bn, piece + size_t(quarter * 32) * p.bn, p.bn, 32, p.bn, 1, nullptr, 0);
-      } else {
-        const int64_t row0 = kMode == kRows ? int64_t(it.lo) + m0 : int64_t(it.group) * p.m_extent + m0;
-        const int rows = (kMode == kRows ? static_cast<int>(it.hi - it.lo) : p.m_extent) - m0;
-        const void* bias = p.bias == nullptr ? nullptr
-                           : static_cast<const char*>(p.bias) + (int64_t(it.group) * p.n_extent + n0) * static_cast<int64_t>(sizeof(T));
-        store_tile<T>(tmem, stage, bias_buf, lane, group, p.bn, static_cast<T*>(p.out) + row0 * p.out_ld + n0, p.out_ld, rows, p.n_extent - n0, p.vec_ok,
-                      bias, kParamDtype);
-      }
-      if (kMode == kWeight && p.db != nullptr && n0 == 0 && group == 0 && !*abort_flag) {
-        uint32_t acc[32];
-        tmem_ld_32x32(tmem + p.bn, acc);
-        tmem_ld_wait();
-        if (!meets_first_plane(p, it.from, it.to)) acc[0] = 0u;  // no product with the ones: the accumulator holds nothing
-        const int m = m0 + lane;
-        if (piece != nullptr) piece[128 * p.bn + quarter * 32 + lane] = __uint_as_float(acc[0]);
-        else if (m < p.m_extent) store_value(static_cast<T*>(p.db) + int64_t(it.group) * p.m_extent + m, __uint_as_float(acc[0]));
-      }
+      return tmem_base + set * p.acc_stride + lanes;
+    };
+    auto give_back = [&]() {
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl->acc_empty[set]);
       if (++set == static_cast<uint32_t>(p.acc_sets)) set = 0, set_ph ^= 1;
+    };
+    while (walk.next(it)) {
+      const int m0 = static_cast<int>(m_tile_of(it)) * 128 + quarter * 32, n0 = static_cast<int>(n_tile_of(it)) * p.bn;
+      const bool whole = it.from == 0u && it.to == it.whole;
+      const bool with_db = kMode == kWeight && p.db != nullptr && n0 == 0 && group == 0;
+      float db = 0.f;
+      uint32_t tmem = 0;
+      if constexpr (kBlocks) {
+#pragma unroll
+        for (int b = 0; b < kSums; ++b)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sum[b][i] = 0u;
+        for (uint32_t at = it.from; at < it.to;) {
+          const uint32_t end = min(it.to, (at / p.terms + 1u) * p.terms);
+          tmem = wait_full();
+#pragma unroll
+          for (int b = 0; b < kSums; ++b) {
+            if (group * 32 + b * 64 < p.bn) {
+              uint32_t acc[32];
+              tmem_ld_32x32(tmem + group * 32 + b * 64, acc);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) sum[b][i] = __float_as_uint(__uint_as_float(sum[b][i]) + __uint_as_float(acc[i]));
+            }
+          }
+          if (with_db && meets_first_plane(p, at, end)) {
+            uint32_t acc[32];
+            tmem_ld_32x32(tmem + p.bn, acc);
+            tmem_ld_wait();
+            db += __uint_as_float(acc[0]);
+          }
+          give_back();
+          at = end;
+        }
+      } else {
+        tmem = wait_full();
+        if (with_db) {
+          uint32_t acc[32];
+          tmem_ld_32x32(tmem + p.bn, acc);
+          tmem_ld_wait();
+          db = __uint_as_float(acc[0]);
+        }
+      }
+      // a piece of a tile: the first slot of its range for one that began before it, else the second
+      float* piece = whole ? nullptr : p.slab + (size_t(it.range) * 2 + (it.from == 0u ? 1 : 0)) * 128 * p.acc_stride;
+      const int64_t row0 = kMode == kRows ? int64_t(it.lo) + m0 : int64_t(it.group) * p.m_extent + m0;
+      const int rows = (kMode == kRows ? static_cast<int>(it.hi - it.lo) : p.m_extent) - m0;
+      const void* bias = p.bias == nullptr ? nullptr
+                         : static_cast<const char*>(p.bias) + (int64_t(it.group) * (kMode == kFew ? p.m_extent : p.n_extent) + (kMode == kFew ? 0 : n0)) *
+                                                                  static_cast<int64_t>(sizeof(T));
+      const float few_bias = kMode == kFew && whole && bias != nullptr && m0 + lane < p.m_extent ? load_param(bias, kParamDtype, m0 + lane) : 0.f;
+      auto put = [&](uint32_t (&acc)[32], int c0) {
+        if constexpr (kMode == kFew) {
+          const int left = static_cast<int>(it.hi - it.lo) - n0;  // rows of the tile, and more
+          T* out = static_cast<T*>(p.out) + int64_t(it.lo + n0) * p.out_ld + m0 + lane;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int r = c0 + i;
+            if (r < p.bn) {
+              if (piece != nullptr) piece[r * 128 + quarter * 32 + lane] = __uint_as_float(acc[i]);
+              else if (r < left && m0 + lane < p.m_extent) store_value(out + int64_t(r) * p.out_ld, __uint_as_float(acc[i]) + few_bias);
+            }
+          }
+        } else if (piece != nullptr) {
+          store_columns<float>(acc, stage, bias_buf, lane, c0, piece + size_t(quarter * 32) * p.bn, p.bn, 32, p.bn, 1, nullptr, 0);
+        } else {
+          store_columns<T>(acc, stage, bias_buf, lane, c0, static_cast<T*>(p.out) + row0 * p.out_ld + n0, p.out_ld, rows, p.n_extent - n0, p.vec_ok, bias,
+                           kParamDtype);
+        }
+      };
+      if (*abort_flag == 0u) {  // else nothing that was waited for is there, and the status word says so
+        if constexpr (kBlocks) {
+#pragma unroll
+          for (int b = 0; b < kSums; ++b)
+            if (group * 32 + b * 64 < p.bn) put(sum[b], group * 32 + b * 64);
+        } else {
+          for (int c0 = group * 32; c0 < p.bn; c0 += 64) {
+            uint32_t acc[32];
+            tmem_ld_32x32(tmem + c0, acc);
+            tmem_ld_wait();
+            put(acc, c0);
+          }
+        }
+        if (with_db) {
+          const int m = m0 + lane;
+          if (piece != nullptr) piece[128 * p.bn + quarter * 32 + lane] = db;
+          else if (m < p.m_extent) store_value(static_cast<T*>(p.db) + int64_t(it.group) * p.m_extent + m, db);
+        }
+      }
+      if constexpr (!kBlocks) give_back();
     }
     // rows of no group (forward and input gradient): zeros
     if constexpr (kMode != kWeight) {
@@ -611,10 +668,10 @@ static cudaError_t make_operand(Operand& o, const void* src, int64_t rows, int c
   return launch_chained(grouped_planes_kernel<__half>, dim3(grid), dim3(256), 0, s, static_cast<const __half*>(src), dst, static_cast<uint64_t>(rows), c, o.cp, 1);
 }
 
-// columns of a tile over `extent` channels: all of them in steps of 32 up to 256, else equal tiles in steps of 64
-static int tile_columns(int extent) {
-  if (extent <= 256) return (extent + 31) / 32 * 32;
-  const int tiles = (extent + 255) / 256;
+// columns of a tile over `extent` channels: all of them in steps of 32 up to `most`, else equal tiles in steps of 64
+static int tile_columns(int extent, int most) {
+  if (extent <= most) return (extent + 31) / 32 * 32;
+  const int whole = most / 64 * 64, tiles = (extent + whole - 1) / whole;
   return ((extent + tiles - 1) / tiles + 63) / 64 * 64;
 }
 
@@ -622,14 +679,10 @@ struct GroupedPlan {
   int mode, bn, split;
   int64_t slots;        // pieces that the slab holds
   int64_t slab_bytes;
-  uint32_t min_range, max_range;
+  uint32_t min_range;
   int acc_stride;
   int64_t tiles;        // most tiles (those that the join kernel looks at)
 };
-
-// Accumulating over a long k rounds each step towards the accumulator's size: accurate fp32 adds pieces of at most this many
-// stages (64 k of one plane product) to another in fp32.
-constexpr uint32_t kGrExactStages = 192;
 
 // A tile of few rows where a group has at most 64 on average: see the note on kFew above.
 static bool few_rows(const fgb_grouped_linear_call& c) { return c.n <= 64 * c.groups; }
@@ -637,15 +690,16 @@ static bool few_rows(const fgb_grouped_linear_call& c) { return c.n <= 64 * c.gr
 static int grouped_plan(const fgb_grouped_linear_call& c, int pass, GroupedPlan& p) {
   const int64_t sms = device_sm_count(), terms = c.dtype == FGB_F32_IEEE ? 6 : c.dtype == FGB_F32_TF32 ? 3 : 1;
   const int64_t N = c.n, G = c.groups;
+  const int most = is_f32(c.dtype) ? 192 : 256;  // fp32: the blocks' sums of a tile are held in 3 x 32 registers
   int64_t iterations;
-  p.split = 0, p.min_range = p.max_range = 0;
+  p.split = 0, p.min_range = 0;
   if (pass == 2) {
     p.mode = kWeight;
-    p.bn = tile_columns(c.ci);
+    p.bn = tile_columns(c.ci, most);
     const int64_t per = ceil_div(c.ci, p.bn) * ceil_div(c.co, 128);
     p.tiles = G * per;
     iterations = (N / 64 + G) * per * terms;
-    p.split = 1, p.min_range = 4, p.max_range = c.dtype == FGB_F32_IEEE ? kGrExactStages : 0x40000000u;
+    p.split = 1, p.min_range = 4;
   } else {
     const int nout = pass == 0 ? c.co : c.ci, k = pass == 0 ? c.ci : c.co;
     const int64_t kb = ceil_div(k, 64);
@@ -656,17 +710,17 @@ static int grouped_plan(const fgb_grouped_linear_call& c, int pass, GroupedPlan&
       const int64_t m_tiles = ceil_div(nout, 128);
       p.tiles = std::min<int64_t>(N, N / p.bn + G) * m_tiles;
       iterations = p.tiles * kb * terms;
-      if (p.tiles <= sms / 2 && kb * terms >= 8) p.split = 1, p.min_range = 4, p.max_range = 0x40000000u;
+      if (p.tiles <= sms / 2 && kb * terms >= 8) p.split = 1, p.min_range = 4;
     } else {
       p.mode = kRows;
-      p.bn = tile_columns(nout);
+      p.bn = tile_columns(nout, most);
       p.tiles = (N / 128 + G) * ceil_div(nout, p.bn);
       iterations = p.tiles * kb * terms;
     }
   }
   if (iterations >= (int64_t(1) << 31) - 1) return FGB_E_SIZE;
   p.acc_stride = std::max(p.bn, 32) + (pass == 2 && c.grad_bias != nullptr ? 32 : 0);
-  p.slots = p.split ? 2 * (std::max<int64_t>(sms, ceil_div(iterations, int64_t(p.max_range))) + 1) : 0;
+  p.slots = p.split ? 2 * sms : 0;
   p.slab_bytes = align256(p.slots * 128 * p.acc_stride * 4);
   return FGB_OK;
 }
@@ -717,8 +771,9 @@ static int grouped_pass(const fgb_grouped_linear_call& c, int pass, const Operan
   a.ranges = RowRanges{c.offsets, c.offsets_bits == 64, static_cast<uint32_t>(c.n), static_cast<uint32_t>(c.groups)};
   a.bn = p.bn;
   a.terms = c.dtype == FGB_F32_IEEE ? 6 : c.dtype == FGB_F32_TF32 ? 3 : 1;
-  a.p_planes = 0x201010u, a.q_planes = 0x021100u;  // (hi hi) (mid hi) (hi mid) | (mid mid) (hi lo) (lo hi)
-  a.min_range = p.min_range, a.max_range = p.max_range;
+  // the small products first: (lo hi) (hi lo) (mid mid) (mid hi) (hi mid) (hi hi), or the last three of them
+  a.p_planes = a.terms == 6 ? 0x001102u : a.terms == 3 ? 0x001u : 0u, a.q_planes = a.terms == 6 ? 0x010120u : a.terms == 3 ? 0x010u : 0u;
+  a.min_range = p.min_range;
   a.acc_stride = p.acc_stride;
   a.acc_sets = 2 * p.acc_stride <= 512 ? 2 : 1;
   a.slab = slab;

@@ -157,6 +157,15 @@ def test_constant_rows():
     assert torch.equal(out.cpu(), torch.full_like(x, 0.5)) and not grads[0].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_statistics_of_one_value(dtype):
+    """One row a sample, one channel a group: the output is act(bias), the gradient zero, not what rounding leaves of it."""
+    x, dy, w, b, ends = problem([1] * 5, 16, dtype, seed=17)
+    for act in (None, "silu"):
+        out, grads = run(x, dy, w, b, ends.to(DEV), 16, act)
+        assert not grads[0].any() and not grads[1].any() and torch.equal(out, out[:1].expand_as(out))
+
+
 def test_repeated_calls_are_equal():
     x, dy, w, b, ends = problem([3000, 2000], 64, torch.bfloat16, seed=11)
     first = run(x, dy, w, b, ends.to(DEV), 8, "silu")
