@@ -3,10 +3,10 @@
 //   out[i] = scale * table[t_i]          grad[v] = scale * sum over i with t_i = v of g[i]
 //
 // The gradient sorts the positions by index (stable, fgb_sort.cu) and walks the sorted list in chunks of fixed length: a
-// group of threads adds the rows of one chunk, one run of equal indices after the other, in fp32.  A run that ends where
-// it began, in one chunk, is final; the two runs of a chunk that reach beyond its ends leave their sums in a slab, and a
-// second kernel adds a run's pieces up.  Nothing is added atomically, so the order of every sum is fixed, and an index
-// that every other position holds costs no more than a spread one.
+// group of threads adds the rows of one chunk, one run of equal indices after the other, in fp32; the CTA's groups then add
+// up the runs that lie in several of its chunks.  A run that lies in one CTA is final.  The two that may reach beyond its ends
+// leave their sums in a slab, and a second kernel adds a run's pieces up.  Nothing is added atomically, so the order of every
+// sum is fixed, and an index that every other position holds costs no more than a spread one.
 #include <algorithm>
 
 #include "fgb_common.cuh"
@@ -74,14 +74,13 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_kernel(const void* __re
 
 // ------------------------------------------------------------------ gradient
 // Sort keys: the index, or `rows` for a position that adds nothing (padding, out of range), which sorts behind all others.
-// Also clears the gradient (rows of indices that no position holds stay zero) and the counter of cut runs.
+// Also clears the gradient (rows of indices that no position holds stay zero).
 __global__ void __launch_bounds__(kEmbThreads) embedding_keys_kernel(const void* __restrict__ indices, int wide, uint32_t n, uint32_t rows, int64_t padding,
                                                                      int32_t* __restrict__ keys, uint16_t* __restrict__ grad, uint64_t grad_halves,
-                                                                     uint32_t* cut_count, int32_t* status, int32_t* mirror) {
+                                                                     int32_t* status, int32_t* mirror) {
   chain_release();
   chain_wait();
   const uint32_t t = blockIdx.x * kEmbThreads + threadIdx.x, total = gridDim.x * kEmbThreads;
-  if (t == 0) *cut_count = 0u;
   for (uint32_t i = t; i < n; i += total) {
     const int64_t v = index_at(indices, wide, i);
     const bool in = v >= 0 && v < int64_t(rows);
@@ -96,14 +95,21 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_keys_kernel(const void*
   if (t < grad_halves - whole * 8) grad[whole * 8 + t] = 0;
 }
 
+// What a CTA of the sum kernel says of its positions
+struct EmbInfo {
+  uint32_t key;    // of its last position
+  uint32_t flags;  // kGoesOn: the run of the last position goes on behind the CTA; kThrough: it began before the CTA, too
+};
+constexpr uint32_t kGoesOn = 1u, kThrough = 2u;
+
 struct EmbGrad {
   const void* g;
   void* grad;
   const int32_t* keys;      // by position
   const int64_t* order;     // positions by key
-  float* slab;              // [chunks][2][C]: the sum of the chunk's run that began before it, and of the one that goes on behind it
-  uint32_t* cut;            // [1 + chunks]: number of runs that go on behind the chunk they begin in, and those chunks
-  uint32_t n, rows, chunk, chunks;
+  float* slab;              // [ctas][2][C]: the sum of the CTA's run that began before it, and of the one that goes on behind it
+  EmbInfo* info;            // [ctas]
+  uint32_t n, rows, chunk, ctas;
   int C;
   float scale;
 };
@@ -112,6 +118,8 @@ template <typename T, int kVec>
 __global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const EmbGrad p) {
   using Ch = Channels<T, kVec>;
   extern __shared__ uint32_t s_mem[];
+  __shared__ float s_head[kVec][kEmbThreads];   // of each group's chunk: the sum of the run that began before it
+  __shared__ uint8_t s_through[kEmbThreads];    // and whether that run goes on behind it
   chain_release();
   const int packs = p.C / kVec, width = min(kEmbThreads, packs), lanes = kEmbThreads / width;
   const int cx = threadIdx.x % width, ry = threadIdx.x / width;
@@ -133,120 +141,172 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const EmbGra
     if (i >= 1u && i <= per_cta) s_pos[i - 1u] = pos;
   }
   __syncthreads();
-  if (ry >= lanes) return;
-  const uint32_t b = ry * p.chunk, e = min(b + p.chunk, p.n > base ? p.n - base : 0u);
-  if (b >= e) return;
-  const uint32_t q = blockIdx.x * lanes + ry;  // chunk
+  const uint32_t count = min(per_cta, p.n - base);  // positions of the CTA
+  const uint32_t b = ry * p.chunk, e = min(b + p.chunk, count);
+  const bool active = ry < lanes && b < e;
   const T* g = static_cast<const T*>(p.g);
   T* grad = static_cast<T*>(p.grad);
-  for (int c = cx; c < packs; c += width) {
+  auto open_at = [&](uint32_t i) { return s_key[int(i) - 1] == s_key[i]; };  // position i continues a run
+  if (threadIdx.x == 0) {
+    const uint32_t last = s_key[count - 1u];
+    p.info[blockIdx.x] = EmbInfo{last, (s_key[count] == last ? kGoesOn : 0u) | (open_at(0) && s_key[0] == last ? kThrough : 0u)};
+  }
+  if (cx == 0 && ry < lanes) s_through[ry] = active && open_at(b) && s_key[b] == s_key[e - 1u] && s_key[e] == s_key[b];
+  for (int c0 = 0; c0 < packs; c0 += width) {
+    const int c = c0 + cx;
+    const bool mine = active && c < packs;
     float acc[kVec];
 #pragma unroll
     for (int i = 0; i < kVec; ++i) acc[i] = 0.f;
-    uint32_t key = s_key[b];
-    bool open = static_cast<int32_t>(s_key[int(b) - 1]) == static_cast<int32_t>(key);  // the run began in an earlier chunk
-    auto flush = [&](bool goes_on) {
-      if (key >= p.rows) return;
-      if (open || goes_on) {
-        float* to = p.slab + (size_t(q) * 2 + (open ? 0 : 1)) * p.C + c * kVec;
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) to[i] = acc[i];
-        if (!open && c == 0) p.cut[1u + atomicAdd(p.cut, 1u)] = q;  // the list's order decides which CTA adds a run up, never a result
-      } else {
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) acc[i] *= p.scale;
-        Ch::store(grad + size_t(key) * p.C + c * kVec, Ch::pack(acc));
-      }
-    };
-    auto add = [&](uint32_t i, const typename Ch::Raw& raw) {
-      const uint32_t k = s_key[i];
-      if (k != key) {
-        flush(false);
-        open = false;
-        key = k;
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) acc[v] = 0.f;
-      }
+    uint32_t key = 0;
+    bool open = false;
+    auto finish = [&](const float (&sum)[kVec], uint32_t k) {
+      if (k >= p.rows) return;
       float f[kVec];
-      Ch::unpack(raw, f);
 #pragma unroll
-      for (int v = 0; v < kVec; ++v) acc[v] += f[v];
+      for (int i = 0; i < kVec; ++i) f[i] = sum[i] * p.scale;
+      Ch::store(grad + size_t(k) * p.C + c * kVec, Ch::pack(f));
     };
-    uint32_t i = b;
-    constexpr int kUnroll = 8;
-    for (; i + kUnroll <= e; i += kUnroll) {
-      typename Ch::Raw raw[kUnroll];
+    auto head = [&]() {
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) raw[u] = Ch::load(g + size_t(s_pos[i + u]) * p.C + c * kVec);
+      for (int i = 0; i < kVec; ++i) s_head[i][threadIdx.x] = acc[i];
+    };
+    if (mine) {
+      key = s_key[b];
+      open = open_at(b);
+      auto add = [&](uint32_t i, const typename Ch::Raw& raw) {
+        const uint32_t k = s_key[i];
+        if (k != key) {
+          if (open) head();
+          else finish(acc, key);
+          open = false;
+          key = k;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) add(i + u, raw[u]);
+          for (int v = 0; v < kVec; ++v) acc[v] = 0.f;
+        }
+        float f[kVec];
+        Ch::unpack(raw, f);
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) acc[v] += f[v];
+      };
+      uint32_t i = b;
+      constexpr int kUnroll = 8;
+      for (; i + kUnroll <= e; i += kUnroll) {
+        typename Ch::Raw raw[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) raw[u] = Ch::load(g + size_t(s_pos[i + u]) * p.C + c * kVec);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) add(i + u, raw[u]);
+      }
+      for (; i < e; ++i) add(i, Ch::load(g + size_t(s_pos[i]) * p.C + c * kVec));
+      if (open) head();  // the chunk's only run began before it
     }
-    for (; i < e; ++i) add(i, Ch::load(g + size_t(s_pos[i]) * p.C + c * kVec));
-    flush(s_key[e] == key);
+    __syncthreads();
+    // The last run of a chunk, where it began there, is its group's to finish, and the CTA's first, where it began before the
+    // CTA, group 0's: the heads of the chunks that follow are added while the run goes on.
+    if (mine) {
+      const bool from_before = ry == 0 && open_at(0);
+      auto collect = [&](float (&sum)[kVec], uint32_t k, int r, bool before) {
+        for (bool more = true; more && r < lanes && r * p.chunk < count; ++r) {
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) sum[i] += s_head[i][r * width + cx];
+          more = s_through[r] != 0;
+          if (!more) {
+            if (!before) {
+              finish(sum, k);
+              return;
+            }
+            break;
+          }
+        }
+        // a run that began before the CTA, or goes on behind it
+        if (k >= p.rows) return;
+        float* to = p.slab + (size_t(blockIdx.x) * 2 + (before ? 0 : 1)) * p.C + c * kVec;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) to[i] = sum[i];
+      };
+      if (!open) {
+        if (s_key[e] != key) finish(acc, key);
+        else collect(acc, key, ry + 1, false);
+      }
+      if (from_before) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) acc[i] = 0.f;
+        collect(acc, s_key[0], 0, true);
+      }
+    }
+    __syncthreads();
   }
 }
 
-// The runs that lie in more than one chunk.  A CTA takes 32 channels of a run: its 32 groups of eight threads add every
-// 32nd piece, and their sums are added in order.
+// The runs that lie in more than one CTA of the sum kernel: CTA q takes the one that began in that kernel's CTA q and goes
+// on behind it, if there is one, and 32 channels of it.  32 groups of eight threads add every 32nd piece, and their sums are
+// added in order.
 constexpr int kJoinCols = 32;
 template <typename T>
 __global__ void __launch_bounds__(kEmbThreads) embedding_join_kernel(const EmbGrad p) {
   __shared__ float s_sum[32][kJoinCols + 1];
   chain_release();
   chain_wait();
-  const uint32_t slices = static_cast<uint32_t>((p.C + kJoinCols - 1) / kJoinCols);
-  const uint32_t work = *p.cut * slices;
+  const uint32_t q = blockIdx.x;
+  const EmbInfo own = p.info[q];
+  if (own.flags != kGoesOn || own.key >= p.rows) return;  // nothing goes on, or its beginning is another CTA's
+  uint32_t last = q + 1u;  // the CTA in which the run ends: the first that it does not run through
+  for (;;) {
+    const uint32_t at = last + threadIdx.x;
+    const bool through = at < p.ctas && p.info[at].flags == (kGoesOn | kThrough);
+    const int run = __syncthreads_count(through);
+    if (run == kEmbThreads) {
+      last += kEmbThreads;
+      continue;
+    }
+    // through holds for a run of threads from the first on: behind the end another run may fill a CTA
+    __shared__ uint32_t s_end;
+    if (threadIdx.x == 0) s_end = 0xFFFFFFFFu;
+    __syncthreads();
+    if (!through) atomicMin(&s_end, at);
+    __syncthreads();
+    last = min(s_end, p.ctas - 1u);
+    break;
+  }
   const int cx = threadIdx.x & 7, ry = threadIdx.x >> 3;
-  for (uint32_t w = blockIdx.x; w < work; w += gridDim.x) {
-    const uint32_t q = p.cut[1u + w / slices];
-    const int c0 = static_cast<int>(w % slices) * kJoinCols + cx * 4;
-    const uint32_t end = min((q + 1u) * p.chunk, p.n);  // > end of the chunk the run begins in
-    auto key_at = [&](uint32_t i) { return p.keys[min(static_cast<uint32_t>(p.order[i]), p.n - 1u)]; };
-    const int32_t key = key_at(end - 1u);
-    uint32_t lo = end, hi = p.n;  // the run's end: positions below lo hold the key, those from hi on do not
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2u;
-      if (key_at(mid) == key) lo = mid + 1u;
-      else hi = mid;
-    }
-    const uint32_t last = (lo - 1u) / p.chunk;  // chunk that holds the run's last position
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t k = q + ry; k <= last; k += 32u) {
-      const float* from = p.slab + (size_t(k) * 2 + (k == q ? 1 : 0)) * p.C + c0;
+  const int c0 = static_cast<int>(blockIdx.y) * kJoinCols + cx * 4;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (uint32_t k = q + ry; k <= last; k += 32u) {
+    const float* from = p.slab + (size_t(k) * 2 + (k == q ? 1 : 0)) * p.C + c0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c0 + i < p.C) acc[i] += from[i];
-    }
+    for (int i = 0; i < 4; ++i)
+      if (c0 + i < p.C) acc[i] += from[i];
+  }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s_sum[ry][cx * 4 + i] = acc[i];
-    __syncthreads();
-    if (threadIdx.x < kJoinCols) {
-      const int c = static_cast<int>(w % slices) * kJoinCols + threadIdx.x;
-      if (c < p.C && key >= 0 && static_cast<uint32_t>(key) < p.rows) {
-        float v = 0.f;
-        for (int i = 0; i < 32; ++i) v += s_sum[i][threadIdx.x];
-        static_cast<T*>(p.grad)[size_t(key) * p.C + c] = static_cast<T>(v * p.scale);
-      }
+  for (int i = 0; i < 4; ++i) s_sum[ry][cx * 4 + i] = acc[i];
+  __syncthreads();
+  if (threadIdx.x < kJoinCols) {
+    const int c = static_cast<int>(blockIdx.y) * kJoinCols + threadIdx.x;
+    if (c < p.C) {
+      float v = 0.f;
+      for (int i = 0; i < 32; ++i) v += s_sum[i][threadIdx.x];
+      static_cast<T*>(p.grad)[size_t(own.key) * p.C + c] = static_cast<T>(v * p.scale);
     }
-    __syncthreads();
   }
 }
 
 // ------------------------------------------------------------------ host side
 struct EmbPlan {
   int vec, lanes;
-  uint32_t chunk, chunks;
-  size_t keys_off, order_off, sort_off, sort_bytes, slab_off, cut_off, bytes;
+  uint32_t chunk, ctas;
+  size_t keys_off, order_off, sort_off, sort_bytes, slab_off, info_off, bytes;
 };
 static int emb_plan(const fgb_embedding_call& c, EmbPlan& p) {
   p.vec = row_pack(c.c, elem_bytes(c.dtype));
   const int packs = c.c / p.vec, width = std::min(packs, kEmbThreads);
   p.lanes = kEmbThreads / width;
-  // long chunks leave little in the slab, short ones make more of them: some 1000 threads for every SM before chunks grow
+  // long chunks leave less to be added up, short ones make more of them: some 1000 threads for every SM before chunks grow
   int64_t chunk = 8;
   while (chunk < 64 && c.n / (2 * chunk) * width >= int64_t(device_sm_count()) * 1024) chunk *= 2;
   p.chunk = static_cast<uint32_t>(chunk);
-  p.chunks = static_cast<uint32_t>(ceil_div(c.n, chunk));
+  p.ctas = static_cast<uint32_t>(ceil_div(c.n, chunk * p.lanes));
   const int64_t sort = fgb_pp_sorted_idx_workspace_bytes(c.n);
   if (sort < 0) return static_cast<int>(sort);
   p.sort_bytes = static_cast<size_t>(sort);
@@ -254,8 +314,8 @@ static int emb_plan(const fgb_embedding_call& c, EmbPlan& p) {
   p.order_off = align256(c.n * 4);
   p.sort_off = p.order_off + align256(c.n * 8);
   p.slab_off = p.sort_off + align256(sort);
-  p.cut_off = p.slab_off + align256(int64_t(p.chunks) * 2 * c.c * 4);
-  p.bytes = p.cut_off + align256((int64_t(p.chunks) + 1) * 4);
+  p.info_off = p.slab_off + align256(int64_t(p.ctas) * 2 * c.c * 4);
+  p.bytes = p.info_off + align256(int64_t(p.ctas) * static_cast<int64_t>(sizeof(EmbInfo)));
   return FGB_OK;
 }
 
@@ -289,8 +349,8 @@ static cudaError_t emb_sum(const EmbGrad& a, const EmbPlan& p, cudaStream_t s) {
   static PerDeviceTable configured;
   if (ensure_dynamic_smem(configured, embedding_sum_kernel<T, kVec>, smem) != FGB_OK) return cudaErrorInvalidConfiguration;
   LaunchErrors chain;
-  chain.add(launch_chained(embedding_sum_kernel<T, kVec>, dim3(static_cast<unsigned>(ceil_div(a.n, per_cta))), dim3(kEmbThreads), smem, s, a));
-  chain.add(launch_chained(embedding_join_kernel<T>, dim3(device_sm_count() * 4), dim3(kEmbThreads), 0, s, a));
+  chain.add(launch_chained(embedding_sum_kernel<T, kVec>, dim3(p.ctas), dim3(kEmbThreads), smem, s, a));
+  if (p.ctas > 1) chain.add(launch_chained(embedding_join_kernel<T>, dim3(p.ctas, static_cast<unsigned>(ceil_div(a.C, kJoinCols))), dim3(kEmbThreads), 0, s, a));
   return chain.first;
 }
 
@@ -341,13 +401,12 @@ extern "C" int fgb_embedding_backward(const fgb_embedding_call* c, void* stream)
   char* ws = static_cast<char*>(c->workspace);
   int32_t* keys = reinterpret_cast<int32_t*>(ws + p.keys_off);
   int64_t* order = reinterpret_cast<int64_t*>(ws + p.order_off);
-  uint32_t* cut = reinterpret_cast<uint32_t*>(ws + p.cut_off);
   const uint32_t n = static_cast<uint32_t>(c->n), rows = static_cast<uint32_t>(c->rows);
   const uint64_t halves = uint64_t(c->rows) * c->c * (elem_bytes(c->dtype) / 2);
   const int64_t units = std::max<int64_t>(c->n, static_cast<int64_t>(halves / 8));
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(ceil_div(units, kEmbThreads), 1), int64_t(device_sm_count()) * 8));
   cudaError_t e = launch_chained(embedding_keys_kernel, dim3(grid), dim3(kEmbThreads), 0, s, c->indices, c->index_bits == 64, n, rows, c->padding_idx, keys,
-                                 static_cast<uint16_t*>(c->grad_table), halves, cut, c->status, status_mirror(c->status));
+                                 static_cast<uint16_t*>(c->grad_table), halves, c->status, status_mirror(c->status));
   if (e != cudaSuccess) return cuda_status(e);
   if (n == 0) return launch_status();
   int key_bits = 1;
@@ -356,8 +415,8 @@ extern "C" int fgb_embedding_backward(const fgb_embedding_call* c, void* stream)
   if (rc != FGB_OK) return rc;
   EmbGrad a{};
   a.g = c->grad_out, a.grad = c->grad_table, a.keys = keys, a.order = order;
-  a.slab = reinterpret_cast<float*>(ws + p.slab_off), a.cut = cut;
-  a.n = n, a.rows = rows, a.chunk = p.chunk, a.chunks = p.chunks, a.C = c->c, a.scale = c->scale;
+  a.slab = reinterpret_cast<float*>(ws + p.slab_off), a.info = reinterpret_cast<EmbInfo*>(ws + p.info_off);
+  a.n = n, a.rows = rows, a.chunk = p.chunk, a.ctas = p.ctas, a.C = c->c, a.scale = c->scale;
   if (c->dtype == FGB_F16) e = FGB_BY_PACK(__half, p.vec, emb_sum)(a, p, s);
   else if (c->dtype == FGB_BF16) e = FGB_BY_PACK(__nv_bfloat16, p.vec, emb_sum)(a, p, s);
   else e = FGB_BY_PACK(float, p.vec, emb_sum)(a, p, s);

@@ -23,6 +23,12 @@
 namespace fgb {
 
 constexpr int kNormThreads = 256;
+constexpr int kNormCtas = 3;  // an SM; the backward kernels need some 80 registers a thread
+
+// Two fp32 operations an instruction: these kernels are as near the issue rate as the memory's
+struct F2 {
+  float x, y;
+};
 
 struct NormArgs {
   const void* x;
@@ -38,7 +44,7 @@ struct NormArgs {
   float eps;
   float* mean;           // [samples, G]
   float* rstd;
-  float* part;           // [blocks + samples - 1][2][C]
+  F2* part;              // [blocks + samples - 1][C]: mean and squared distance from it, or the sums of dz and dz h
   float* joined;         // backward: [samples, G][2] mean(q), mean(q h)
   void* dw;
   void* db;
@@ -46,61 +52,122 @@ struct NormArgs {
   int32_t* mirror;
 };
 
-// the samples a block of rows meets: first .. last; each block's first is the last of the one before
-__device__ __forceinline__ void samples_of_block(const NormArgs& a, uint32_t j, uint32_t& first, uint32_t& last) {
-  const uint32_t before = j == 0u ? 0u : a.ranges.begun_before(j * a.R);
-  first = before > 0u ? before - 1u : 0u;
-  if (j + 1u >= a.blocks) {
-    last = a.ranges.count - 1u;
-  } else {
-    const uint32_t k = a.ranges.begun_before((j + 1u) * a.R);
-    last = k > 0u ? k - 1u : 0u;
-  }
+__device__ __forceinline__ uint64_t bits(F2 v) { return uint64_t(__float_as_uint(v.y)) << 32 | __float_as_uint(v.x); }
+__device__ __forceinline__ F2 from_bits(uint64_t b) { return F2{__uint_as_float(static_cast<uint32_t>(b)), __uint_as_float(static_cast<uint32_t>(b >> 32))}; }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+  return from_bits(d);
 }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+  return from_bits(d);
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+  return from_bits(d);
+}
+__device__ __forceinline__ F2 both(float v) { return F2{v, v}; }
+__device__ __forceinline__ F2 neg2(F2 v) { return F2{-v.x, -v.y}; }
 
-template <bool kExact>
-__device__ __forceinline__ float sigmoid(float z) {
-  // 16-bit results: the fast exponential and reciprocal are exact to some 2^-21, far below the result's half step
-  return kExact ? 1.f / (1.f + expf(-z)) : __fdividef(1.f, 1.f + __expf(-z));
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float reciprocal_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 template <bool kExact>
-__device__ __forceinline__ float activate(float z, int act) {
-  return act == FGB_ACT_SILU ? (z == -INFINITY ? 0.f : z * sigmoid<kExact>(z)) : z;
+__device__ __forceinline__ F2 sigmoid(F2 z) {
+  if constexpr (kExact) return F2{1.f / (1.f + expf(-z.x)), 1.f / (1.f + expf(-z.y))};
+  // 16-bit results: the fast exponential and reciprocal are exact to some 2^-21, far below the result's half step
+  const F2 t = mul2(z, both(-1.44269504f));
+  const F2 d = add2(F2{exp2_fast(t.x), exp2_fast(t.y)}, both(1.f));
+  return F2{reciprocal_fast(d.x), reciprocal_fast(d.y)};
+}
+template <bool kExact, bool kSilu>
+__device__ __forceinline__ F2 activate(F2 z) {
+  if constexpr (!kSilu) return z;
+  return mul2(z, sigmoid<kExact>(z));
 }
 // dy * act'(z).  Every rounding is named: the kernels that call it have to agree on the last bit, so that q - mean(q) is zero
 // where a mean is of one value.
-template <bool kExact>
-__device__ __forceinline__ float activate_grad(float dy, float z, int act) {
-  if (act != FGB_ACT_SILU) return dy;
-  const float s = sigmoid<kExact>(z);
-  return __fmul_rn(dy, __fmul_rn(s, fmaf(z, __fsub_rn(1.f, s), 1.f)));
+template <bool kExact, bool kSilu>
+__device__ __forceinline__ F2 activate_grad(F2 dy, F2 z) {
+  if constexpr (!kSilu) return dy;
+  const F2 s = sigmoid<kExact>(z), y = mul2(z, s);
+  return mul2(dy, add2(fma2(neg2(y), s, y), s));  // s + z s (1 - s)
 }
 
-// What a thread keeps of its kVec channels for one sample
-template <int kVec>
-struct ChannelParams {
-  float mean[kVec], r[kVec], w[kVec], b[kVec];
-  __device__ __forceinline__ void load(const NormArgs& p, uint32_t s, int c0) {
+// kVec channels as pairs (a single one leaves the second of its pair unused)
+template <typename T, int kVec>
+struct Pairs {
+  static constexpr int kPairs = (kVec + 1) / 2;
+  using Ch = Channels<T, kVec>;
+  F2 v[kPairs];
+  __device__ __forceinline__ void unpack(const typename Ch::Raw& raw) {
+    float f[kVec];
+    Ch::unpack(raw, f);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const int c = c0 + i;
-      const size_t g = size_t(s) * p.G + c / p.cpg;
-      mean[i] = p.mean[g];
-      r[i] = p.rstd[g];
-      w[i] = p.w != nullptr ? load_param(p.w, p.param_dtype, c) : 1.f;
-      b[i] = p.b != nullptr ? load_param(p.b, p.param_dtype, c) : 0.f;
+    for (int i = 0; i < kPairs; ++i) v[i] = F2{f[2 * i], kVec > 1 ? f[(2 * i + 1) % kVec] : 0.f};
+  }
+  __device__ __forceinline__ typename Ch::Raw pack() const {
+    float f[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) f[i] = i % 2 ? v[i / 2].y : v[i / 2].x;
+    return Ch::pack(f);
+  }
+};
+
+// What a thread keeps of its kVec channels: weight and bias, and the statistics of a sample -- one value where the channels
+// lie in one group (kOne), which saves the registers of the others
+template <int kVec, bool kOne>
+struct ChannelParams {
+  static constexpr int kPairs = (kVec + 1) / 2, kStats = kOne ? 1 : kPairs;
+  F2 w[kPairs], b[kPairs], minus_mean[kStats], r[kStats];
+  __device__ __forceinline__ void load(const NormArgs& p, int c0) {
+    float fw[2 * kPairs], fb[2 * kPairs];
+#pragma unroll
+    for (int i = 0; i < 2 * kPairs; ++i) {
+      fw[i] = p.w != nullptr && i < kVec ? load_param(p.w, p.param_dtype, c0 + i) : 1.f;
+      fb[i] = p.b != nullptr && i < kVec ? load_param(p.b, p.param_dtype, c0 + i) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) w[i] = F2{fw[2 * i], fw[2 * i + 1]}, b[i] = F2{fb[2 * i], fb[2 * i + 1]};
+  }
+  // statistic `of` of the channels' groups: stride values apart
+  __device__ __forceinline__ static void gather(F2 (&to)[kStats], const float* of, int stride, const NormArgs& p, uint32_t s, int c0) {
+    const float* row = of + size_t(s) * p.G * stride;
+#pragma unroll
+    for (int i = 0; i < kStats; ++i) {
+      const float a = row[size_t((c0 + 2 * i) / p.cpg) * stride];
+      to[i] = F2{a, kOne || kVec == 1 ? a : row[size_t((c0 + 2 * i + 1) / p.cpg) * stride]};
     }
   }
-  __device__ __forceinline__ float h(float x, int i) const { return __fmul_rn(__fsub_rn(x, mean[i]), r[i]); }
-  __device__ __forceinline__ float z(float h, int i) const { return fmaf(h, w[i], b[i]); }
+  __device__ __forceinline__ void load_stats(const NormArgs& p, uint32_t s, int c0) {
+    gather(minus_mean, p.mean, 1, p, s, c0);
+#pragma unroll
+    for (int i = 0; i < kStats; ++i) minus_mean[i] = neg2(minus_mean[i]);
+    gather(r, p.rstd, 1, p, s, c0);
+  }
+  __device__ __forceinline__ F2 h(F2 x, int i) const { return mul2(add2(x, minus_mean[kOne ? 0 : i]), r[kOne ? 0 : i]); }
+  __device__ __forceinline__ F2 z(F2 h, int i) const { return fma2(h, w[i], b[i]); }
 };
 
 // ------------------------------------------------------------------ 1. sums
-template <typename T, int kVec, bool kBackward>
-__global__ void __launch_bounds__(kNormThreads) norm_sums_kernel(const NormArgs p) {
+template <typename T, int kVec, bool kOne, bool kBackward, bool kSilu>
+__global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_sums_kernel(const NormArgs p) {
   using Ch = Channels<T, kVec>;
+  using Raw = typename Ch::Raw;
+  using P = Pairs<T, kVec>;
   constexpr bool kExact = sizeof(T) == 4;
-  __shared__ float s_sum[kNormThreads * kVec * 2];
+  constexpr int kPairs = P::kPairs;
+  __shared__ F2 s_sum[2 * kPairs][kNormThreads];
   chain_release();
   chain_wait();
   if constexpr (!kBackward) p.ranges.check(p.status, p.mirror);
@@ -111,62 +178,73 @@ __global__ void __launch_bounds__(kNormThreads) norm_sums_kernel(const NormArgs 
   const int cx = threadIdx.x % width, ry = threadIdx.x / width;
   const bool active = ry < lanes;
   const int c0 = (pack0 + cx) * kVec;
-  uint32_t first, last;
-  samples_of_block(p, j, first, last);
   const uint32_t row0 = j * p.R, row1 = min(p.ranges.n, row0 + p.R);
+  ChannelParams<kVec, kOne> k;
+  if (kBackward && active) k.load(p, c0);
+  uint32_t first, last;
+  p.ranges.of_block(row0, row0 + p.R, j + 1u >= p.blocks, first, last);
   const T* x = static_cast<const T*>(p.x) + c0;
   const T* dy = static_cast<const T*>(p.dy) + c0;
   for (uint32_t s = first; s <= last; ++s) {
     const uint32_t lo = max(p.ranges.at(s), row0), hi = min(p.ranges.at(s + 1u), row1);
-    float sum0[kVec], sum1[kVec], pivot[kVec];
+    F2 sum0[kPairs], sum1[kPairs], minus_pivot[kPairs];
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) sum0[i] = sum1[i] = pivot[i] = 0.f;
+    for (int i = 0; i < kPairs; ++i) sum0[i] = sum1[i] = minus_pivot[i] = both(0.f);
     if (lo < hi && active) {
+      const size_t step = size_t(lanes) * p.C;
       if constexpr (!kBackward) {
         // distances from the range's first row: what cancels in sum1 - sum0^2 / n is at most its share of the rows
-        Ch::unpack(Ch::load(x + size_t(lo) * p.C), pivot);
-        auto add = [&](const typename Ch::Raw& raw) {
-          float v[kVec];
-          Ch::unpack(raw, v);
+        P pivot;
+        pivot.unpack(Ch::load(x + size_t(lo) * p.C));
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            const float d = v[i] - pivot[i];
-            sum0[i] += d;
-            sum1[i] = fmaf(d, d, sum1[i]);
+        for (int i = 0; i < kPairs; ++i) minus_pivot[i] = neg2(pivot.v[i]);
+        auto add = [&](const Raw& raw) {
+          P v;
+          v.unpack(raw);
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) {
+            const F2 d = add2(v.v[i], minus_pivot[i]);
+            sum0[i] = add2(sum0[i], d);
+            sum1[i] = fma2(d, d, sum1[i]);
           }
         };
+        constexpr int kRows = 8;
         uint32_t r = lo + ry;
-        for (; r + 3u * lanes < hi; r += 4u * lanes) {
-          typename Ch::Raw raw[4];
+        const T* px = x + size_t(r) * p.C;
+        for (; r + (kRows - 1u) * lanes < hi; r += kRows * lanes, px += kRows * step) {
+          Raw raw[kRows];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) raw[u] = Ch::load(x + size_t(r + u * lanes) * p.C);
+          for (int u = 0; u < kRows; ++u) raw[u] = Ch::load(px + u * step);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) add(raw[u]);
+          for (int u = 0; u < kRows; ++u) add(raw[u]);
         }
-        for (; r < hi; r += lanes) add(Ch::load(x + size_t(r) * p.C));
+        for (; r < hi; r += lanes, px += step) add(Ch::load(px));
       } else {
-        ChannelParams<kVec> k;
-        k.load(p, s, c0);
-        auto add = [&](const typename Ch::Raw& raw, const typename Ch::Raw& raw_dy) {
-          float v[kVec], g[kVec];
-          Ch::unpack(raw, v);
-          Ch::unpack(raw_dy, g);
+        k.load_stats(p, s, c0);
+        auto add = [&](const Raw& raw, const Raw& raw_dy) {
+          P v, g;
+          v.unpack(raw);
+          g.unpack(raw_dy);
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            const float h = k.h(v[i], i);
-            const float dz = activate_grad<kExact>(g[i], k.z(h, i), p.act);
-            sum0[i] += dz;
-            sum1[i] = fmaf(dz, h, sum1[i]);
+          for (int i = 0; i < kPairs; ++i) {
+            const F2 h = k.h(v.v[i], i);
+            const F2 dz = activate_grad<kExact, kSilu>(g.v[i], k.z(h, i));
+            sum0[i] = add2(sum0[i], dz);
+            sum1[i] = fma2(dz, h, sum1[i]);
           }
         };
+        constexpr int kRows = 4;
         uint32_t r = lo + ry;
-        for (; r + lanes < hi; r += 2u * lanes) {
-          const typename Ch::Raw x0 = Ch::load(x + size_t(r) * p.C), x1 = Ch::load(x + size_t(r + lanes) * p.C);
-          const typename Ch::Raw g0 = Ch::load(dy + size_t(r) * p.C), g1 = Ch::load(dy + size_t(r + lanes) * p.C);
-          add(x0, g0);
-          add(x1, g1);
+        const T* px = x + size_t(r) * p.C;
+        const T* pg = dy + size_t(r) * p.C;
+        for (; r + (kRows - 1u) * lanes < hi; r += kRows * lanes, px += kRows * step, pg += kRows * step) {
+          Raw raw[kRows], raw_dy[kRows];
+#pragma unroll
+          for (int u = 0; u < kRows; ++u) raw[u] = Ch::load(px + u * step), raw_dy[u] = Ch::load(pg + u * step);
+#pragma unroll
+          for (int u = 0; u < kRows; ++u) add(raw[u], raw_dy[u]);
         }
-        if (r < hi) add(Ch::load(x + size_t(r) * p.C), Ch::load(dy + size_t(r) * p.C));
+        for (; r < hi; r += lanes, px += step, pg += step) add(Ch::load(px), Ch::load(pg));
       }
     }
     // the row lanes' sums: halved until one is left (always in the same order)
@@ -174,36 +252,29 @@ __global__ void __launch_bounds__(kNormThreads) norm_sums_kernel(const NormArgs 
       const int half = (m + 1) / 2;
       if (active && ry >= half && ry < m) {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          s_sum[i * kNormThreads + threadIdx.x] = sum0[i];
-          s_sum[(kVec + i) * kNormThreads + threadIdx.x] = sum1[i];
-        }
+        for (int i = 0; i < kPairs; ++i) s_sum[i][threadIdx.x] = sum0[i], s_sum[kPairs + i][threadIdx.x] = sum1[i];
       }
       __syncthreads();
       if (ry < m - half) {
         const int from = threadIdx.x + half * width;
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          sum0[i] += s_sum[i * kNormThreads + from];
-          sum1[i] += s_sum[(kVec + i) * kNormThreads + from];
-        }
+        for (int i = 0; i < kPairs; ++i) sum0[i] = add2(sum0[i], s_sum[i][from]), sum1[i] = add2(sum1[i], s_sum[kPairs + i][from]);
       }
       __syncthreads();
       m = half;
     }
     if (ry == 0) {
-      float* out = p.part + size_t(j + s) * 2 * p.C + c0;
+      F2* out = p.part + size_t(j + s) * p.C + c0;
       const float n = lo < hi ? static_cast<float>(hi - lo) : 1.f;
 #pragma unroll
       for (int i = 0; i < kVec; ++i) {
+        const float v0 = i % 2 ? sum0[i / 2].y : sum0[i / 2].x, v1 = i % 2 ? sum1[i / 2].y : sum1[i / 2].x;
         if constexpr (kBackward) {
-          out[i] = sum0[i];
-          out[p.C + i] = sum1[i];
+          out[i] = F2{v0, v1};
         } else {
-          const float d = sum0[i] / n;
-          out[i] = pivot[i] + d;                              // mean
-          out[p.C + i] = fmaxf(fmaf(-sum0[i], d, sum1[i]), 0.f);  // squared distance from it
-          if (isnan(sum1[i])) out[p.C + i] = sum1[i];
+          const float d = v0 / n, within = fmaf(-v0, d, v1);
+          // mean and squared distance from it (not below zero; a NaN stays)
+          out[i] = F2{d - (i % 2 ? minus_pivot[i / 2].y : minus_pivot[i / 2].x), within < 0.f ? 0.f : within};
         }
       }
     }
@@ -226,33 +297,35 @@ __device__ __forceinline__ double sum_of_threads(double v, double* s_red) {
   return v;
 }
 
-// kThreads threads of the CTA's 256 take one (sample, group); backward: the CTAs from `join_ctas` on add up 32 columns each
+// kThreads threads of the CTA's 256 take one (sample, group); backward: the CTAs from `join_ctas` on add up eight columns each.
+// A unit's entries are (block, channel of the group): a thread keeps to one channel and takes every few blocks.
 template <int kThreads, bool kBackward>
 __global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const NormArgs p, uint32_t join_ctas) {
   __shared__ double s_red[kNormThreads / 32];
-  __shared__ float s_col[2][8][32];
+  __shared__ float s_col[2][32][8];
   chain_release();
   chain_wait();
   if (kBackward && blockIdx.x >= join_ctas) {
-    const int c = (blockIdx.x - join_ctas) * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
+    const int c = (blockIdx.x - join_ctas) * 8 + (threadIdx.x & 7), w = threadIdx.x >> 3;
     const uint32_t slots = p.blocks + p.ranges.count - 1u;
-    double db = 0, dw = 0;  // some thousand terms of fp32 sums each
+    float db = 0.f, dw = 0.f;
     if (c < p.C) {
-#pragma unroll 4
-      for (uint32_t k = w; k < slots; k += 8u) {
-        db += p.part[size_t(k) * 2 * p.C + c];
-        dw += p.part[size_t(k) * 2 * p.C + p.C + c];
+#pragma unroll 8
+      for (uint32_t k = w; k < slots; k += 32u) {
+        const F2 v = p.part[size_t(k) * p.C + c];
+        db += v.x, dw += v.y;
       }
     }
-    s_col[0][w][threadIdx.x & 31] = static_cast<float>(db);
-    s_col[1][w][threadIdx.x & 31] = static_cast<float>(dw);
+    s_col[0][w][threadIdx.x & 7] = db;
+    s_col[1][w][threadIdx.x & 7] = dw;
     __syncthreads();
-    if (w < 2 && c < p.C) {
+    const int which = threadIdx.x >> 3;
+    if (which < 2 && c < p.C) {
       float v = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v += s_col[w][i][threadIdx.x & 31];
-      if (w == 0 && p.db != nullptr) store_param(p.db, p.param_dtype, c, v);
-      if (w == 1 && p.dw != nullptr) store_param(p.dw, p.param_dtype, c, v);
+      for (int i = 0; i < 32; ++i) v += s_col[which][i][threadIdx.x & 7];
+      if (which == 0 && p.db != nullptr) store_param(p.db, p.param_dtype, c, v);
+      if (which == 1 && p.dw != nullptr) store_param(p.dw, p.param_dtype, c, v);
     }
     return;
   }
@@ -260,35 +333,53 @@ __global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const NormArgs 
   if (unit >= uint64_t(p.ranges.count) * p.G) return;  // whole warps; with 256 threads a unit whole CTAs
   const uint32_t s = static_cast<uint32_t>(unit / p.G), g = static_cast<uint32_t>(unit % p.G), t = threadIdx.x % kThreads;
   const uint32_t lo = p.ranges.at(s), hi = max(lo, p.ranges.at(s + 1u));
-  const uint32_t j0 = lo / p.R, entries = lo < hi ? ((hi - 1u) / p.R - j0 + 1u) * p.cpg : 0u;
-  const double count = static_cast<double>(hi - lo) * p.cpg;
-  const float* part = p.part + size_t(j0 + s) * 2 * p.C + g * p.cpg;
-  auto rows_of = [&](uint32_t k) { return min(hi, (j0 + k + 1u) * p.R) - max(lo, (j0 + k) * p.R); };
+  const uint32_t j0 = lo / p.R, blocks = lo < hi ? (hi - 1u) / p.R - j0 + 1u : 0u;
+  const uint32_t cpg = p.cpg, across = min(cpg, static_cast<uint32_t>(kThreads)), down = kThreads / across;
+  const uint32_t c_own = t % across, k_own = t / across;
+  const double count = static_cast<double>(hi - lo) * cpg;
+  const F2* part = p.part + size_t(j0 + s) * p.C + g * cpg;
   double v0 = 0, v1 = 0;
   if constexpr (!kBackward) {
-    for (uint32_t e = t; e < entries; e += kThreads) {
-      const uint32_t k = e / p.cpg, c = e - k * p.cpg;
-      v0 += static_cast<double>(rows_of(k)) * part[size_t(k) * 2 * p.C + c];
+    // with d = (a block's mean) - (the first block's): mean = first + sum n d / count, and the squared distances from it are
+    // those within the blocks + sum n d^2 - (sum n d)^2 / count, all in 64 bits
+    const double pivot = blocks > 0u ? part[0].x : 0.f;
+    if (k_own < down) {
+      for (uint32_t c = c_own; c < cpg; c += across) {
+#pragma unroll 8
+        for (uint32_t k = k_own; k < blocks; k += down) {
+          const F2 v = part[size_t(k) * p.C + c];
+          const double rows = static_cast<double>(min(hi, (j0 + k + 1u) * p.R) - max(lo, (j0 + k) * p.R)), d = v.x - pivot;
+          v0 += rows * d;
+          v1 += v.y + rows * d * d;
+        }
+      }
     }
-    const double mean = entries > 0u ? sum_of_threads<kThreads>(v0, s_red) / count : 0.0;
-    for (uint32_t e = t; e < entries; e += kThreads) {
-      const uint32_t k = e / p.cpg, c = e - k * p.cpg;
-      const double d = part[size_t(k) * 2 * p.C + c] - mean;
-      v1 += part[size_t(k) * 2 * p.C + p.C + c] + rows_of(k) * d * d;
+    double mean = 0, var = 0;
+    if (blocks > 0u) {
+      v0 = sum_of_threads<kThreads>(v0, s_red) / count;
+      v1 = sum_of_threads<kThreads>(v1, s_red) / count;
+      mean = pivot + v0, var = v1 - v0 * v0;
+      if (var < 0) var = 0;
     }
-    const double var = entries > 0u ? sum_of_threads<kThreads>(v1, s_red) / count : 0.0;
     if (t == 0) {
       p.mean[unit] = static_cast<float>(mean);
       p.rstd[unit] = static_cast<float>(1.0 / sqrt(var + static_cast<double>(p.eps)));
     }
   } else {
-    for (uint32_t e = t; e < entries; e += kThreads) {
-      const uint32_t k = e / p.cpg, c = e - k * p.cpg;
-      const double w = p.w != nullptr ? load_param(p.w, p.param_dtype, g * p.cpg + c) : 1.f;
-      v0 += w * part[size_t(k) * 2 * p.C + c];
-      v1 += w * part[size_t(k) * 2 * p.C + p.C + c];
+    if (k_own < down) {
+      for (uint32_t c = c_own; c < cpg; c += across) {
+        const double w = p.w != nullptr ? load_param(p.w, p.param_dtype, g * cpg + c) : 1.f;
+        double q0 = 0, q1 = 0;
+#pragma unroll 8
+        for (uint32_t k = k_own; k < blocks; k += down) {
+          const F2 v = part[size_t(k) * p.C + c];
+          q0 += v.x, q1 += v.y;
+        }
+        v0 += w * q0;
+        v1 += w * q1;
+      }
     }
-    if (entries > 0u) {
+    if (blocks > 0u) {
       v0 = sum_of_threads<kThreads>(v0, s_red) / count;
       v1 = sum_of_threads<kThreads>(v1, s_red) / count;
     }
@@ -300,10 +391,13 @@ __global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const NormArgs 
 }
 
 // ------------------------------------------------------------------ 3. apply
-template <typename T, int kVec, bool kBackward>
-__global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(const NormArgs p) {
+template <typename T, int kVec, bool kOne, bool kBackward, bool kSilu>
+__global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_apply_kernel(const NormArgs p) {
   using Ch = Channels<T, kVec>;
+  using Raw = typename Ch::Raw;
+  using P = Pairs<T, kVec>;
   constexpr bool kExact = sizeof(T) == 4;
+  constexpr int kPairs = P::kPairs;
   chain_release();
   chain_wait();
   const uint32_t j = p.blocks - 1u - blockIdx.x;
@@ -311,68 +405,74 @@ __global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(const NormArgs
   const int width = min(kNormThreads, packs - pack0), lanes = kNormThreads / width;
   const int cx = threadIdx.x % width, ry = threadIdx.x / width;
   const int c0 = (pack0 + cx) * kVec;
-  uint32_t first, last;
-  samples_of_block(p, j, first, last);  // whole warps take part
-  if (ry >= lanes) return;
   const uint32_t row0 = j * p.R, row1 = min(p.ranges.n, row0 + p.R);
+  ChannelParams<kVec, kOne> k;
+  if (ry < lanes) k.load(p, c0);
+  uint32_t first, last;
+  p.ranges.of_block(row0, row0 + p.R, j + 1u >= p.blocks, first, last);  // whole warps take part
+  if (ry >= lanes) return;
   const T* x = static_cast<const T*>(p.x) + c0;
   const T* dy = static_cast<const T*>(p.dy) + c0;
   T* out = static_cast<T*>(p.out) + c0;
+  const size_t step = size_t(lanes) * p.C;
   for (uint32_t s = first; s <= last; ++s) {
     const uint32_t lo = max(p.ranges.at(s), row0), hi = min(p.ranges.at(s + 1u), row1);
     if (lo >= hi) continue;
-    ChannelParams<kVec> k;
-    k.load(p, s, c0);
+    k.load_stats(p, s, c0);
+    uint32_t r = lo + ry;
+    size_t at = size_t(r) * p.C;
+    constexpr int kRows = 4;
     if constexpr (!kBackward) {
-      auto one = [&](const typename Ch::Raw& raw, uint32_t r) {
-        float v[kVec];
-        Ch::unpack(raw, v);
+      auto one = [&](const Raw& raw) {
+        P v;
+        v.unpack(raw);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) v[i] = activate<kExact>(k.z(k.h(v[i], i), i), p.act);
-        Ch::store(out + size_t(r) * p.C, Ch::pack(v));
+        for (int i = 0; i < kPairs; ++i) v.v[i] = activate<kExact, kSilu>(k.z(k.h(v.v[i], i), i));
+        return v.pack();
       };
-      uint32_t r = lo + ry;
-      for (; r + 3u * lanes < hi; r += 4u * lanes) {
-        typename Ch::Raw raw[4];
+      for (; r + (kRows - 1u) * lanes < hi; r += kRows * lanes, at += kRows * step) {
+        Raw raw[kRows];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) raw[u] = Ch::load(x + size_t(r + u * lanes) * p.C);
+        for (int u = 0; u < kRows; ++u) raw[u] = Ch::load(x + at + u * step);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) one(raw[u], r + u * lanes);
+        for (int u = 0; u < kRows; ++u) Ch::store(out + at + u * step, one(raw[u]));
       }
-      for (; r < hi; r += lanes) one(Ch::load(x + size_t(r) * p.C), r);
+      for (; r < hi; r += lanes, at += step) Ch::store(out + at, one(Ch::load(x + at)));
     } else {
-      float m1[kVec], m2[kVec];
+      constexpr int kStats = ChannelParams<kVec, kOne>::kStats;
+      F2 minus_m1[kStats], m2[kStats];
+      ChannelParams<kVec, kOne>::gather(minus_m1, p.joined, 2, p, s, c0);
+      ChannelParams<kVec, kOne>::gather(m2, p.joined + 1, 2, p, s, c0);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        const size_t g = size_t(s) * p.G + (c0 + i) / p.cpg;
-        m1[i] = p.joined[g * 2], m2[i] = p.joined[g * 2 + 1];
-      }
-      auto one = [&](const typename Ch::Raw& raw, const typename Ch::Raw& raw_dy, uint32_t r) {
-        float v[kVec], g[kVec];
-        Ch::unpack(raw, v);
-        Ch::unpack(raw_dy, g);
+      for (int i = 0; i < kStats; ++i) minus_m1[i] = neg2(minus_m1[i]);
+      auto one = [&](const Raw& raw, const Raw& raw_dy) {
+        P v, g;
+        v.unpack(raw);
+        g.unpack(raw_dy);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          const float h = k.h(v[i], i);
-          const float q = __fmul_rn(activate_grad<kExact>(g[i], k.z(h, i), p.act), k.w[i]);
-          v[i] = k.r[i] * fmaf(-h, m2[i], __fsub_rn(q, m1[i]));
+        for (int i = 0; i < kPairs; ++i) {
+          const F2 h = k.h(v.v[i], i), dz = activate_grad<kExact, kSilu>(g.v[i], k.z(h, i));
+          // not mul2: the compiler joins that with the subtraction of the mean to one operation with one rounding
+          const F2 q = F2{__fmul_rn(dz.x, k.w[i].x), __fmul_rn(dz.y, k.w[i].y)};
+          const int t = kOne ? 0 : i;
+          v.v[i] = mul2(k.r[t], fma2(neg2(h), m2[t], add2(q, minus_m1[t])));
         }
-        Ch::store(out + size_t(r) * p.C, Ch::pack(v));
+        return v.pack();
       };
-      uint32_t r = lo + ry;
-      for (; r + lanes < hi; r += 2u * lanes) {
-        const typename Ch::Raw x0 = Ch::load(x + size_t(r) * p.C), x1 = Ch::load(x + size_t(r + lanes) * p.C);
-        const typename Ch::Raw g0 = Ch::load(dy + size_t(r) * p.C), g1 = Ch::load(dy + size_t(r + lanes) * p.C);
-        one(x0, g0, r);
-        one(x1, g1, r + lanes);
+      for (; r + (kRows - 1u) * lanes < hi; r += kRows * lanes, at += kRows * step) {
+        Raw raw[kRows], raw_dy[kRows];
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) raw[u] = Ch::load(x + at + u * step), raw_dy[u] = Ch::load(dy + at + u * step);
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) Ch::store(out + at + u * step, one(raw[u], raw_dy[u]));
       }
-      if (r < hi) one(Ch::load(x + size_t(r) * p.C), Ch::load(dy + size_t(r) * p.C), r);
+      for (; r < hi; r += lanes, at += step) Ch::store(out + at, one(Ch::load(x + at), Ch::load(dy + at)));
     }
   }
   // rows of no sample
   const uint32_t begin = p.ranges.at(0u), end = max(begin, p.ranges.at(p.ranges.count));
   if (row0 >= begin && row1 <= end) return;
-  typename Ch::Raw zero{};
+  Raw zero{};
   for (uint32_t r = row0 + ry; r < row1; r += lanes)
     if (r < begin || r >= end) Ch::store(out + size_t(r) * p.C, zero);
 }
@@ -380,6 +480,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(const NormArgs
 // ------------------------------------------------------------------ host side
 struct NormPlan {
   int vec;
+  bool one;           // a pack lies in one group
   unsigned columns;   // CTAs along a row
   uint32_t R, blocks;
   size_t joined_off, bytes;
@@ -387,11 +488,13 @@ struct NormPlan {
 static NormPlan norm_plan(const fgb_group_norm_call& c) {
   NormPlan p;
   p.vec = row_pack(c.c, elem_bytes(c.dtype));
+  if (p.vec == 8 && c.c / c.groups % 8 != 0) p.vec = 4;  // eight channels of several groups would take too many registers
+  p.one = c.c / c.groups % p.vec == 0;
   const int packs = c.c / p.vec;
   p.columns = static_cast<unsigned>(ceil_div(packs, kNormThreads));
   const int width = packs < kNormThreads ? packs : kNormThreads, lanes = kNormThreads / width;
-  // four CTAs on every SM, each thread at least eight rows
-  const int64_t want = std::max<int64_t>(ceil_div(int64_t(device_sm_count()) * 4, p.columns), 1);
+  // as many CTAs as run at a time, each thread at least eight rows
+  const int64_t want = std::max<int64_t>(int64_t(device_sm_count()) * kNormCtas / p.columns, 1);
   const int64_t R = std::max<int64_t>(ceil_div(c.n, want), int64_t(lanes) * 8);
   p.R = static_cast<uint32_t>(R);
   p.blocks = static_cast<uint32_t>(std::max<int64_t>(ceil_div(c.n, R), 1));
@@ -412,8 +515,8 @@ static int norm_check(const fgb_group_norm_call* c) {
   return FGB_OK;
 }
 
-template <typename T, int kVec>
-static int norm_run(const NormArgs& a, const NormPlan& p, bool backward, bool want_out, bool want_param, cudaStream_t s) {
+template <typename T, int kVec, bool kOne, bool kSilu>
+static int norm_run_act(const NormArgs& a, const NormPlan& p, bool backward, bool want_out, bool want_param, cudaStream_t s) {
   const dim3 grid(p.blocks, p.columns);
   LaunchErrors chain;
   const int64_t units = int64_t(a.ranges.count) * a.G;
@@ -421,16 +524,22 @@ static int norm_run(const NormArgs& a, const NormPlan& p, bool backward, bool wa
   const bool warps = int64_t(p.blocks) * a.cpg / a.ranges.count < 64;
   const uint32_t join = static_cast<uint32_t>(warps ? ceil_div(units, kNormThreads / 32) : units);
   if (!backward) {
-    chain.add(launch_chained(norm_sums_kernel<T, kVec, false>, grid, dim3(kNormThreads), 0, s, a));
+    chain.add(launch_chained(norm_sums_kernel<T, kVec, kOne, false, false>, grid, dim3(kNormThreads), 0, s, a));
     chain.add(launch_chained(warps ? norm_join_kernel<32, false> : norm_join_kernel<kNormThreads, false>, dim3(join), dim3(kNormThreads), 0, s, a, join));
-    chain.add(launch_chained(norm_apply_kernel<T, kVec, false>, grid, dim3(kNormThreads), 0, s, a));
+    chain.add(launch_chained(norm_apply_kernel<T, kVec, kOne, false, kSilu>, grid, dim3(kNormThreads), 0, s, a));
   } else {
-    chain.add(launch_chained(norm_sums_kernel<T, kVec, true>, grid, dim3(kNormThreads), 0, s, a));
-    const unsigned cols = want_param ? static_cast<unsigned>(ceil_div(a.C, 32)) : 0u;
+    chain.add(launch_chained(norm_sums_kernel<T, kVec, kOne, true, kSilu>, grid, dim3(kNormThreads), 0, s, a));
+    const unsigned cols = want_param ? static_cast<unsigned>(ceil_div(a.C, 8)) : 0u;
     chain.add(launch_chained(warps ? norm_join_kernel<32, true> : norm_join_kernel<kNormThreads, true>, dim3(join + cols), dim3(kNormThreads), 0, s, a, join));
-    if (want_out) chain.add(launch_chained(norm_apply_kernel<T, kVec, true>, grid, dim3(kNormThreads), 0, s, a));
+    if (want_out) chain.add(launch_chained(norm_apply_kernel<T, kVec, kOne, true, kSilu>, grid, dim3(kNormThreads), 0, s, a));
   }
   return chain.first != cudaSuccess ? cuda_status(chain.first) : launch_status();
+}
+
+template <typename T, int kVec, bool kOne>
+static int norm_run(const NormArgs& a, const NormPlan& p, bool backward, bool want_out, bool want_param, cudaStream_t s) {
+  return a.act == FGB_ACT_SILU ? norm_run_act<T, kVec, kOne, true>(a, p, backward, want_out, want_param, s)
+                               : norm_run_act<T, kVec, kOne, false>(a, p, backward, want_out, want_param, s);
 }
 
 static int norm_call(const fgb_group_norm_call* c, bool backward, cudaStream_t s) {
@@ -451,27 +560,22 @@ static int norm_call(const fgb_group_norm_call* c, bool backward, cudaStream_t s
   a.R = p.R, a.blocks = p.blocks;
   a.w = c->weight, a.b = c->bias, a.param_dtype = c->param_dtype, a.act = c->act, a.eps = c->eps;
   a.mean = c->mean, a.rstd = c->rstd;
-  a.part = static_cast<float*>(c->workspace);
+  a.part = static_cast<F2*>(c->workspace);
   a.joined = reinterpret_cast<float*>(static_cast<char*>(c->workspace) + p.joined_off);
   a.dw = c->grad_weight, a.db = c->grad_bias;
   a.status = c->status, a.mirror = status_mirror(c->status);
   const bool want_out = c->out != nullptr;
-  switch (c->dtype) {
-    case FGB_F16:
-      return p.vec == 8   ? norm_run<__half, 8>(a, p, backward, want_out, want_param, s)
-             : p.vec == 4 ? norm_run<__half, 4>(a, p, backward, want_out, want_param, s)
-             : p.vec == 2 ? norm_run<__half, 2>(a, p, backward, want_out, want_param, s)
-                          : norm_run<__half, 1>(a, p, backward, want_out, want_param, s);
-    case FGB_BF16:
-      return p.vec == 8   ? norm_run<__nv_bfloat16, 8>(a, p, backward, want_out, want_param, s)
-             : p.vec == 4 ? norm_run<__nv_bfloat16, 4>(a, p, backward, want_out, want_param, s)
-             : p.vec == 2 ? norm_run<__nv_bfloat16, 2>(a, p, backward, want_out, want_param, s)
-                          : norm_run<__nv_bfloat16, 1>(a, p, backward, want_out, want_param, s);
-    default:
-      return p.vec == 4   ? norm_run<float, 4>(a, p, backward, want_out, want_param, s)
-             : p.vec == 2 ? norm_run<float, 2>(a, p, backward, want_out, want_param, s)
-                          : norm_run<float, 1>(a, p, backward, want_out, want_param, s);
-  }
+#define FGB_NORM(T, v, one) norm_run<T, v, one>(a, p, backward, want_out, want_param, s)
+#define FGB_NORM_16(T)                                                   \
+  (p.vec == 8   ? FGB_NORM(T, 8, true)                                   \
+   : p.vec == 4 ? (p.one ? FGB_NORM(T, 4, true) : FGB_NORM(T, 4, false)) \
+   : p.vec == 2 ? FGB_NORM(T, 2, false)                                  \
+                : FGB_NORM(T, 1, true))
+  if (c->dtype == FGB_F16) return FGB_NORM_16(__half);
+  if (c->dtype == FGB_BF16) return FGB_NORM_16(__nv_bfloat16);
+  return p.vec == 4 ? (p.one ? FGB_NORM(float, 4, true) : FGB_NORM(float, 4, false)) : p.vec == 2 ? FGB_NORM(float, 2, false) : FGB_NORM(float, 1, true);
+#undef FGB_NORM_16
+#undef FGB_NORM
 }
 
 // ------------------------------------------------------------------ row ranges of the samples

@@ -45,6 +45,21 @@ struct RowRanges {
     }
     return lo;
   }
+  // the samples that a block of rows [row0, row1) meets: first .. last; a block's first is the last of the block before.  The
+  // whole warp calls it.
+  __device__ __forceinline__ void of_block(uint32_t row0, uint32_t row1, bool last_block, uint32_t& first, uint32_t& last) const {
+    uint32_t a, b;
+    if (count <= 32u) {  // one load for both
+      const uint32_t lane = threadIdx.x & 31u, v = lane < count ? at(lane) : 0xFFFFFFFFu;
+      a = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, v < row0)));
+      b = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, v < row1)));
+    } else {
+      a = row0 == 0u ? 0u : begun_before(row0);
+      b = last_block ? count : begun_before(row1);
+    }
+    first = a > 0u ? a - 1u : 0u;
+    last = last_block ? count - 1u : b > 0u ? b - 1u : 0u;
+  }
   // every entry of the grid's share is looked at; threads of the whole grid call it
   __device__ __forceinline__ void check(int32_t* status, int32_t* mirror) const {
     if (offsets == nullptr) return;
