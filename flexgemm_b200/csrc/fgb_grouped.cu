@@ -16,10 +16,12 @@
 // Warps: 0-7 store tiles (two per quarter of the accumulator rows), 8 loads (TMA), 9 multiplies; two accumulators in TMEM
 // where they fit, so that a tile is stored while the next is multiplied.
 //
-// Work is a line of iterations (one stage each): the tiles of group 0, then group 1, ..., a tile's iterations together.
-// Where every CTA has several tiles to do, the line is cut at tiles; otherwise (the weight gradient; a few rows) into equal
-// ranges, one for each CTA: a tile that lies in several ranges leaves fp32 pieces in a slab, which a second kernel adds up
-// in their order.  What each CTA does follows from the sizes alone, so results do not depend on the run.
+// Work is dealt out in units, one after the other to the CTAs in turn: a tile, or where there are too few tiles to go round
+// (the weight gradient; a few rows) one of the equal parts of its iterations (a stage each).  The parts of a group's tiles that
+// read the same k are neighbours, so that they find it in L2: equal ranges of one long line of iterations, which need no
+// rounding up, read everything from memory once for each tile (16 groups of 8192 rows, 1024 x 1024: 422 us).  A tile in parts
+// leaves fp32 pieces in a slab, which a second kernel adds up in their order.  Every CTA finds the number of parts from the
+// sizes alone, so results do not depend on the run.
 //
 // fp32 operands are written as sums of bf16 planes (hi + mid + lo, 8 bits each) and multiplied plane by plane: six products
 // (all whose weight is 2^-16 and more) for accurate fp32, three (2^-8 and more) where TF32 is allowed.  bf16 has
@@ -41,9 +43,9 @@ constexpr int kGrThreads = 320;
 constexpr int kGrEpilogueWarps = 8;
 constexpr int kGrMaxStages = 12;
 constexpr int kGrMaxGroups = 2048;
-constexpr int kGrCtrlBytes = 1024 + 2048 + 2048;  // barriers; a block of ones; bias of a pass for each warp
-constexpr int kGrStoreBytes = kGrEpilogueWarps * 2048;
-constexpr int kGrSmemLimit = 227 * 1024;
+constexpr int kGrCtrlBytes = 1024 + 4096;  // barriers; a block of ones (kWeight) or the storing warps' bias (kRows)
+constexpr int kGrStoreBytes = kGrEpilogueWarps * 4096;
+constexpr int kGrSmemLimit = 226 * 1024;  // of dynamic shared memory, beside 1 KB of static
 constexpr int kGrPBytes = 128 * 128;
 
 enum { kRows = 0, kFew = 1, kWeight = 2 };
@@ -51,6 +53,7 @@ enum { kRows = 0, kFew = 1, kWeight = 2 };
 struct GroupedArgs {
   RowRanges ranges;
   int bn;               // columns of a tile
+  int tile_m;           // rows of it: 128, or 256 of a pair of CTAs
   int n_tiles;          // tiles along the channels that are not rows: kRows along n, kFew along m, kWeight along n
   int m_tiles;          // kWeight: tiles along co
   int k_blocks;         // kRows, kFew: blocks of 64 along k
@@ -59,13 +62,15 @@ struct GroupedArgs {
   uint32_t p_planes, q_planes;  // their planes, four bits a term
   int p_mn, q_mn;       // operand is MN-major
   int stages, q_bytes, acc_sets, acc_stride;
-  uint32_t min_range;   // iterations that a range has at least; 0: a range is a tile
+  uint32_t min_part;    // iterations that a part of a tile has at least; 0: tiles are not cut
+  uint32_t piece_cost;  // what writing and adding up a piece takes, in iterations
   uint32_t idesc, idesc_ones;
   uint32_t one_pair;    // two ones of the operand type
   const void* bias;     // [groups, nout] or null
   void* out;
   void* db;             // kWeight: [groups, co] or null
-  float* slab;          // pieces of tiles that lie in several ranges
+  float* slab;          // pieces of tiles: [tile_m][bn] each (kFew [bn][128])
+  float* db_parts;      // kWeight: [units][tile_m], the unit's share of db
   int m_extent, n_extent;  // channels: kRows n; kFew m; kWeight m and n
   int out_ld;
   int vec_ok;           // rows of the output are whole 16-byte pieces
@@ -75,115 +80,174 @@ struct GroupedArgs {
 
 struct GroupedSmem {
   uint64_t full[kGrMaxStages], empty[kGrMaxStages];
+  uint64_t peer_full[kGrMaxStages];  // pairs: the other CTA has cleared its operands of a stage
   uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem_base, abort_flag;
 };
 static_assert(sizeof(GroupedSmem) <= 1024, "control block too large");
 
-// iterations that group g has: tiles x blocks x terms
+// The rows, tiles and iterations a tile of group g; `offsets` are those of the groups in shared memory
+struct GroupSize {
+  uint32_t lo, hi, tiles, whole;
+};
 template <int kMode>
-__device__ __forceinline__ uint32_t group_iterations(const GroupedArgs& p, uint32_t g) {
-  const uint32_t lo = p.ranges.at(g), hi = p.ranges.at(g + 1u), len = hi > lo ? hi - lo : 0u;
-  if constexpr (kMode == kRows) return (len + 127u) / 128u * p.n_tiles * p.k_blocks * p.terms;
-  else if constexpr (kMode == kFew) return (len + p.bn - 1u) / p.bn * p.n_tiles * p.k_blocks * p.terms;
-  else return (len + 63u) / 64u * p.terms * p.n_tiles * p.m_tiles;
+__device__ __forceinline__ GroupSize group_size(const GroupedArgs& p, const uint32_t* offsets, uint32_t g) {  // tiles of tile_m rows, or of bn where n is rows
+  GroupSize s;
+  s.lo = offsets[g];
+  s.hi = offsets[g + 1u];
+  const uint32_t len = s.hi - s.lo;
+  if constexpr (kMode == kRows) s.tiles = (len + p.tile_m - 1u) / p.tile_m * p.n_tiles;
+  else if constexpr (kMode == kFew) s.tiles = (len + p.bn - 1u) / p.bn * p.n_tiles;
+  else s.tiles = len > 0u ? p.n_tiles * p.m_tiles : 0u;
+  s.whole = static_cast<uint32_t>((kMode == kWeight ? (len + 63u) / 64u : p.k_blocks) * p.terms);
+  return s;
 }
+// length of the parts of a tile of `whole` iterations where `unit` are wanted: whole blocks of k, all parts but the last alike
+__device__ __forceinline__ uint32_t part_length(const GroupedArgs& p, uint32_t whole, uint32_t unit) {
+  if (p.min_part == 0u || whole <= unit) return whole;
+  const uint32_t parts = min((whole + unit - 1u) / unit, max(whole / p.min_part, 1u));
+  const uint32_t blocks = whole / p.terms;
+  return (blocks + parts - 1u) / parts * p.terms;
+}
+__device__ __forceinline__ uint32_t parts_of(uint32_t whole, uint32_t length) { return length == 0u ? 0u : (whole + length - 1u) / length; }
 
-// first[g] = iterations of the groups before g, first[groups] all of them; the whole CTA calls it (and waits at its end)
+// What every CTA works out at its start: first[g] = units of the groups before g, piece[g] = pieces of tiles before g, and
+// the length that parts should have.  The whole CTA calls it (and waits at its end).
+constexpr uint32_t kGrMostUnits = 3;  // units that a CTA gets on average where tiles are cut: 1, 2 or 3
+struct GroupedSchedule {
+  uint32_t* first;
+  uint32_t* piece;
+  uint32_t* offsets;
+  uint32_t unit;
+};
+inline int64_t schedule_bytes(int64_t groups) { return align256((groups + 1) * 12); }
 template <int kMode>
-__device__ __forceinline__ void plan_groups(const GroupedArgs& p, uint32_t* first) {
-  const uint32_t G = p.ranges.count;
+__device__ __forceinline__ GroupedSchedule plan_groups(const GroupedArgs& p, uint32_t* s_first, uint32_t ctas) {
+  __shared__ unsigned long long s_total;
+  __shared__ float s_cost[kGrMostUnits + 1];
+  __shared__ uint32_t s_unit[kGrMostUnits + 1];
+  const uint32_t G = p.ranges.count, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+  GroupedSchedule plan{s_first, s_first + G + 1u, s_first + 2u * (G + 1u), 0xFFFFFFFFu};
   bool bad = false;
-  for (uint32_t g = threadIdx.x; g < G; g += blockDim.x) {
-    first[g + 1u] = group_iterations<kMode>(p, g);
-    bad |= !p.ranges.good(g);
+  for (uint32_t g = threadIdx.x; g <= G; g += blockDim.x) {
+    plan.offsets[g] = p.ranges.at(g);
+    bad |= g < G && !p.ranges.good(g);
   }
   // ranges that overlap could ask for more tiles than there is room for: nothing is done
-  if (__syncthreads_or(bad)) {
-    for (uint32_t g = threadIdx.x; g < G; g += blockDim.x) first[g + 1u] = 0u;
-    __syncthreads();
+  bad = __syncthreads_or(bad) != 0;
+  if (bad && threadIdx.x == 0) {
+    report(p.status, FGB_S_BAD_OFFSETS);
+    mirror_code(p.mirror, FGB_S_BAD_OFFSETS);
   }
-  if (threadIdx.x < 32) {
-    const uint32_t lane = threadIdx.x;
-    uint32_t run = 0;
-    for (uint32_t g0 = 0; g0 < G; g0 += 32u) {
-      uint32_t v = g0 + lane < G ? first[g0 + lane + 1u] : 0u;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t o = __shfl_up_sync(0xffffffffu, v, d);
-        if (lane >= static_cast<uint32_t>(d)) v += o;
+  if (p.min_part != 0u && !bad) {
+    // the cost of uncut tiles, and of units of 1, 2 and 3 to a CTA: the CTA with the most work, and the pieces
+    if (warp == 0) {
+      unsigned long long total = 0;
+      for (uint32_t g = lane; g < G; g += 32u) {
+        const GroupSize z = group_size<kMode>(p, plan.offsets, g);
+        total += static_cast<unsigned long long>(z.tiles) * z.whole;
       }
-      if (g0 + lane < G) first[g0 + lane + 1u] = run + v;
-      run += __shfl_sync(0xffffffffu, v, 31);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+      if (lane == 0) s_total = total;
     }
-    if (lane == 0) first[0] = 0u;
+    __syncthreads();
+    if (warp <= kGrMostUnits) {
+      const unsigned long long total = s_total;
+      const uint32_t unit = warp == 0u ? 0xFFFFFFFFu : static_cast<uint32_t>((total + ctas * warp - 1u) / (ctas * warp));
+      uint32_t units = 0, pieces = 0, longest = 0, shortest = 0xFFFFFFFFu;
+      for (uint32_t g = lane; g < G; g += 32u) {
+        const GroupSize z = group_size<kMode>(p, plan.offsets, g);
+        if (z.tiles == 0u) continue;
+        const uint32_t len = part_length(p, z.whole, unit), parts = parts_of(z.whole, len);
+        units += parts * z.tiles;
+        if (parts > 1u) pieces += parts * z.tiles;
+        longest = max(longest, len), shortest = min(shortest, len);
+      }
+      units = __reduce_add_sync(0xffffffffu, units), pieces = __reduce_add_sync(0xffffffffu, pieces);
+      longest = __reduce_max_sync(0xffffffffu, longest), shortest = __reduce_min_sync(0xffffffffu, shortest);
+      if (lane == 0) {
+        const float share = static_cast<float>(total) / ctas;
+        const float most = longest == shortest ? static_cast<float>((units + ctas - 1u) / ctas) * longest : fmaxf(share + 0.5f * longest, longest);
+        s_cost[warp] = most + static_cast<float>(pieces) / ctas * p.piece_cost;
+        s_unit[warp] = unit;
+      }
+    }
+    __syncthreads();
+    uint32_t best = 0;
+#pragma unroll
+    for (uint32_t i = 1; i <= kGrMostUnits; ++i)
+      if (s_cost[i] < s_cost[best]) best = i;
+    plan.unit = s_unit[best];
+  }
+  for (uint32_t g = threadIdx.x; g < G; g += blockDim.x) {
+    const GroupSize z = group_size<kMode>(p, plan.offsets, g);
+    const uint32_t parts = bad ? 0u : parts_of(z.whole, part_length(p, z.whole, plan.unit));
+    plan.first[g + 1u] = parts * z.tiles;
+    plan.piece[g + 1u] = parts > 1u ? parts * z.tiles : 0u;
   }
   __syncthreads();
+  if (warp < 2) {
+    uint32_t* v = warp == 0 ? plan.first : plan.piece;
+    uint32_t run = 0;
+    for (uint32_t g0 = 0; g0 < G; g0 += 32u) {
+      uint32_t x = g0 + lane < G ? v[g0 + lane + 1u] : 0u;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t o = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= static_cast<uint32_t>(d)) x += o;
+      }
+      if (g0 + lane < G) v[g0 + lane + 1u] = run + x;
+      run += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) v[0] = 0u;
+  }
+  __syncthreads();
+  return plan;
 }
 
-// iterations of a range
-template <int kMode>
-__device__ __forceinline__ uint32_t range_length(const GroupedArgs& p, uint32_t total, uint32_t ctas) {
-  if (p.min_range == 0u) return static_cast<uint32_t>(p.k_blocks * p.terms);  // a tile
-  return max((total + ctas - 1u) / ctas, p.min_range);
-}
-
-// A tile, or the part of one that a range holds
+// A tile, or the part of one that is a unit
 struct GroupedItem {
   uint32_t group, tile;     // tile within the group
-  uint32_t from, to, whole; // its iterations, of `whole`
+  uint32_t from, to;        // its iterations
   uint32_t lo, hi;          // rows of the group
-  uint32_t range;
+  uint32_t piece;           // its place in the slab, or kInvalid for a whole tile
+  uint32_t unit;
 };
 
-// walks the items of a CTA's ranges: every role goes through the same sequence
+// walks the units of a CTA: every role goes through the same sequence
 template <int kMode>
 struct GroupedWalk {
   const GroupedArgs& p;
-  const uint32_t* first;
-  uint32_t total, length, range, at, end;
-  __device__ __forceinline__ GroupedWalk(const GroupedArgs& p_, const uint32_t* first_, uint32_t ctas, uint32_t cta) : p(p_), first(first_) {
-    total = first[p.ranges.count];
-    length = range_length<kMode>(p, total, ctas);
-    range = cta;
-    at = 0, end = 0;
-    step = ctas;
-    begin_range();
-  }
+  const GroupedSchedule& plan;
+  uint32_t at, step, total;
+  __device__ __forceinline__ GroupedWalk(const GroupedArgs& p_, const GroupedSchedule& plan_, uint32_t ctas, uint32_t cta)
+      : p(p_), plan(plan_), at(cta), step(ctas), total(plan_.first[p_.ranges.count]) {}
   __device__ __forceinline__ bool next(GroupedItem& it) {
-    if (at >= end) {
-      range += step;
-      begin_range();
-    }
-    if (at >= end) return false;
-    uint32_t lo = 0, hi = p.ranges.count - 1u;  // the last group that begins at or before `at` and is not empty
+    if (at >= total) return false;
+    uint32_t lo = 0, hi = p.ranges.count - 1u;  // the last group that begins at or before `at`: not an empty one
     while (lo < hi) {
       const uint32_t mid = (lo + hi + 1u) / 2u;
-      if (first[mid] <= at) lo = mid;
+      if (plan.first[mid] <= at) lo = mid;
       else hi = mid - 1u;
     }
+    const GroupSize z = group_size<kMode>(p, plan.offsets, lo);
+    const uint32_t length = part_length(p, z.whole, plan.unit), local = at - plan.first[lo], part = local / z.tiles;
     it.group = lo;
-    const uint32_t begin = p.ranges.at(lo), stop = p.ranges.at(lo + 1u);
-    it.lo = begin, it.hi = max(begin, stop);
-    it.whole = kMode == kWeight ? (it.hi - it.lo + 63u) / 64u * p.terms : static_cast<uint32_t>(p.k_blocks * p.terms);
-    const uint32_t local = at - first[lo];
-    it.tile = local / it.whole;
-    it.from = local - it.tile * it.whole;
-    it.to = min(it.whole, it.from + (end - at));
-    it.range = range;
-    at += it.to - it.from;
+    it.tile = local - part * z.tiles;
+    it.from = part * length, it.to = min(z.whole, it.from + length);
+    it.lo = z.lo, it.hi = z.hi;
+    it.piece = length < z.whole ? plan.piece[lo] + local : kInvalid;
+    it.unit = at;
+    at += step;
     return true;
   }
-
- private:
-  uint32_t step;
-  __device__ __forceinline__ void begin_range() {
-    // total and the number of ranges are below 2^31, checked on the host
-    const uint64_t a = uint64_t(range) * length;
-    at = a < total ? static_cast<uint32_t>(a) : total;
-    end = min(total, at + length);
-  }
 };
+
+// A value that all lanes of the warp have, in a form that tells the compiler so: TMA and MMA instructions take their operands
+// from registers that are uniform over the warp, and the loops around them have to be uniform for such registers to be used.
+// The loads' and the products' loop took 860 cycles a stage of a 512-cycle product without it.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
 template <typename T>
 __device__ __forceinline__ void store_value(T* p, float v) {
@@ -195,20 +259,9 @@ __device__ __forceinline__ void store_value(T* p, float v) {
 // at a time go through the warp's staging buffer (32 rows of 64 bytes, 16-byte pieces XORed with half the row), so that a
 // store instruction writes whole sectors of eight rows.
 template <typename T>
-__device__ __forceinline__ void store_columns(uint32_t (&acc)[32], uint8_t* stage, float* s_bias, int lane, int c0, T* out, int64_t ld, int rows, int cols,
-                                              int vec_ok, const void* bias, int bias_dtype) {
+__device__ __forceinline__ void store_columns(uint32_t (&acc)[32], uint8_t* stage, int lane, int c0, T* out, int64_t ld, int rows, int cols, int vec_ok) {
   constexpr int kPiece = 16 / sizeof(T), kCols = 4 * kPiece;  // columns of a piece, and of 64 bytes
   uint8_t* mine = stage + lane * 64;
-  if (bias != nullptr) {
-    s_bias[lane] = c0 + lane < cols ? load_param(bias, bias_dtype, c0 + lane) : 0.f;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float4 b = reinterpret_cast<const float4*>(s_bias)[i];
-      acc[4 * i] = __float_as_uint(__uint_as_float(acc[4 * i]) + b.x), acc[4 * i + 1] = __float_as_uint(__uint_as_float(acc[4 * i + 1]) + b.y);
-      acc[4 * i + 2] = __float_as_uint(__uint_as_float(acc[4 * i + 2]) + b.z), acc[4 * i + 3] = __float_as_uint(__uint_as_float(acc[4 * i + 3]) + b.w);
-    }
-  }
 #pragma unroll
   for (int h = 0; h < 32 / kCols; ++h) {
 #pragma unroll
@@ -240,43 +293,41 @@ __device__ __forceinline__ void store_columns(uint32_t (&acc)[32], uint8_t* stag
   }
 }
 
-// whether the iterations [from, to) of a tile hold one whose second operand is the first plane
-__device__ __forceinline__ bool meets_first_plane(const GroupedArgs& p, uint32_t from, uint32_t to) {
-  uint32_t term = from % p.terms;
-  for (uint32_t i = from; i < to && i < from + p.terms; ++i) {
-    if (((p.q_planes >> (4 * term)) & 15u) == 0u) return true;
-    if (++term == static_cast<uint32_t>(p.terms)) term = 0;
-  }
-  return false;
-}
-
-template <int kMode, typename T>
+// kPair: launched as clusters of two CTAs, which work on tiles of 256 rows together: each loads its 128 rows and half of the
+// columns, the first CTA (the leader) issues products over both CTAs' operands, each gets its rows' accumulators.  A CTA loads
+// 32 KB a stage instead of 48 for the same products: with one CTA a tile L2's rate to the SMs was the bound.
+template <int kMode, typename T, bool kPair>
 __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
-                                                                const __grid_constant__ GroupedArgs p) {
+                                                                const __grid_constant__ CUtensorMap tmap_o, const __grid_constant__ GroupedArgs p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   GroupedSmem* ctl = reinterpret_cast<GroupedSmem*>(smem);
   uint8_t* ones = smem + 1024;
-  float* s_bias = reinterpret_cast<float*>(smem + 3072);
+  float* s_bias = reinterpret_cast<float*>(smem + 1024);  // of the storing warps' columns: 128 each
   uint8_t* stages = smem + kGrCtrlBytes;  // multiples of 1024 from here on
   const int stage_bytes = kGrPBytes + p.q_bytes;
   uint8_t* store = stages + size_t(p.stages) * stage_bytes;
   uint32_t* first = reinterpret_cast<uint32_t*>(store + kGrStoreBytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = kPair ? cluster_ctarank() : 0u;
+  const int half = kPair ? p.bn / 2 : p.bn;  // columns whose operand this CTA holds
+  const uint32_t workers = kPair ? gridDim.x / 2u : gridDim.x, worker = kPair ? blockIdx.x / 2u : blockIdx.x;
   volatile uint32_t* abort_flag = &ctl->abort_flag;
   constexpr int kParamDtype = std::is_same<T, __half>::value ? FGB_F16 : std::is_same<T, __nv_bfloat16>::value ? FGB_BF16 : FGB_F32_IEEE;
   constexpr bool kBlocks = std::is_same<T, float>::value;  // the accumulator is emptied after every block of 64 k
   constexpr int kSums = kMode == kFew ? 1 : 3;             // blocks of 32 columns that a storing warp adds up
+  auto wait = [&](uint64_t* bar, uint32_t parity) { mbar_wait_tries(bar, parity, abort_flag); };
 
   chain_release();
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(&ctl->full[s], 1);
       mbar_init(&ctl->empty[s], 1);
+      mbar_init(&ctl->peer_full[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&ctl->acc_full[a], 1);
-      mbar_init(&ctl->acc_empty[a], kGrEpilogueWarps);
+      mbar_init(&ctl->acc_empty[a], kPair ? 2 * kGrEpilogueWarps : kGrEpilogueWarps);
     }
     ctl->abort_flag = 0;
     mbar_init_fence();
@@ -290,57 +341,77 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
     tma_prefetch_desc(&tmap_q);
   }
   if (warp == 9) {
-    tmem_alloc_dyn(&ctl->tmem_base, 512u);
-    tmem_relinquish();
+    if constexpr (kPair) {
+      tmem_alloc_pair(&ctl->tmem_base, 512u);
+    } else {
+      tmem_alloc_dyn(&ctl->tmem_base, 512u);
+      tmem_relinquish();
+    }
   }
   chain_wait();
-  p.ranges.check(p.status, p.mirror);
-  plan_groups<kMode>(p, first);
+  const GroupedSchedule plan = plan_groups<kMode>(p, first, workers);
   tc_fence_before_sync();
   __syncthreads();
+  if constexpr (kPair) cluster_sync_all();
   tc_fence_after_sync();
   const uint32_t tmem_base = ctl->tmem_base;
-  GroupedWalk<kMode> walk(p, first, gridDim.x, blockIdx.x);
+  GroupedWalk<kMode> walk(p, plan, workers, worker);
   GroupedItem it;
 
   // where the rows and columns of an item's tile begin
   auto m_tile_of = [&](const GroupedItem& t) { return kMode == kFew ? t.tile % p.n_tiles : t.tile / p.n_tiles; };
   auto n_tile_of = [&](const GroupedItem& t) { return kMode == kFew ? t.tile / p.n_tiles : t.tile % p.n_tiles; };
+  // the bias gradient's products: of a block of k in one of the tiles that read the same rows of dy, in turn
+  auto ones_in = [&](const GroupedItem& t, uint32_t kb) { return kMode == kWeight && p.db != nullptr && kb % p.n_tiles == n_tile_of(t); };
 
+  const uint32_t stage0 = uniform(smem_u32(stages));
   if (warp == 8) {
     // ------------------------------------------------------------------ loads
-    if (elect_one()) {
-      uint32_t s = 0, ph = 0;
-      while (walk.next(it)) {
-        // first row (or channel) of the tile along m and n, first k
-        const int m0 = static_cast<int>(m_tile_of(it)) * 128, n0 = static_cast<int>(n_tile_of(it)) * p.bn;
-        const int lo = static_cast<int>(it.lo), g = static_cast<int>(it.group), G = static_cast<int>(p.ranges.count);
-        uint32_t kb = it.from / p.terms, term = it.from - kb * p.terms;
-        for (uint32_t i = it.from; i < it.to; ++i) {
-          mbar_wait(&ctl->empty[s], ph ^ 1, abort_flag);
-          mbar_arrive_expect_tx(&ctl->full[s], static_cast<uint32_t>(stage_bytes));
-          const uint32_t pd = smem_u32(stages + size_t(s) * stage_bytes), qd = pd + kGrPBytes;
-          const int pp = (p.p_planes >> (4 * term)) & 15, pq = (p.q_planes >> (4 * term)) & 15;
-          const int k0 = static_cast<int>(kb) * 64;
-          if constexpr (kMode == kRows) {
-            tma_load_3d(pd, &tmap_p, &ctl->full[s], k0, lo + m0, pp);
-            if (p.q_mn) {
-              for (int c = 0; c * 64 < p.bn; ++c) tma_load_3d(qd + c * 8192, &tmap_q, &ctl->full[s], n0 + c * 64, k0, pq * G + g);
+    uint32_t s = 0, ph = 0;
+    const int G = static_cast<int>(p.ranges.count), terms = p.terms;
+    const uint32_t full_own = uniform(smem_u32(&ctl->full[0])), full_leader = kPair ? uniform(cluster_map(full_own, 0)) : full_own;
+    while (__any_sync(0xffffffffu, walk.next(it))) {
+      // first row (or channel) of the tile along m and n, first k
+      const int m0 = static_cast<int>(uniform(m_tile_of(it) * p.tile_m + rank * 128u)), n0 = static_cast<int>(uniform(n_tile_of(it) * p.bn + rank * half));
+      const int lo = static_cast<int>(uniform(it.lo)), g = static_cast<int>(uniform(it.group));
+      const int n_blocks = static_cast<int>(uniform((it.to - it.from) / terms));
+      int k0 = static_cast<int>(uniform(it.from / terms * 64u));
+      const int len = static_cast<int>(uniform(it.hi - it.lo));
+      for (int kb = 0; kb < n_blocks; ++kb, k0 += 64) {
+        const bool cleared = kMode == kWeight && k0 + 64 > len && (len & 15) != 0;  // see the products
+        for (int term = 0; term < terms; ++term) {
+          wait(&ctl->empty[s], ph ^ 1);
+          if (elect_one()) {
+            // Pairs: both CTAs' bytes count on the leader's barrier, so that it has one to wait for -- but for a block that
+            // either has to clear rows of first.
+            const bool shared = kPair && !cleared;
+            const uint32_t full = shared ? full_leader + 8u * s : full_own + 8u * s;
+            if (!shared || rank == 0u) mbar_arrive_expect_tx(&ctl->full[s], static_cast<uint32_t>(shared ? 2 * stage_bytes : stage_bytes));
+            auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
+              if constexpr (kPair) tma_load_3d_pair(dst, map, full, c0, c1, c2);
+              else tma_load_3d(dst, map, &ctl->full[s], c0, c1, c2);
+            };
+            const uint32_t pd = stage0 + s * stage_bytes, qd = pd + kGrPBytes;
+            const int pp = (p.p_planes >> (4 * term)) & 15, pq = (p.q_planes >> (4 * term)) & 15;
+            if constexpr (kMode == kRows) {
+              load(pd, &tmap_p, k0, lo + m0, pp);
+              if (p.q_mn) {
+                for (int c = 0; c * 64 < half; ++c) load(qd + c * 8192, &tmap_q, n0 + c * 64, k0, pq * G + g);
+              } else {
+                load(qd, &tmap_q, k0, n0, pq * G + g);
+              }
+            } else if constexpr (kMode == kFew) {
+              if (p.p_mn) {
+                for (int c = 0; c < 2; ++c) load(pd + c * 8192, &tmap_p, m0 + c * 64, k0, pp * G + g);
+              } else {
+                load(pd, &tmap_p, k0, m0, pp * G + g);
+              }
+              load(qd, &tmap_q, k0, lo + n0, pq);
             } else {
-              tma_load_3d(qd, &tmap_q, &ctl->full[s], k0, n0, pq * G + g);
+              for (int c = 0; c < 2; ++c) load(pd + c * 8192, &tmap_p, m0 + c * 64, lo + k0, pp);
+              for (int c = 0; c * 64 < half; ++c) load(qd + c * 8192, &tmap_q, n0 + c * 64, lo + k0, pq);
             }
-          } else if constexpr (kMode == kFew) {
-            if (p.p_mn) {
-              for (int c = 0; c < 2; ++c) tma_load_3d(pd + c * 8192, &tmap_p, &ctl->full[s], m0 + c * 64, k0, pp * G + g);
-            } else {
-              tma_load_3d(pd, &tmap_p, &ctl->full[s], k0, m0, pp * G + g);
-            }
-            tma_load_3d(qd, &tmap_q, &ctl->full[s], k0, lo + n0, pq);
-          } else {
-            for (int c = 0; c < 2; ++c) tma_load_3d(pd + c * 8192, &tmap_p, &ctl->full[s], m0 + c * 64, lo + k0, pp);
-            for (int c = 0; c * 64 < p.bn; ++c) tma_load_3d(qd + c * 8192, &tmap_q, &ctl->full[s], n0 + c * 64, lo + k0, pq);
           }
-          if (++term == static_cast<uint32_t>(p.terms)) term = 0, ++kb;
           if (++s == static_cast<uint32_t>(p.stages)) s = 0, ph ^= 1;
         }
       }
@@ -348,55 +419,90 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
   } else if (warp == 9) {
     // ------------------------------------------------------------------ products
     uint32_t s = 0, ph = 0, set = 0, set_ph = 0;
+    const bool leader = uniform(rank) == 0u;
     const uint64_t p_step = kMode == kWeight || p.p_mn ? 128u : 2u, q_step = kMode == kWeight || p.q_mn ? 128u : 2u;
     const uint32_t p_lbo = kMode == kWeight || p.p_mn ? 8192u : 16u, q_lbo = kMode == kWeight || p.q_mn ? 8192u : 16u;
-    const uint64_t d_ones = make_smem_desc(smem_u32(ones), 16, 1024);
-    while (walk.next(it)) {
-      const bool with_ones = kMode == kWeight && p.db != nullptr && n_tile_of(it) == 0u;
-      uint32_t kb = it.from / p.terms, term = it.from - kb * p.terms;
+    const uint64_t d_ones = make_smem_desc(uniform(smem_u32(ones)), 16, 1024);
+    const uint64_t dp0 = make_smem_desc(stage0, p_lbo, 1024), dq0 = make_smem_desc(stage0 + kGrPBytes, q_lbo, 1024);
+    const uint32_t tmem0 = uniform(tmem_base), peer_full0 = kPair ? uniform(cluster_map(smem_u32(&ctl->peer_full[0]), 0)) : 0u;
+    const uint32_t empty0 = uniform(smem_u32(&ctl->empty[0])), acc_full0 = uniform(smem_u32(&ctl->acc_full[0]));
+    const uint32_t empty1 = kPair ? uniform(cluster_map(empty0, 1)) : 0u, acc_full1 = kPair ? uniform(cluster_map(acc_full0, 1)) : 0u;
+    auto product = [&](uint32_t acc, uint64_t dp, uint64_t dq, uint32_t idesc, uint32_t add) {
+      if constexpr (kPair) umma_ss_pair(acc, dp, dq, idesc, add);
+      else umma_ss<false>(acc, dp, dq, idesc, add);
+    };
+    auto commit = [&](uint32_t bar0, uint32_t bar1, uint32_t i) {  // barrier i, in both CTAs of a pair
+      if constexpr (kPair) {
+        umma_commit_pair(bar0 + 8u * i);
+        umma_commit_pair(bar1 + 8u * i);
+      } else {
+        umma_commit(bar0 + 8u * i);
+      }
+    };
+    uint32_t own_ph = 0, peer_ph = 0;  // a bit for each stage: the phases of the barriers that only cleared blocks use
+    while (__any_sync(0xffffffffu, walk.next(it))) {
+      const uint32_t n_blocks = uniform((it.to - it.from) / p.terms);
+      uint32_t left = uniform((kMode == kWeight ? it.hi - it.lo : static_cast<uint32_t>(p.k_extent)) - it.from / p.terms * 64u);  // k from here on
+      uint32_t turn = kMode == kWeight ? uniform((it.from / p.terms + p.n_tiles - n_tile_of(it)) % p.n_tiles) : 0u;  // 0: the ones' products are ours
       uint32_t any = 0, any_ones = 0, acc = 0;
-      for (uint32_t i = it.from; i < it.to; ++i) {
-        if (any == 0u) {  // a new accumulator
-          mbar_wait(&ctl->acc_empty[set], set_ph ^ 1, abort_flag);
-          tc_fence_after_sync();
-          acc = tmem_base + set * p.acc_stride;
-        }
-        mbar_wait(&ctl->full[s], ph, abort_flag);
-        __syncwarp();
-        tc_fence_after_sync();
-        const uint32_t base = smem_u32(stages + size_t(s) * stage_bytes);
-        const uint32_t left = (kMode == kWeight ? it.hi - it.lo : static_cast<uint32_t>(p.k_extent)) - kb * 64u;
+      for (uint32_t kb = 0; kb < n_blocks; ++kb) {
         const uint32_t valid = min(left, 64u), steps = (valid + 15u) / 16u;
-        if (kMode == kWeight && (valid & 15u) != 0u) {
-          // rows of other groups in the last step: cleared in both operands
-          const uint32_t chunks = 2u + (p.bn + 63u) / 64u, rows = steps * 16u - valid;
-          uint8_t* at = stages + size_t(s) * stage_bytes;
-          for (uint32_t c = 0; c < chunks; ++c)
-            for (uint32_t r = lane >> 3; r < rows; r += 4u)
-              *reinterpret_cast<uint4*>(at + c * 8192u + (valid + r) * 128u + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-        const bool ones_now = with_ones && ((p.q_planes >> (4 * term)) & 15u) == 0u;  // once for each plane of dy
-        if (elect_one()) {
-          const uint64_t dp = make_smem_desc(base, p_lbo, 1024), dq = make_smem_desc(base + kGrPBytes, q_lbo, 1024);
-#pragma unroll
-          for (uint32_t k = 0; k < 4; ++k) {
-            if (k < steps) {
-              umma_ss<false>(acc, dp + k * p_step, dq + k * q_step, p.idesc, k == 0 ? any : 1u);
-              if (ones_now) umma_ss<false>(acc + p.bn, dp + k * p_step, d_ones, p.idesc_ones, k == 0 ? any_ones : 1u);
+        const bool cleared = kMode == kWeight && (valid & 15u) != 0u;
+        const bool with_ones = kMode == kWeight && p.db != nullptr && turn == 0u;
+        for (int term = 0; term < p.terms; ++term) {
+          if (leader || cleared) {
+            if (leader && any == 0u) {  // a new accumulator
+              wait(&ctl->acc_empty[set], set_ph ^ 1);
+              tc_fence_after_sync();
+              acc = tmem0 + set * p.acc_stride;
+            }
+            if (leader) {
+              wait(&ctl->full[s], ph);
+            } else {
+              wait(&ctl->full[s], own_ph >> s & 1u);
+              own_ph ^= 1u << s;
+            }
+            if (cleared) {
+              // rows of other groups in the last step: cleared in both operands
+              __syncwarp();
+              const uint32_t chunks = 2u + (half + 63u) / 64u, rows = steps * 16u - valid;
+              uint8_t* at = stages + size_t(s) * stage_bytes;
+              for (uint32_t c = 0; c < chunks; ++c)
+                for (uint32_t r = lane >> 3; r < rows; r += 4u)
+                  *reinterpret_cast<uint4*>(at + c * 8192u + (valid + r) * 128u + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+              fence_proxy_async_smem();
+              __syncwarp();
+              if constexpr (kPair) {
+                // the peer's ordinary stores: cluster scope on both sides, here only (a wait of that scope takes some 1000 cycles)
+                if (leader) mbar_wait_cluster(&ctl->peer_full[s], peer_ph >> s & 1u, abort_flag);
+                else if (lane == 0) mbar_arrive_cluster_release(peer_full0 + 8u * s);
+                peer_ph ^= 1u << s;
+                __syncwarp();
+              }
             }
           }
-          umma_commit(&ctl->empty[s]);
+          const bool ones_now = with_ones && ((p.q_planes >> (4 * term)) & 15u) == 0u;  // once for each plane of dy
+          if (leader) {
+            if (elect_one()) {
+              const uint64_t dp = dp0 + ((s * stage_bytes) >> 4), dq = dq0 + ((s * stage_bytes) >> 4);
+#pragma unroll
+              for (uint32_t k = 0; k < 4; ++k) {
+                if (k < steps) {
+                  product(acc, dp + k * p_step, dq + k * q_step, p.idesc, k == 0 ? any : 1u);
+                  if (ones_now) product(acc + p.bn, dp + k * p_step, d_ones, p.idesc_ones, k == 0 ? any_ones : 1u);
+                }
+              }
+              commit(empty0, empty1, s);
+            }
+          }
+          any = 1u;
+          any_ones |= ones_now ? 1u : 0u;
+          if (++s == static_cast<uint32_t>(p.stages)) s = 0, ph ^= 1;
         }
-        __syncwarp();
-        any = 1u;
-        any_ones |= ones_now ? 1u : 0u;
-        if (++term == static_cast<uint32_t>(p.terms)) term = 0, ++kb;
-        if (++s == static_cast<uint32_t>(p.stages)) s = 0, ph ^= 1;
-        if (i + 1u == it.to || (kBlocks && term == 0u)) {  // the accumulator is done: the tile's last, or the block's
-          if (elect_one()) umma_commit(&ctl->acc_full[set]);
-          __syncwarp();
+        left -= 64u;
+        if (kMode == kWeight && ++turn == static_cast<uint32_t>(p.n_tiles)) turn = 0u;
+        if (kBlocks || kb + 1u == n_blocks) {  // the accumulator is done: the block's, or the tile's last
+          if (leader && elect_one()) commit(acc_full0, acc_full1, set);
           if (++set == static_cast<uint32_t>(p.acc_sets)) set = 0, set_ph ^= 1;
           any = any_ones = 0u;
         }
@@ -405,36 +511,58 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
   } else {
     // ------------------------------------------------------------------ stores
     const int quarter = warp & 3, group = warp >> 2;
-    uint8_t* stage = store + warp * 2048;
-    float* bias_buf = s_bias + warp * 64;
+    uint8_t* stage = store + warp * 4096;  // two buffers of 32 rows x 64 bytes
+    float* bias_buf = s_bias + warp * 128;
+    uint32_t buffer = 0;
     uint32_t set = 0, set_ph = 0;
     // this warp's columns are [32 group, 32 group + 32) of every 64: at most 3 x 32 of them in fp32
     uint32_t sum[kBlocks ? kSums : 1][32];
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t acc_empty[2] = {kPair ? cluster_map(smem_u32(&ctl->acc_empty[0]), 0) : 0u, kPair ? cluster_map(smem_u32(&ctl->acc_empty[1]), 0) : 0u};
     auto wait_full = [&]() {
-      mbar_wait(&ctl->acc_full[set], set_ph, abort_flag);
+      wait(&ctl->acc_full[set], set_ph);
       tc_fence_after_sync();
       return tmem_base + set * p.acc_stride + lanes;
     };
     auto give_back = [&]() {
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl->acc_empty[set]);
+      if (lane == 0) {
+        if constexpr (kPair) mbar_arrive_cluster(acc_empty[set]);
+        else mbar_arrive(&ctl->acc_empty[set]);
+      }
       if (++set == static_cast<uint32_t>(p.acc_sets)) set = 0, set_ph ^= 1;
     };
     while (walk.next(it)) {
-      const int m0 = static_cast<int>(m_tile_of(it)) * 128 + quarter * 32, n0 = static_cast<int>(n_tile_of(it)) * p.bn;
-      const bool whole = it.from == 0u && it.to == it.whole;
-      const bool with_db = kMode == kWeight && p.db != nullptr && n0 == 0 && group == 0;
+      const int in_tile = static_cast<int>(rank) * 128 + quarter * 32;  // the warp's first row within the tile
+      const int m0 = static_cast<int>(m_tile_of(it)) * p.tile_m + in_tile, n0 = static_cast<int>(n_tile_of(it)) * p.bn;
+      const bool whole = it.piece == kInvalid;
+      const bool with_db = kMode == kWeight && p.db != nullptr && group == 0;
       float db = 0.f;
       uint32_t tmem = 0;
+      // 16-bit results go out by TMA (rows of other matrices are cut off by the map; rows of other groups by nothing, so all 32
+      // have to be the group's); else, and for pieces, by ordinary stores, for which both buffers have to be free
+      const bool by_tma = !kBlocks && kMode != kFew && whole && p.vec_ok && (kMode == kWeight || static_cast<int>(it.hi - it.lo) - m0 >= 32);
+      if (kMode != kFew && !by_tma) {
+        if (elect_one()) bulk_wait_read<0>();
+        __syncwarp();
+      }
+      if (kMode == kRows && p.bias != nullptr) {
+        __syncwarp();
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int c = n0 + group * 32 + b * 64 + lane;
+          bias_buf[b * 32 + lane] = group * 32 + b * 64 < p.bn && c < p.n_extent ? load_param(p.bias, kParamDtype, int64_t(it.group) * p.n_extent + c) : 0.f;
+        }
+        __syncwarp();
+      }
       if constexpr (kBlocks) {
 #pragma unroll
         for (int b = 0; b < kSums; ++b)
 #pragma unroll
           for (int i = 0; i < 32; ++i) sum[b][i] = 0u;
         for (uint32_t at = it.from; at < it.to;) {
-          const uint32_t end = min(it.to, (at / p.terms + 1u) * p.terms);
+          const uint32_t end = at + p.terms;  // a unit has whole blocks
           tmem = wait_full();
 #pragma unroll
           for (int b = 0; b < kSums; ++b) {
@@ -446,7 +574,7 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
               for (int i = 0; i < 32; ++i) sum[b][i] = __float_as_uint(__uint_as_float(sum[b][i]) + __uint_as_float(acc[i]));
             }
           }
-          if (with_db && meets_first_plane(p, at, end)) {
+          if (with_db && ones_in(it, at / p.terms)) {
             uint32_t acc[32];
             tmem_ld_32x32(tmem + p.bn, acc);
             tmem_ld_wait();
@@ -457,21 +585,29 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
         }
       } else {
         tmem = wait_full();
-        if (with_db) {
+        // the first of the unit's blocks whose turn it was, if there is one
+        if (with_db && it.from + (n_tile_of(it) + p.n_tiles - it.from % p.n_tiles) % p.n_tiles < it.to) {
           uint32_t acc[32];
           tmem_ld_32x32(tmem + p.bn, acc);
           tmem_ld_wait();
           db = __uint_as_float(acc[0]);
         }
       }
-      // a piece of a tile: the first slot of its range for one that began before it, else the second
-      float* piece = whole ? nullptr : p.slab + (size_t(it.range) * 2 + (it.from == 0u ? 1 : 0)) * 128 * p.acc_stride;
+      float* piece = whole ? nullptr : p.slab + size_t(it.piece) * p.tile_m * p.bn;
       const int64_t row0 = kMode == kRows ? int64_t(it.lo) + m0 : int64_t(it.group) * p.m_extent + m0;
       const int rows = (kMode == kRows ? static_cast<int>(it.hi - it.lo) : p.m_extent) - m0;
-      const void* bias = p.bias == nullptr ? nullptr
-                         : static_cast<const char*>(p.bias) + (int64_t(it.group) * (kMode == kFew ? p.m_extent : p.n_extent) + (kMode == kFew ? 0 : n0)) *
-                                                                  static_cast<int64_t>(sizeof(T));
-      const float few_bias = kMode == kFew && whole && bias != nullptr && m0 + lane < p.m_extent ? load_param(bias, kParamDtype, m0 + lane) : 0.f;
+      // bias (kRows): column c of the tile at bias_buf[c / 64 * 32 + c % 32], read ahead of the accumulator
+      auto add_bias = [&](uint32_t (&acc)[32], int c0) {
+        if (kMode != kRows || p.bias == nullptr) return;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 b = reinterpret_cast<const float4*>(bias_buf + c0 / 64 * 32)[i];
+          acc[4 * i] = __float_as_uint(__uint_as_float(acc[4 * i]) + b.x), acc[4 * i + 1] = __float_as_uint(__uint_as_float(acc[4 * i + 1]) + b.y);
+          acc[4 * i + 2] = __float_as_uint(__uint_as_float(acc[4 * i + 2]) + b.z), acc[4 * i + 3] = __float_as_uint(__uint_as_float(acc[4 * i + 3]) + b.w);
+        }
+      };
+      const float few_bias =
+          kMode == kFew && whole && p.bias != nullptr && m0 + lane < p.m_extent ? load_param(p.bias, kParamDtype, int64_t(it.group) * p.m_extent + m0 + lane) : 0.f;
       auto put = [&](uint32_t (&acc)[32], int c0) {
         if constexpr (kMode == kFew) {
           const int left = static_cast<int>(it.hi - it.lo) - n0;  // rows of the tile, and more
@@ -485,10 +621,30 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
             }
           }
         } else if (piece != nullptr) {
-          store_columns<float>(acc, stage, bias_buf, lane, c0, piece + size_t(quarter * 32) * p.bn, p.bn, 32, p.bn, 1, nullptr, 0);
+          store_columns<float>(acc, stage, lane, c0, piece + size_t(in_tile) * p.bn, p.bn, 32, p.bn, 1);
+        } else if (by_tma) {
+          // the buffer before this one may still be read; 32 rows of 64 bytes in the order that the map's swizzle says
+          uint8_t* to = stage + buffer * 2048;
+          add_bias(acc, c0);
+          if (elect_one()) bulk_wait_read<1>();
+          __syncwarp();
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(acc[g * 8 + i]);
+            if constexpr (!kBlocks) *reinterpret_cast<uint4*>(to + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4)) = Channels<T, 8>::pack(f);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (elect_one()) {
+            tma_store_3d(&tmap_o, smem_u32(to), n0 + c0, kMode == kRows ? static_cast<int>(it.lo) + m0 : m0, kMode == kRows ? 0 : static_cast<int>(it.group));
+            bulk_commit();
+          }
+          buffer ^= 1u;
         } else {
-          store_columns<T>(acc, stage, bias_buf, lane, c0, static_cast<T*>(p.out) + row0 * p.out_ld + n0, p.out_ld, rows, p.n_extent - n0, p.vec_ok, bias,
-                           kParamDtype);
+          add_bias(acc, c0);
+          store_columns<T>(acc, stage, lane, c0, static_cast<T*>(p.out) + row0 * p.out_ld + n0, p.out_ld, rows, p.n_extent - n0, p.vec_ok);
         }
       };
       if (*abort_flag == 0u) {  // else nothing that was waited for is there, and the status word says so
@@ -497,18 +653,20 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
           for (int b = 0; b < kSums; ++b)
             if (group * 32 + b * 64 < p.bn) put(sum[b], group * 32 + b * 64);
         } else {
-          for (int c0 = group * 32; c0 < p.bn; c0 += 64) {
-            uint32_t acc[32];
-            tmem_ld_32x32(tmem + c0, acc);
-            tmem_ld_wait();
-            put(acc, c0);
+          // the next 32 columns are on their way while these are stored
+          uint32_t acc[2][32];
+          if (group * 32 < p.bn) tmem_ld_32x32(tmem + group * 32, acc[0]);
+#pragma unroll
+          for (int b = 0; b < (kMode == kFew ? 1 : 4); ++b) {
+            const int c0 = group * 32 + b * 64;
+            if (c0 < p.bn) {
+              tmem_ld_wait();
+              if (kMode != kFew && c0 + 64 < p.bn) tmem_ld_32x32(tmem + c0 + 64, acc[(b + 1) % 2]);
+              put(acc[b % 2], c0);
+            }
           }
         }
-        if (with_db) {
-          const int m = m0 + lane;
-          if (piece != nullptr) piece[128 * p.bn + quarter * 32 + lane] = db;
-          else if (m < p.m_extent) store_value(static_cast<T*>(p.db) + int64_t(it.group) * p.m_extent + m, db);
-        }
+        if (with_db) p.db_parts[size_t(it.unit) * p.tile_m + in_tile + lane] = db;
       }
       if constexpr (!kBlocks) give_back();
     }
@@ -524,11 +682,15 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
     }
   }
 
+  if (warp < kGrEpilogueWarps && elect_one()) bulk_wait_all();
+  __syncwarp();
   tc_fence_before_sync();
   __syncthreads();
+  if constexpr (kPair) cluster_sync_all();  // no CTA leaves while the other may still arrive on its barriers or read its operands
   if (warp == 9) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, 512u);
+    if constexpr (kPair) tmem_dealloc_pair(tmem_base, 512u);
+    else tmem_dealloc(tmem_base, 512u);
   }
   if (tid == 0 && ctl->abort_flag) {
     report(p.status, FGB_S_WAIT_TIMEOUT);
@@ -537,8 +699,8 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
 }
 
 // ------------------------------------------------------------------ pieces
-// Tiles that lie in several ranges: their pieces added in order, and the tiles of empty groups (weight gradient), which no
-// range holds: zeros.  gridDim.y CTAs a tile.
+// Tiles in parts: their pieces added in order; and the tiles of empty groups (weight gradient), of which there are no units:
+// zeros.  gridDim.y CTAs a tile; `ctas`: those of the products' kernel.
 constexpr int kGrJoinThreads = 256;
 template <int kMode, typename T>
 __global__ void __launch_bounds__(kGrJoinThreads) grouped_join_kernel(const __grid_constant__ GroupedArgs p, uint32_t ctas, uint32_t tiles) {
@@ -546,59 +708,82 @@ __global__ void __launch_bounds__(kGrJoinThreads) grouped_join_kernel(const __gr
   constexpr int kParamDtype = std::is_same<T, __half>::value ? FGB_F16 : std::is_same<T, __nv_bfloat16>::value ? FGB_BF16 : FGB_F32_IEEE;
   chain_release();
   chain_wait();
-  plan_groups<kMode>(p, s_first);
-  const uint32_t G = p.ranges.count, total = s_first[G], length = range_length<kMode>(p, total, ctas);
+  const GroupedSchedule plan = plan_groups<kMode>(p, s_first, ctas);
+  const uint32_t G = p.ranges.count;
   for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-    uint32_t g, tile, whole;
+    uint32_t g, tile;
     if constexpr (kMode == kWeight) {
       const uint32_t per = p.n_tiles * p.m_tiles;
       g = t / per, tile = t - g * per;
-      whole = (s_first[g + 1u] - s_first[g]) / per;
     } else {
-      whole = static_cast<uint32_t>(p.k_blocks * p.terms);
-      if (uint64_t(t) * whole >= total) return;
+      // all tiles have equally many parts: that of tile t's first is t * parts
+      const uint32_t whole = static_cast<uint32_t>(p.k_blocks * p.terms), parts = parts_of(whole, part_length(p, whole, plan.unit));
+      if (uint64_t(t) * parts >= plan.first[G]) return;
       uint32_t lo = 0, hi = G - 1u;
       while (lo < hi) {
         const uint32_t mid = (lo + hi + 1u) / 2u;
-        if (s_first[mid] <= t * whole) lo = mid;
+        if (plan.first[mid] <= t * parts) lo = mid;
         else hi = mid - 1u;
       }
-      g = lo, tile = t - s_first[g] / whole;
+      g = lo, tile = t - plan.first[g] / parts;
     }
-    const uint32_t begin = s_first[g] + tile * whole, end = begin + whole;
-    const uint32_t r0 = begin / length, r1 = whole > 0u ? (end - 1u) / length : r0;
-    if (whole > 0u && r0 == r1) continue;  // stored as a whole
-    const uint32_t pieces = whole > 0u ? r1 - r0 + 1u : 0u;
-    const size_t size = size_t(128) * p.acc_stride;
-    const float* from = p.slab + (size_t(r0) * 2 + 1) * size;  // then (r0 + 1) * 2, (r0 + 2) * 2, ...
-    auto sum_at = [&](uint32_t e) {
-      float v = 0.f;
-      if (pieces > 0u) {
-        v = from[e];
-#pragma unroll 8
-        for (uint32_t k = 1; k < pieces; ++k) v += from[size * (2u * k - 1u) + e];
+    const GroupSize z = group_size<kMode>(p, plan.offsets, g);
+    const uint32_t pieces = z.tiles == 0u ? 0u : parts_of(z.whole, part_length(p, z.whole, plan.unit));
+    const uint32_t elements = static_cast<uint32_t>(p.tile_m) * p.bn;
+    if (kMode == kWeight && p.db != nullptr && tile % p.n_tiles == 0u && blockIdx.y == 0u && threadIdx.x < p.tile_m) {
+      // the shares of db: of every part of the n tiles that read the same rows of dy
+      const uint32_t m = tile / p.n_tiles * p.tile_m + threadIdx.x;
+      if (m < static_cast<uint32_t>(p.m_extent)) {
+        float v = 0.f;
+        const float* share = p.db_parts + (size_t(plan.first[g]) + tile) * p.tile_m + threadIdx.x;
+        for (uint32_t k = 0; k < pieces; ++k)
+#pragma unroll 4
+          for (int n = 0; n < p.n_tiles; ++n) v += share[(size_t(k) * z.tiles + n) * p.tile_m];
+        store_value(static_cast<T*>(p.db) + int64_t(g) * p.m_extent + m, v);
       }
-      return v;
-    };
-    const uint32_t lo = p.ranges.at(g), hi = p.ranges.at(g + 1u);
-    const uint32_t elements = 128u * p.bn, share = (elements + gridDim.y - 1u) / gridDim.y;
-    const uint32_t e0 = blockIdx.y * share, e1 = min(elements, e0 + share);
-    for (uint32_t e = e0 + threadIdx.x; e < e1; e += kGrJoinThreads) {
-      if constexpr (kMode == kWeight) {
-        const uint32_t a = e / p.bn, m = tile / p.n_tiles * 128u + a, n = tile % p.n_tiles * p.bn + (e - a * p.bn);
-        if (m < static_cast<uint32_t>(p.m_extent) && n < static_cast<uint32_t>(p.n_extent))
-          store_value(static_cast<T*>(p.out) + (int64_t(g) * p.m_extent + m) * p.out_ld + n, sum_at(e));
-      } else {
-        const uint32_t a = e / 128u, row = lo + tile / p.n_tiles * p.bn + a, m = tile % p.n_tiles * 128u + (e & 127u);
-        if (row < hi && m < static_cast<uint32_t>(p.m_extent)) {
-          const float b = p.bias != nullptr ? load_param(p.bias, kParamDtype, int64_t(g) * p.m_extent + m) : 0.f;
-          store_value(static_cast<T*>(p.out) + int64_t(row) * p.out_ld + m, sum_at(e) + b);
+    }
+    if (pieces == 1u) continue;  // stored as a whole
+    const size_t apart = size_t(elements) * z.tiles;
+    const float* from = p.slab + size_t(elements) * (plan.piece[g] + tile);
+    // four elements a thread: neighbours in the piece, and in the output
+    const uint32_t quads = elements / 4u, share = (quads + gridDim.y - 1u) / gridDim.y;
+    const uint32_t q0 = blockIdx.y * share, q1 = min(quads, q0 + share);
+    for (uint32_t q = q0 + threadIdx.x; q < q1; q += kGrJoinThreads) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (pieces > 0u) {
+        v = __ldcg(reinterpret_cast<const float4*>(from) + q);
+#pragma unroll 8
+        for (uint32_t k = 1; k < pieces; ++k) {
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(from + apart * k) + q);
+          v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
         }
       }
-    }
-    if (kMode == kWeight && p.db != nullptr && tile % p.n_tiles == 0u && blockIdx.y == 0u && threadIdx.x < 128u) {
-      const uint32_t m = tile / p.n_tiles * 128u + threadIdx.x;
-      if (m < static_cast<uint32_t>(p.m_extent)) store_value(static_cast<T*>(p.db) + int64_t(g) * p.m_extent + m, sum_at(elements + threadIdx.x));
+      const uint32_t e = q * 4u;
+      float f[4] = {v.x, v.y, v.z, v.w};
+      uint32_t col, cols;
+      T* out;
+      if constexpr (kMode == kWeight) {
+        const uint32_t a = e / p.bn, m = tile / p.n_tiles * p.tile_m + a;
+        if (m >= static_cast<uint32_t>(p.m_extent)) continue;
+        col = tile % p.n_tiles * p.bn + (e - a * p.bn), cols = p.n_extent;
+        out = static_cast<T*>(p.out) + (int64_t(g) * p.m_extent + m) * p.out_ld;
+      } else {
+        const uint32_t a = e / 128u, row = z.lo + tile / p.n_tiles * p.bn + a;
+        if (row >= z.hi) continue;
+        col = tile % p.n_tiles * 128u + (e & 127u), cols = p.m_extent;
+        out = static_cast<T*>(p.out) + int64_t(row) * p.out_ld;
+        if (p.bias != nullptr)
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i)
+            if (col + i < cols) f[i] += load_param(p.bias, kParamDtype, int64_t(g) * p.m_extent + col + i);
+      }
+      if (p.vec_ok && col + 4u <= cols) {
+        Channels<T, 4>::store(out + col, Channels<T, 4>::pack(f));
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+          if (col + i < cols) store_value(out + col + i, f[i]);
+      }
     }
   }
 }
@@ -676,10 +861,10 @@ static int tile_columns(int extent, int most) {
 }
 
 struct GroupedPlan {
-  int mode, bn, split;
-  int64_t slots;        // pieces that the slab holds
-  int64_t slab_bytes;
-  uint32_t min_range;
+  int mode, bn, split, pair;
+  int64_t pieces;       // that the slab holds
+  int64_t slab_bytes, db_bytes;
+  uint32_t min_part;
   int acc_stride;
   int64_t tiles;        // most tiles (those that the join kernel looks at)
 };
@@ -691,15 +876,17 @@ static int grouped_plan(const fgb_grouped_linear_call& c, int pass, GroupedPlan&
   const int64_t sms = device_sm_count(), terms = c.dtype == FGB_F32_IEEE ? 6 : c.dtype == FGB_F32_TF32 ? 3 : 1;
   const int64_t N = c.n, G = c.groups;
   const int most = is_f32(c.dtype) ? 192 : 256;  // fp32: the blocks' sums of a tile are held in 3 x 32 registers
-  int64_t iterations;
-  p.split = 0, p.min_range = 0;
+  int64_t iterations, db_units = 0;
+  p = GroupedPlan{};
   if (pass == 2) {
     p.mode = kWeight;
+    p.pair = c.co > 128 && c.ci > 64;
     p.bn = tile_columns(c.ci, most);
-    const int64_t per = ceil_div(c.ci, p.bn) * ceil_div(c.co, 128);
+    const int64_t per = ceil_div(c.ci, p.bn) * ceil_div(c.co, p.pair ? 256 : 128);
     p.tiles = G * per;
     iterations = (N / 64 + G) * per * terms;
-    p.split = 1, p.min_range = 4;
+    p.split = 1, p.min_part = static_cast<uint32_t>(4 * terms);
+    if (c.grad_bias != nullptr) db_units = p.tiles;
   } else {
     const int nout = pass == 0 ? c.co : c.ci, k = pass == 0 ? c.ci : c.co;
     const int64_t kb = ceil_div(k, 64);
@@ -710,18 +897,23 @@ static int grouped_plan(const fgb_grouped_linear_call& c, int pass, GroupedPlan&
       const int64_t m_tiles = ceil_div(nout, 128);
       p.tiles = std::min<int64_t>(N, N / p.bn + G) * m_tiles;
       iterations = p.tiles * kb * terms;
-      if (p.tiles <= sms / 2 && kb * terms >= 8) p.split = 1, p.min_range = 4;
+      if (p.tiles <= sms / 2 && kb >= 8) p.split = 1, p.min_part = static_cast<uint32_t>(4 * terms);
     } else {
       p.mode = kRows;
+      p.pair = N >= 512 * G && nout > 64;
       p.bn = tile_columns(nout, most);
-      p.tiles = (N / 128 + G) * ceil_div(nout, p.bn);
+      p.tiles = (N / (p.pair ? 256 : 128) + G) * ceil_div(nout, p.bn);
       iterations = p.tiles * kb * terms;
     }
   }
   if (iterations >= (int64_t(1) << 31) - 1) return FGB_E_SIZE;
+  // two accumulators a tile; the products with ones take 32 columns more
   p.acc_stride = std::max(p.bn, 32) + (pass == 2 && c.grad_bias != nullptr ? 32 : 0);
-  p.slots = p.split ? 2 * sms : 0;
-  p.slab_bytes = align256(p.slots * 128 * p.acc_stride * 4);
+  const int64_t tile_m = p.pair ? 256 : 128, workers = p.pair ? sms / 2 : sms;
+  // a part has half of the wanted length at least (a tile is cut only where it is longer), and min_part at least
+  p.pieces = p.split ? std::min<int64_t>(2 * kGrMostUnits * workers, iterations / p.min_part) : 0;
+  p.slab_bytes = align256(p.pieces * tile_m * p.bn * 4);
+  p.db_bytes = db_units > 0 ? align256((db_units + p.pieces) * tile_m * 4) : 0;
   return FGB_OK;
 }
 
@@ -739,23 +931,23 @@ static int64_t backward_planes(const fgb_grouped_linear_call& c) {
          (c.grad_weight != nullptr ? plane_bytes(c.n, c.ci, c.dtype) : 0);
 }
 
-template <int kMode, typename T>
-static int launch_grouped(const CUtensorMap& tp, const CUtensorMap& tq, GroupedArgs& a, const GroupedPlan& p, cudaStream_t s) {
-  const int prefix = static_cast<int>(align256((int64_t(a.ranges.count) + 1) * 4));
+template <int kMode, typename T, bool kPair>
+static int launch_grouped(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMap& to, GroupedArgs& a, const GroupedPlan& p, cudaStream_t s) {
+  const int prefix = static_cast<int>(schedule_bytes(a.ranges.count));
   const int fixed = 1024 + kGrCtrlBytes + kGrStoreBytes + prefix;
   const int stage = kGrPBytes + a.q_bytes;
   a.stages = std::min(kGrMaxStages, (kGrSmemLimit - fixed) / stage);
   const size_t smem = size_t(fixed) + size_t(a.stages) * stage;
   static PerDeviceTable configured;
-  const int rc = ensure_dynamic_smem(configured, grouped_kernel<kMode, T>, smem);
+  const int rc = ensure_dynamic_smem(configured, grouped_kernel<kMode, T, kPair>, smem);
   if (rc != FGB_OK) return rc;
-  const int ctas = device_sm_count();
-  const unsigned grid = static_cast<unsigned>(p.split ? ctas : std::max<int64_t>(std::min<int64_t>(p.tiles, ctas), 1));
-  cudaError_t e = launch_chained(grouped_kernel<kMode, T>, dim3(grid), dim3(kGrThreads), smem, s, tp, tq, a);
+  const int workers = kPair ? device_sm_count() / 2 : device_sm_count();
+  const unsigned grid = static_cast<unsigned>(p.split ? workers : std::max<int64_t>(std::min<int64_t>(p.tiles, workers), 1));
+  cudaError_t e = launch_chained_clusters(grouped_kernel<kMode, T, kPair>, dim3(grid * (kPair ? 2 : 1)), dim3(kGrThreads), smem, kPair ? 2 : 1, s, tp, tq, to, a);
   if (e == cudaSuccess && p.split) {
     if constexpr (kMode != kRows) {
       const unsigned tiles = static_cast<unsigned>(p.tiles), x = std::min(tiles, 65535u * 8u);
-      const unsigned y = static_cast<unsigned>(std::clamp<int64_t>(ceil_div(int64_t(ctas) * 8, tiles), 1, 64));
+      const unsigned y = static_cast<unsigned>(std::clamp<int64_t>(ceil_div(int64_t(device_sm_count()) * 8, tiles), 1, 64));
       e = launch_chained(grouped_join_kernel<kMode, T>, dim3(x, y), dim3(kGrJoinThreads), size_t(prefix), s, a, grid, tiles);
     }
   }
@@ -769,25 +961,27 @@ static int grouped_pass(const fgb_grouped_linear_call& c, int pass, const Operan
   if (rc != FGB_OK) return rc;
   GroupedArgs a{};
   a.ranges = RowRanges{c.offsets, c.offsets_bits == 64, static_cast<uint32_t>(c.n), static_cast<uint32_t>(c.groups)};
-  a.bn = p.bn;
+  a.bn = p.bn, a.tile_m = p.pair ? 256 : 128;
+  const int half = p.pair ? p.bn / 2 : p.bn;
   a.terms = c.dtype == FGB_F32_IEEE ? 6 : c.dtype == FGB_F32_TF32 ? 3 : 1;
   // the small products first: (lo hi) (hi lo) (mid mid) (mid hi) (hi mid) (hi hi), or the last three of them
   a.p_planes = a.terms == 6 ? 0x001102u : a.terms == 3 ? 0x001u : 0u, a.q_planes = a.terms == 6 ? 0x010120u : a.terms == 3 ? 0x010u : 0u;
-  a.min_range = p.min_range;
+  a.min_part = p.min_part;
+  a.piece_cost = static_cast<uint32_t>(ceil_div(10 * p.bn, 256));  // 128 KB a CTA written, then read: the time of some ten stages
   a.acc_stride = p.acc_stride;
   a.acc_sets = 2 * p.acc_stride <= 512 ? 2 : 1;
-  a.slab = slab;
+  a.slab = slab, a.db_parts = slab + p.slab_bytes / 4;
   a.status = c.status, a.mirror = status_mirror(c.status);
   const uint32_t fmt = features.dtype16 == FGB_F16 ? kFmtF16 : kFmtBF16;
   a.one_pair = features.dtype16 == FGB_F16 ? 0x3C003C00u : 0x3F803F80u;
   const int eb = elem_bytes(c.dtype);
-  CUtensorMap tp, tq;
+  CUtensorMap tp, tq, to{};
   const uint64_t N = static_cast<uint64_t>(c.n), G = static_cast<uint64_t>(c.groups);
   if (pass == 2) {
     // features = dy, other = x
-    a.m_extent = c.co, a.n_extent = c.ci, a.m_tiles = static_cast<int>(ceil_div(c.co, 128)), a.n_tiles = static_cast<int>(ceil_div(c.ci, p.bn));
+    a.m_extent = c.co, a.n_extent = c.ci, a.m_tiles = static_cast<int>(ceil_div(c.co, a.tile_m)), a.n_tiles = static_cast<int>(ceil_div(c.ci, p.bn));
     a.p_mn = a.q_mn = 1;
-    a.q_bytes = (p.bn + 63) / 64 * 8192;
+    a.q_bytes = (half + 63) / 64 * 8192;
     a.out = c.grad_weight, a.out_ld = c.ci, a.db = c.grad_bias;
     rc = make_rows_tmap_3d(&tp, features.base, features.dtype16, features.cp, N, features.planes, 64, 64);
     if (rc == FGB_OK) rc = make_rows_tmap_3d(&tq, other.base, other.dtype16, other.cp, N, other.planes, 64, 64);
@@ -809,20 +1003,26 @@ static int grouped_pass(const fgb_grouped_linear_call& c, int pass, const Operan
     } else {
       a.n_extent = nout, a.n_tiles = static_cast<int>(ceil_div(nout, p.bn));
       a.q_mn = mn;
-      a.q_bytes = mn ? (p.bn + 63) / 64 * 8192 : p.bn * 128;
+      a.q_bytes = mn ? (half + 63) / 64 * 8192 : half * 128;
       rc = make_rows_tmap_3d(&tp, features.base, features.dtype16, features.cp, N, features.planes, 64, 128);
-      if (rc == FGB_OK) rc = make_rows_tmap_3d(&tq, other.base, other.dtype16, wc, wr, w_planes, 64, mn ? 64 : p.bn);
+      if (rc == FGB_OK) rc = make_rows_tmap_3d(&tq, other.base, other.dtype16, wc, wr, w_planes, 64, mn ? 64 : half);
     }
   }
   if (rc != FGB_OK) return rc;
   a.vec_ok = a.out_ld * eb % 16 == 0;
-  a.idesc = make_idesc(fmt, 128, p.bn, a.p_mn, a.q_mn);
-  a.idesc_ones = make_idesc(fmt, 128, 16, a.p_mn, 0);
-#define FGB_GROUPED(mode)                                                              \
-  (c.dtype == FGB_F16    ? launch_grouped<mode, __half>(tp, tq, a, p, s)               \
-   : c.dtype == FGB_BF16 ? launch_grouped<mode, __nv_bfloat16>(tp, tq, a, p, s)        \
-                         : launch_grouped<mode, float>(tp, tq, a, p, s))
-  return p.mode == kRows ? FGB_GROUPED(kRows) : p.mode == kFew ? FGB_GROUPED(kFew) : FGB_GROUPED(kWeight);
+  if (a.vec_ok && eb == 2 && p.mode != kFew) {  // what is stored: 32 rows x 32 columns at a time
+    rc = pass == 2 ? make_rows_tmap_3d(&to, a.out, c.dtype, c.ci, c.co, G, 32, 32) : make_rows_tmap_3d(&to, a.out, c.dtype, a.out_ld, N, 1, 32, 32);
+    if (rc != FGB_OK) return rc;
+  }
+  a.idesc = make_idesc(fmt, a.tile_m, p.bn, a.p_mn, a.q_mn);
+  a.idesc_ones = make_idesc(fmt, a.tile_m, p.pair ? 32 : 16, a.p_mn, 0);
+#define FGB_GROUPED(mode, pair)                                                        \
+  (c.dtype == FGB_F16    ? launch_grouped<mode, __half, pair>(tp, tq, to, a, p, s)         \
+   : c.dtype == FGB_BF16 ? launch_grouped<mode, __nv_bfloat16, pair>(tp, tq, to, a, p, s)  \
+                         : launch_grouped<mode, float, pair>(tp, tq, to, a, p, s))
+  if (p.mode == kFew) return FGB_GROUPED(kFew, false);
+  if (p.mode == kRows) return p.pair ? FGB_GROUPED(kRows, true) : FGB_GROUPED(kRows, false);
+  return p.pair ? FGB_GROUPED(kWeight, true) : FGB_GROUPED(kWeight, false);
 #undef FGB_GROUPED
 }
 
@@ -852,7 +1052,7 @@ extern "C" int64_t fgb_grouped_linear_workspace_bytes(const fgb_grouped_linear_c
     if (pass == 1 ? c->grad_x == nullptr : c->grad_weight == nullptr) continue;
     rc = grouped_plan(*c, pass, p);
     if (rc != FGB_OK) return rc;
-    slab = std::max(slab, p.slab_bytes);
+    slab = std::max(slab, p.slab_bytes + p.db_bytes);
   }
   return bytes + slab + backward_planes(*c);
 }
