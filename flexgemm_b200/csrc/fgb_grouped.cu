@@ -4,7 +4,8 @@
 //   input gradient    dx_r = W_g^T dy_r
 //   weight gradient   dW_g = sum_r dy_r x_r^T,  db_g = sum_r dy_r
 //
-// One persistent tcgen05 kernel for all of them: D[m, n] = sum_k P[m, k] Q[n, k], tiles of 128 x BN, 64 k a stage.
+// One persistent tcgen05 kernel for all of them: D[m, n] = sum_k P[m, k] Q[n, k], tiles of 128 (256 for a pair of CTAs) x BN,
+// a block of 64 k a stage.
 //   kRows    m = rows, n = channels of the output.  The rows of a tile may reach into the next group: what they give is not
 //            stored.  The gradient reads W_g as stored, with k along its rows (MN-major operand).
 //   kFew     m = channels, n = rows (16 to 64 of them): where groups have few rows the matrices are what is read, and a tile
@@ -17,8 +18,8 @@
 // where they fit, so that a tile is stored while the next is multiplied.
 //
 // Work is dealt out in units, one after the other to the CTAs in turn: a tile, or where there are too few tiles to go round
-// (the weight gradient; a few rows) one of the equal parts of its iterations (a stage each).  The parts of a group's tiles that
-// read the same k are neighbours, so that they find it in L2: equal ranges of one long line of iterations, which need no
+// (the weight gradient; a few rows) one of the equal parts of its blocks of k.  The parts of a group's tiles that
+// read the same k are neighbours, so that they find it in L2: equal ranges of one long line of blocks, which need no
 // rounding up, read everything from memory once for each tile (16 groups of 8192 rows, 1024 x 1024: 422 us).  A tile in parts
 // leaves fp32 pieces in a slab, which a second kernel adds up in their order.  Every CTA finds the number of parts from the
 // sizes alone, so results do not depend on the run.
@@ -28,7 +29,8 @@
 // fp32's range, so no scaling is needed, and six of them cost what three TF32 products do (half the rate, twice the bytes).
 // The tensor cores cut what they add to an accumulator at its last bit instead of rounding: over a long k that is a bias
 // (2e-8 of the sum for every 16 k; 1e-5 where k was 10^5).  So fp32 leaves the accumulator after each block of 64 k, the small
-// products first, the large one last, and the storing warps add the blocks up in registers, rounding to nearest.
+// products first, the large one last, and the storing warps add the blocks up in registers, rounding to nearest.  A stage has
+// all planes of its block: each is loaded once for the two or three products that it is in.
 #include <algorithm>
 #include <type_traits>
 
@@ -44,7 +46,6 @@ constexpr int kGrEpilogueWarps = 8;
 constexpr int kGrMaxStages = 12;
 constexpr int kGrMaxGroups = 2048;
 constexpr int kGrCtrlBytes = 1024 + 4096;  // barriers; a block of ones (kWeight) or the storing warps' bias (kRows)
-constexpr int kGrStoreBytes = kGrEpilogueWarps * 4096;
 constexpr int kGrSmemLimit = 226 * 1024;  // of dynamic shared memory, beside 1 KB of static
 constexpr int kGrPBytes = 128 * 128;
 
@@ -58,12 +59,14 @@ struct GroupedArgs {
   int m_tiles;          // kWeight: tiles along co
   int k_blocks;         // kRows, kFew: blocks of 64 along k
   int k_extent;         // kRows, kFew: k
+  int planes;           // of an operand
   int terms;            // products of planes
   uint32_t p_planes, q_planes;  // their planes, four bits a term
   int p_mn, q_mn;       // operand is MN-major
   int stages, q_bytes, acc_sets, acc_stride;
-  uint32_t min_part;    // iterations that a part of a tile has at least; 0: tiles are not cut
-  uint32_t piece_cost;  // what writing and adding up a piece takes, in iterations
+  uint32_t min_part;    // blocks of k that a part of a tile has at least; 0: tiles are not cut
+  float piece_cost;     // what writing and adding up a piece takes, in blocks
+  uint32_t* plan;       // where tiles are cut: the schedule, for the kernel that adds the pieces up
   uint32_t idesc, idesc_ones;
   uint32_t one_pair;    // two ones of the operand type
   const void* bias;     // [groups, nout] or null
@@ -86,7 +89,7 @@ struct GroupedSmem {
 };
 static_assert(sizeof(GroupedSmem) <= 1024, "control block too large");
 
-// The rows, tiles and iterations a tile of group g; `offsets` are those of the groups in shared memory
+// The rows and tiles of group g, and the blocks of k of a tile; `offsets` are those of the groups in shared memory
 struct GroupSize {
   uint32_t lo, hi, tiles, whole;
 };
@@ -99,33 +102,36 @@ __device__ __forceinline__ GroupSize group_size(const GroupedArgs& p, const uint
   if constexpr (kMode == kRows) s.tiles = (len + p.tile_m - 1u) / p.tile_m * p.n_tiles;
   else if constexpr (kMode == kFew) s.tiles = (len + p.bn - 1u) / p.bn * p.n_tiles;
   else s.tiles = len > 0u ? p.n_tiles * p.m_tiles : 0u;
-  s.whole = static_cast<uint32_t>((kMode == kWeight ? (len + 63u) / 64u : p.k_blocks) * p.terms);
+  s.whole = kMode == kWeight ? (len + 63u) / 64u : static_cast<uint32_t>(p.k_blocks);
   return s;
 }
-// length of the parts of a tile of `whole` iterations where `unit` are wanted: whole blocks of k, all parts but the last alike
+// length of the parts of a tile of `whole` blocks where `unit` are wanted: all parts but the last alike
 __device__ __forceinline__ uint32_t part_length(const GroupedArgs& p, uint32_t whole, uint32_t unit) {
   if (p.min_part == 0u || whole <= unit) return whole;
   const uint32_t parts = min((whole + unit - 1u) / unit, max(whole / p.min_part, 1u));
-  const uint32_t blocks = whole / p.terms;
-  return (blocks + parts - 1u) / parts * p.terms;
+  return (whole + parts - 1u) / parts;
 }
 __device__ __forceinline__ uint32_t parts_of(uint32_t whole, uint32_t length) { return length == 0u ? 0u : (whole + length - 1u) / length; }
 
-// What every CTA works out at its start: first[g] = units of the groups before g, piece[g] = pieces of tiles before g, and
-// the length that parts should have.  The whole CTA calls it (and waits at its end).
-constexpr uint32_t kGrMostUnits = 3;  // units that a CTA gets on average where tiles are cut: 1, 2 or 3
+// What every CTA works out at its start: first[g] = units of the groups before g, piece[g] = pieces of tiles before g, the
+// groups' offsets, and the length that parts should have.  The whole CTA calls it (and waits at its end).
+//
+// Cut tiles: 31 lengths between twice and a third of a CTA's share of the blocks (and none: whole tiles) are weighed by what
+// the CTA with the most work then has -- rounds of equal units, or the share and half a unit where they differ -- and by
+// the pieces.
+constexpr int kGrMostUnits = 3;  // units of a CTA, on average, at the smallest length
 struct GroupedSchedule {
   uint32_t* first;
   uint32_t* piece;
   uint32_t* offsets;
   uint32_t unit;
 };
-inline int64_t schedule_bytes(int64_t groups) { return align256((groups + 1) * 12); }
+inline int64_t schedule_bytes(int64_t groups) { return align256((groups + 1) * 12 + 4); }
 template <int kMode>
 __device__ __forceinline__ GroupedSchedule plan_groups(const GroupedArgs& p, uint32_t* s_first, uint32_t ctas) {
   __shared__ unsigned long long s_total;
-  __shared__ float s_cost[kGrMostUnits + 1];
-  __shared__ uint32_t s_unit[kGrMostUnits + 1];
+  __shared__ uint32_t s_units[32], s_pieces[32], s_longest[32], s_shortest[32];
+  __shared__ uint32_t s_best;
   const uint32_t G = p.ranges.count, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
   GroupedSchedule plan{s_first, s_first + G + 1u, s_first + 2u * (G + 1u), 0xFFFFFFFFu};
   bool bad = false;
@@ -133,6 +139,7 @@ __device__ __forceinline__ GroupedSchedule plan_groups(const GroupedArgs& p, uin
     plan.offsets[g] = p.ranges.at(g);
     bad |= g < G && !p.ranges.good(g);
   }
+  if (p.min_part != 0u && threadIdx.x < 32u) s_units[lane] = s_pieces[lane] = s_longest[lane] = 0u, s_shortest[lane] = 0xFFFFFFFFu;
   // ranges that overlap could ask for more tiles than there is room for: nothing is done
   bad = __syncthreads_or(bad) != 0;
   if (bad && threadIdx.x == 0) {
@@ -140,7 +147,6 @@ __device__ __forceinline__ GroupedSchedule plan_groups(const GroupedArgs& p, uin
     mirror_code(p.mirror, FGB_S_BAD_OFFSETS);
   }
   if (p.min_part != 0u && !bad) {
-    // the cost of uncut tiles, and of units of 1, 2 and 3 to a CTA: the CTA with the most work, and the pieces
     if (warp == 0) {
       unsigned long long total = 0;
       for (uint32_t g = lane; g < G; g += 32u) {
@@ -152,33 +158,32 @@ __device__ __forceinline__ GroupedSchedule plan_groups(const GroupedArgs& p, uin
       if (lane == 0) s_total = total;
     }
     __syncthreads();
-    if (warp <= kGrMostUnits) {
-      const unsigned long long total = s_total;
-      const uint32_t unit = warp == 0u ? 0xFFFFFFFFu : static_cast<uint32_t>((total + ctas * warp - 1u) / (ctas * warp));
-      uint32_t units = 0, pieces = 0, longest = 0, shortest = 0xFFFFFFFFu;
-      for (uint32_t g = lane; g < G; g += 32u) {
-        const GroupSize z = group_size<kMode>(p, plan.offsets, g);
-        if (z.tiles == 0u) continue;
-        const uint32_t len = part_length(p, z.whole, unit), parts = parts_of(z.whole, len);
-        units += parts * z.tiles;
-        if (parts > 1u) pieces += parts * z.tiles;
-        longest = max(longest, len), shortest = min(shortest, len);
-      }
-      units = __reduce_add_sync(0xffffffffu, units), pieces = __reduce_add_sync(0xffffffffu, pieces);
-      longest = __reduce_max_sync(0xffffffffu, longest), shortest = __reduce_min_sync(0xffffffffu, shortest);
-      if (lane == 0) {
-        const float share = static_cast<float>(total) / ctas;
-        const float most = longest == shortest ? static_cast<float>((units + ctas - 1u) / ctas) * longest : fmaxf(share + 0.5f * longest, longest);
-        s_cost[warp] = most + static_cast<float>(pieces) / ctas * p.piece_cost;
-        s_unit[warp] = unit;
-      }
+    const float share = static_cast<float>(s_total) / static_cast<float>(ctas);
+    const uint32_t unit = lane == 31u ? 0xFFFFFFFFu : static_cast<uint32_t>(ceilf(share * 2.f * exp2f(-2.5849625f / 30.f * static_cast<float>(lane))));
+    uint32_t units = 0, pieces = 0, longest = 0, shortest = 0xFFFFFFFFu;
+    for (uint32_t g = warp; g < G; g += blockDim.x / 32u) {
+      const GroupSize z = group_size<kMode>(p, plan.offsets, g);
+      if (z.tiles == 0u) continue;
+      const uint32_t len = part_length(p, z.whole, max(unit, 1u)), parts = parts_of(z.whole, len);
+      units += parts * z.tiles;
+      if (parts > 1u) pieces += parts * z.tiles;
+      longest = max(longest, len), shortest = min(shortest, len);
+    }
+    atomicAdd(&s_units[lane], units);
+    atomicAdd(&s_pieces[lane], pieces);
+    atomicMax(&s_longest[lane], longest);
+    atomicMin(&s_shortest[lane], shortest);
+    __syncthreads();
+    if (warp == 0) {
+      const float len = static_cast<float>(s_longest[lane]);
+      const float most = s_longest[lane] == s_shortest[lane] ? static_cast<float>((s_units[lane] + ctas - 1u) / ctas) * len : fmaxf(share + 0.5f * len, len);
+      const float cost = most + static_cast<float>(s_pieces[lane]) / static_cast<float>(ctas) * p.piece_cost;
+      // the cheapest, of equally cheap ones the longest
+      const uint32_t least = __reduce_min_sync(0xffffffffu, __float_as_uint(cost));
+      if (static_cast<uint32_t>(__ffs(__ballot_sync(0xffffffffu, __float_as_uint(cost) == least)) - 1) == lane) s_best = max(unit, 1u);
     }
     __syncthreads();
-    uint32_t best = 0;
-#pragma unroll
-    for (uint32_t i = 1; i <= kGrMostUnits; ++i)
-      if (s_cost[i] < s_cost[best]) best = i;
-    plan.unit = s_unit[best];
+    plan.unit = s_best;
   }
   for (uint32_t g = threadIdx.x; g < G; g += blockDim.x) {
     const GroupSize z = group_size<kMode>(p, plan.offsets, g);
@@ -203,13 +208,17 @@ __device__ __forceinline__ GroupedSchedule plan_groups(const GroupedArgs& p, uin
     if (lane == 0) v[0] = 0u;
   }
   __syncthreads();
+  if (p.min_part != 0u && blockIdx.x == 0) {
+    for (uint32_t i = threadIdx.x; i < 3u * (G + 1u); i += blockDim.x) p.plan[i] = s_first[i];
+    if (threadIdx.x == 0) p.plan[3u * (G + 1u)] = plan.unit;
+  }
   return plan;
 }
 
 // A tile, or the part of one that is a unit
 struct GroupedItem {
   uint32_t group, tile;     // tile within the group
-  uint32_t from, to;        // its iterations
+  uint32_t from, to;        // its blocks of k
   uint32_t lo, hi;          // rows of the group
   uint32_t piece;           // its place in the slab, or kInvalid for a whole tile
   uint32_t unit;
@@ -299,23 +308,24 @@ __device__ __forceinline__ void store_columns(uint32_t (&acc)[32], uint8_t* stag
 template <int kMode, typename T, bool kPair>
 __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
                                                                 const __grid_constant__ CUtensorMap tmap_o, const __grid_constant__ GroupedArgs p) {
+  constexpr int kParamDtype = std::is_same<T, __half>::value ? FGB_F16 : std::is_same<T, __nv_bfloat16>::value ? FGB_BF16 : FGB_F32_IEEE;
+  constexpr bool kBlocks = std::is_same<T, float>::value;  // the accumulator is emptied after every block of 64 k
+  constexpr int kSums = kMode == kFew ? 1 : 3;             // blocks of 32 columns that a storing warp adds up
+  constexpr int kStore = kBlocks ? 2048 : 4096;            // a storing warp's buffers
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   GroupedSmem* ctl = reinterpret_cast<GroupedSmem*>(smem);
   uint8_t* ones = smem + 1024;
   float* s_bias = reinterpret_cast<float*>(smem + 1024);  // of the storing warps' columns: 128 each
   uint8_t* stages = smem + kGrCtrlBytes;  // multiples of 1024 from here on
-  const int stage_bytes = kGrPBytes + p.q_bytes;
+  const int plane_bytes = kGrPBytes + p.q_bytes, stage_bytes = p.planes * plane_bytes;  // of a plane: P, then Q
   uint8_t* store = stages + size_t(p.stages) * stage_bytes;
-  uint32_t* first = reinterpret_cast<uint32_t*>(store + kGrStoreBytes);
+  uint32_t* first = reinterpret_cast<uint32_t*>(store + kGrEpilogueWarps * kStore);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = kPair ? cluster_ctarank() : 0u;
   const int half = kPair ? p.bn / 2 : p.bn;  // columns whose operand this CTA holds
   const uint32_t workers = kPair ? gridDim.x / 2u : gridDim.x, worker = kPair ? blockIdx.x / 2u : blockIdx.x;
   volatile uint32_t* abort_flag = &ctl->abort_flag;
-  constexpr int kParamDtype = std::is_same<T, __half>::value ? FGB_F16 : std::is_same<T, __nv_bfloat16>::value ? FGB_BF16 : FGB_F32_IEEE;
-  constexpr bool kBlocks = std::is_same<T, float>::value;  // the accumulator is emptied after every block of 64 k
-  constexpr int kSums = kMode == kFew ? 1 : 3;             // blocks of 32 columns that a storing warp adds up
   auto wait = [&](uint64_t* bar, uint32_t parity) { mbar_wait_tries(bar, parity, abort_flag); };
 
   chain_release();
@@ -368,52 +378,50 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
   if (warp == 8) {
     // ------------------------------------------------------------------ loads
     uint32_t s = 0, ph = 0;
-    const int G = static_cast<int>(p.ranges.count), terms = p.terms;
+    const int G = static_cast<int>(p.ranges.count);
     const uint32_t full_own = uniform(smem_u32(&ctl->full[0])), full_leader = kPair ? uniform(cluster_map(full_own, 0)) : full_own;
     while (__any_sync(0xffffffffu, walk.next(it))) {
       // first row (or channel) of the tile along m and n, first k
       const int m0 = static_cast<int>(uniform(m_tile_of(it) * p.tile_m + rank * 128u)), n0 = static_cast<int>(uniform(n_tile_of(it) * p.bn + rank * half));
-      const int lo = static_cast<int>(uniform(it.lo)), g = static_cast<int>(uniform(it.group));
-      const int n_blocks = static_cast<int>(uniform((it.to - it.from) / terms));
-      int k0 = static_cast<int>(uniform(it.from / terms * 64u));
-      const int len = static_cast<int>(uniform(it.hi - it.lo));
-      for (int kb = 0; kb < n_blocks; ++kb, k0 += 64) {
+      const int lo = static_cast<int>(uniform(it.lo)), g = static_cast<int>(uniform(it.group)), len = static_cast<int>(uniform(it.hi - it.lo));
+      const int k_end = static_cast<int>(uniform(it.to * 64u));
+      for (int k0 = static_cast<int>(uniform(it.from * 64u)); k0 < k_end; k0 += 64) {
         const bool cleared = kMode == kWeight && k0 + 64 > len && (len & 15) != 0;  // see the products
-        for (int term = 0; term < terms; ++term) {
-          wait(&ctl->empty[s], ph ^ 1);
-          if (elect_one()) {
-            // Pairs: both CTAs' bytes count on the leader's barrier, so that it has one to wait for -- but for a block that
-            // either has to clear rows of first.
-            const bool shared = kPair && !cleared;
-            const uint32_t full = shared ? full_leader + 8u * s : full_own + 8u * s;
-            if (!shared || rank == 0u) mbar_arrive_expect_tx(&ctl->full[s], static_cast<uint32_t>(shared ? 2 * stage_bytes : stage_bytes));
-            auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
-              if constexpr (kPair) tma_load_3d_pair(dst, map, full, c0, c1, c2);
-              else tma_load_3d(dst, map, &ctl->full[s], c0, c1, c2);
-            };
-            const uint32_t pd = stage0 + s * stage_bytes, qd = pd + kGrPBytes;
-            const int pp = (p.p_planes >> (4 * term)) & 15, pq = (p.q_planes >> (4 * term)) & 15;
+        wait(&ctl->empty[s], ph ^ 1);
+        if (elect_one()) {
+          // Pairs: both CTAs' bytes count on the leader's barrier, so that it has one to wait for -- but for a block that
+          // either has to clear rows of first.
+          const bool shared = kPair && !cleared;
+          const uint32_t full = shared ? full_leader + 8u * s : full_own + 8u * s;
+          if (!shared || rank == 0u) mbar_arrive_expect_tx(&ctl->full[s], static_cast<uint32_t>(shared ? 2 * stage_bytes : stage_bytes));
+          auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
+            if constexpr (kPair) tma_load_3d_pair(dst, map, full, c0, c1, c2);
+            else tma_load_3d(dst, map, &ctl->full[s], c0, c1, c2);
+          };
+          uint32_t pd = stage0 + s * stage_bytes;
+          for (int i = 0; i < p.planes; ++i, pd += plane_bytes) {
+            const uint32_t qd = pd + kGrPBytes;
             if constexpr (kMode == kRows) {
-              load(pd, &tmap_p, k0, lo + m0, pp);
+              load(pd, &tmap_p, k0, lo + m0, i);
               if (p.q_mn) {
-                for (int c = 0; c * 64 < half; ++c) load(qd + c * 8192, &tmap_q, n0 + c * 64, k0, pq * G + g);
+                for (int c = 0; c * 64 < half; ++c) load(qd + c * 8192, &tmap_q, n0 + c * 64, k0, i * G + g);
               } else {
-                load(qd, &tmap_q, k0, n0, pq * G + g);
+                load(qd, &tmap_q, k0, n0, i * G + g);
               }
             } else if constexpr (kMode == kFew) {
               if (p.p_mn) {
-                for (int c = 0; c < 2; ++c) load(pd + c * 8192, &tmap_p, m0 + c * 64, k0, pp * G + g);
+                for (int c = 0; c < 2; ++c) load(pd + c * 8192, &tmap_p, m0 + c * 64, k0, i * G + g);
               } else {
-                load(pd, &tmap_p, k0, m0, pp * G + g);
+                load(pd, &tmap_p, k0, m0, i * G + g);
               }
-              load(qd, &tmap_q, k0, lo + n0, pq);
+              load(qd, &tmap_q, k0, lo + n0, i);
             } else {
-              for (int c = 0; c < 2; ++c) load(pd + c * 8192, &tmap_p, m0 + c * 64, lo + k0, pp);
-              for (int c = 0; c * 64 < half; ++c) load(qd + c * 8192, &tmap_q, n0 + c * 64, lo + k0, pq);
+              for (int c = 0; c < 2; ++c) load(pd + c * 8192, &tmap_p, m0 + c * 64, lo + k0, i);
+              for (int c = 0; c * 64 < half; ++c) load(qd + c * 8192, &tmap_q, n0 + c * 64, lo + k0, i);
             }
           }
-          if (++s == static_cast<uint32_t>(p.stages)) s = 0, ph ^= 1;
         }
+        if (++s == static_cast<uint32_t>(p.stages)) s = 0, ph ^= 1;
       }
     }
   } else if (warp == 9) {
@@ -441,77 +449,75 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
     };
     uint32_t own_ph = 0, peer_ph = 0;  // a bit for each stage: the phases of the barriers that only cleared blocks use
     while (__any_sync(0xffffffffu, walk.next(it))) {
-      const uint32_t n_blocks = uniform((it.to - it.from) / p.terms);
-      uint32_t left = uniform((kMode == kWeight ? it.hi - it.lo : static_cast<uint32_t>(p.k_extent)) - it.from / p.terms * 64u);  // k from here on
-      uint32_t turn = kMode == kWeight ? uniform((it.from / p.terms + p.n_tiles - n_tile_of(it)) % p.n_tiles) : 0u;  // 0: the ones' products are ours
-      uint32_t any = 0, any_ones = 0, acc = 0;
+      const uint32_t n_blocks = uniform(it.to - it.from);
+      uint32_t left = uniform((kMode == kWeight ? it.hi - it.lo : static_cast<uint32_t>(p.k_extent)) - it.from * 64u);  // k from here on
+      uint32_t turn = kMode == kWeight ? uniform((it.from + p.n_tiles - n_tile_of(it)) % p.n_tiles) : 0u;  // 0: the ones' products are ours
+      uint32_t any_ones = 0, acc = 0;
       for (uint32_t kb = 0; kb < n_blocks; ++kb) {
         const uint32_t valid = min(left, 64u), steps = (valid + 15u) / 16u;
         const bool cleared = kMode == kWeight && (valid & 15u) != 0u;
         const bool with_ones = kMode == kWeight && p.db != nullptr && turn == 0u;
-        for (int term = 0; term < p.terms; ++term) {
-          if (leader || cleared) {
-            if (leader && any == 0u) {  // a new accumulator
-              wait(&ctl->acc_empty[set], set_ph ^ 1);
-              tc_fence_after_sync();
-              acc = tmem0 + set * p.acc_stride;
-            }
-            if (leader) {
-              wait(&ctl->full[s], ph);
-            } else {
-              wait(&ctl->full[s], own_ph >> s & 1u);
-              own_ph ^= 1u << s;
-            }
-            if (cleared) {
-              // rows of other groups in the last step: cleared in both operands
-              __syncwarp();
-              const uint32_t chunks = 2u + (half + 63u) / 64u, rows = steps * 16u - valid;
-              uint8_t* at = stages + size_t(s) * stage_bytes;
-              for (uint32_t c = 0; c < chunks; ++c)
-                for (uint32_t r = lane >> 3; r < rows; r += 4u)
-                  *reinterpret_cast<uint4*>(at + c * 8192u + (valid + r) * 128u + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-              fence_proxy_async_smem();
-              __syncwarp();
-              if constexpr (kPair) {
-                // the peer's ordinary stores: cluster scope on both sides, here only (a wait of that scope takes some 1000 cycles)
-                if (leader) mbar_wait_cluster(&ctl->peer_full[s], peer_ph >> s & 1u, abort_flag);
-                else if (lane == 0) mbar_arrive_cluster_release(peer_full0 + 8u * s);
-                peer_ph ^= 1u << s;
-                __syncwarp();
-              }
-            }
-          }
-          const bool ones_now = with_ones && ((p.q_planes >> (4 * term)) & 15u) == 0u;  // once for each plane of dy
-          if (leader) {
-            if (elect_one()) {
-              const uint64_t dp = dp0 + ((s * stage_bytes) >> 4), dq = dq0 + ((s * stage_bytes) >> 4);
-#pragma unroll
-              for (uint32_t k = 0; k < 4; ++k) {
-                if (k < steps) {
-                  product(acc, dp + k * p_step, dq + k * q_step, p.idesc, k == 0 ? any : 1u);
-                  if (ones_now) product(acc + p.bn, dp + k * p_step, d_ones, p.idesc_ones, k == 0 ? any_ones : 1u);
-                }
-              }
-              commit(empty0, empty1, s);
-            }
-          }
-          any = 1u;
-          any_ones |= ones_now ? 1u : 0u;
-          if (++s == static_cast<uint32_t>(p.stages)) s = 0, ph ^= 1;
+        const bool begins = kBlocks || kb == 0u;  // a new accumulator
+        if (begins && leader) {
+          wait(&ctl->acc_empty[set], set_ph ^ 1);
+          tc_fence_after_sync();
+          acc = tmem0 + set * p.acc_stride;
+          any_ones = 0;
         }
+        if (leader) {
+          wait(&ctl->full[s], ph);
+        } else if (cleared) {
+          wait(&ctl->full[s], own_ph >> s & 1u);
+          own_ph ^= 1u << s;
+        }
+        if (cleared) {
+          // rows of other groups in the last step: cleared in both operands
+          __syncwarp();
+          const uint32_t chunks = static_cast<uint32_t>(stage_bytes) / 8192u, rows = steps * 16u - valid;
+          uint8_t* at = stages + size_t(s) * stage_bytes;
+          for (uint32_t c = 0; c < chunks; ++c)
+            for (uint32_t r = lane >> 3; r < rows; r += 4u)
+              *reinterpret_cast<uint4*>(at + c * 8192u + (valid + r) * 128u + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if constexpr (kPair) {
+            // the peer's ordinary stores: cluster scope on both sides, here only (a wait of that scope takes some 1000 cycles)
+            if (leader) mbar_wait_cluster(&ctl->peer_full[s], peer_ph >> s & 1u, abort_flag);
+            else if (lane == 0) mbar_arrive_cluster_release(peer_full0 + 8u * s);
+            peer_ph ^= 1u << s;
+            __syncwarp();
+          }
+        }
+        if (leader && elect_one()) {
+          const uint64_t dp = dp0 + ((s * stage_bytes) >> 4), dq = dq0 + ((s * stage_bytes) >> 4);
+          for (int term = 0; term < p.terms; ++term) {
+            const uint32_t pp = (p.p_planes >> (4 * term)) & 15u, pq = (p.q_planes >> (4 * term)) & 15u;
+            const uint64_t da = dp + ((pp * plane_bytes) >> 4), db = dq + ((pq * plane_bytes) >> 4);
+            const uint32_t add = begins && term == 0 ? 0u : 1u;
+            const bool ones_now = with_ones && pq == 0u;  // once for each plane of dy
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+              if (k < steps) {
+                product(acc, da + k * p_step, db + k * q_step, p.idesc, k == 0 ? add : 1u);
+                if (ones_now) product(acc + p.bn, da + k * p_step, d_ones, p.idesc_ones, k == 0 ? any_ones : 1u);
+              }
+            }
+            if (ones_now) any_ones = 1u;
+          }
+          commit(empty0, empty1, s);
+          if (kBlocks || kb + 1u == n_blocks) commit(acc_full0, acc_full1, set);  // the accumulator is done
+        }
+        if (with_ones) any_ones = 1u;
+        if (++s == static_cast<uint32_t>(p.stages)) s = 0, ph ^= 1;
         left -= 64u;
         if (kMode == kWeight && ++turn == static_cast<uint32_t>(p.n_tiles)) turn = 0u;
-        if (kBlocks || kb + 1u == n_blocks) {  // the accumulator is done: the block's, or the tile's last
-          if (leader && elect_one()) commit(acc_full0, acc_full1, set);
-          if (++set == static_cast<uint32_t>(p.acc_sets)) set = 0, set_ph ^= 1;
-          any = any_ones = 0u;
-        }
+        if ((kBlocks || kb + 1u == n_blocks) && ++set == static_cast<uint32_t>(p.acc_sets)) set = 0, set_ph ^= 1;
       }
     }
   } else {
     // ------------------------------------------------------------------ stores
     const int quarter = warp & 3, group = warp >> 2;
-    uint8_t* stage = store + warp * 4096;  // two buffers of 32 rows x 64 bytes
+    uint8_t* stage = store + warp * kStore;  // 16-bit results: two buffers of 32 rows x 64 bytes
     float* bias_buf = s_bias + warp * 128;
     uint32_t buffer = 0;
     uint32_t set = 0, set_ph = 0;
@@ -561,8 +567,7 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
         for (int b = 0; b < kSums; ++b)
 #pragma unroll
           for (int i = 0; i < 32; ++i) sum[b][i] = 0u;
-        for (uint32_t at = it.from; at < it.to;) {
-          const uint32_t end = at + p.terms;  // a unit has whole blocks
+        for (uint32_t at = it.from; at < it.to; ++at) {
           tmem = wait_full();
 #pragma unroll
           for (int b = 0; b < kSums; ++b) {
@@ -574,14 +579,13 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
               for (int i = 0; i < 32; ++i) sum[b][i] = __float_as_uint(__uint_as_float(sum[b][i]) + __uint_as_float(acc[i]));
             }
           }
-          if (with_db && ones_in(it, at / p.terms)) {
+          if (with_db && ones_in(it, at)) {
             uint32_t acc[32];
             tmem_ld_32x32(tmem + p.bn, acc);
             tmem_ld_wait();
             db += __uint_as_float(acc[0]);
           }
           give_back();
-          at = end;
         }
       } else {
         tmem = wait_full();
@@ -700,16 +704,17 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
 
 // ------------------------------------------------------------------ pieces
 // Tiles in parts: their pieces added in order; and the tiles of empty groups (weight gradient), of which there are no units:
-// zeros.  gridDim.y CTAs a tile; `ctas`: those of the products' kernel.
+// zeros.  gridDim.y CTAs a tile.
 constexpr int kGrJoinThreads = 256;
 template <int kMode, typename T>
-__global__ void __launch_bounds__(kGrJoinThreads) grouped_join_kernel(const __grid_constant__ GroupedArgs p, uint32_t ctas, uint32_t tiles) {
-  extern __shared__ uint32_t s_first[];
+__global__ void __launch_bounds__(kGrJoinThreads) grouped_join_kernel(const __grid_constant__ GroupedArgs p, uint32_t tiles) {
+  __shared__ uint32_t s_count;
   constexpr int kParamDtype = std::is_same<T, __half>::value ? FGB_F16 : std::is_same<T, __nv_bfloat16>::value ? FGB_BF16 : FGB_F32_IEEE;
   chain_release();
   chain_wait();
-  const GroupedSchedule plan = plan_groups<kMode>(p, s_first, ctas);
   const uint32_t G = p.ranges.count;
+  const uint32_t *first = p.plan, *piece = p.plan + G + 1u, *offsets = p.plan + 2u * (G + 1u);
+  const uint32_t unit = p.plan[3u * (G + 1u)];
   for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
     uint32_t g, tile;
     if constexpr (kMode == kWeight) {
@@ -717,25 +722,27 @@ __global__ void __launch_bounds__(kGrJoinThreads) grouped_join_kernel(const __gr
       g = t / per, tile = t - g * per;
     } else {
       // all tiles have equally many parts: that of tile t's first is t * parts
-      const uint32_t whole = static_cast<uint32_t>(p.k_blocks * p.terms), parts = parts_of(whole, part_length(p, whole, plan.unit));
-      if (uint64_t(t) * parts >= plan.first[G]) return;
-      uint32_t lo = 0, hi = G - 1u;
-      while (lo < hi) {
-        const uint32_t mid = (lo + hi + 1u) / 2u;
-        if (plan.first[mid] <= t * parts) lo = mid;
-        else hi = mid - 1u;
-      }
-      g = lo, tile = t - plan.first[g] / parts;
+      const uint32_t whole = static_cast<uint32_t>(p.k_blocks), parts = parts_of(whole, part_length(p, whole, unit));
+      if (uint64_t(t) * parts >= first[G]) return;
+      if (threadIdx.x == 0) s_count = 0;
+      __syncthreads();
+      uint32_t before = 0;  // groups that begin at or before the tile, the last of which is not empty
+      for (uint32_t i = threadIdx.x; i < G; i += kGrJoinThreads) before += first[i] <= t * parts ? 1u : 0u;
+      atomicAdd(&s_count, before);
+      __syncthreads();
+      g = s_count - 1u, tile = t - first[g] / parts;
+      __syncthreads();
     }
-    const GroupSize z = group_size<kMode>(p, plan.offsets, g);
-    const uint32_t pieces = z.tiles == 0u ? 0u : parts_of(z.whole, part_length(p, z.whole, plan.unit));
+    const GroupSize z = group_size<kMode>(p, offsets, g);
+    // none where the group is empty (or the offsets were bad)
+    const uint32_t pieces = first[g] == first[g + 1u] ? 0u : parts_of(z.whole, part_length(p, z.whole, unit));
     const uint32_t elements = static_cast<uint32_t>(p.tile_m) * p.bn;
     if (kMode == kWeight && p.db != nullptr && tile % p.n_tiles == 0u && blockIdx.y == 0u && threadIdx.x < p.tile_m) {
       // the shares of db: of every part of the n tiles that read the same rows of dy
       const uint32_t m = tile / p.n_tiles * p.tile_m + threadIdx.x;
       if (m < static_cast<uint32_t>(p.m_extent)) {
         float v = 0.f;
-        const float* share = p.db_parts + (size_t(plan.first[g]) + tile) * p.tile_m + threadIdx.x;
+        const float* share = p.db_parts + (size_t(first[g]) + tile) * p.tile_m + threadIdx.x;
         for (uint32_t k = 0; k < pieces; ++k)
 #pragma unroll 4
           for (int n = 0; n < p.n_tiles; ++n) v += share[(size_t(k) * z.tiles + n) * p.tile_m];
@@ -744,7 +751,7 @@ __global__ void __launch_bounds__(kGrJoinThreads) grouped_join_kernel(const __gr
     }
     if (pieces == 1u) continue;  // stored as a whole
     const size_t apart = size_t(elements) * z.tiles;
-    const float* from = p.slab + size_t(elements) * (plan.piece[g] + tile);
+    const float* from = p.slab + size_t(elements) * (piece[g] + tile);
     // four elements a thread: neighbours in the piece, and in the output
     const uint32_t quads = elements / 4u, share = (quads + gridDim.y - 1u) / gridDim.y;
     const uint32_t q0 = blockIdx.y * share, q1 = min(quads, q0 + share);
@@ -792,32 +799,58 @@ __global__ void __launch_bounds__(kGrJoinThreads) grouped_join_kernel(const __gr
 // dst[plane][rows][cp] (16-bit) of src[rows][c]: fp32 as bf16 planes hi + mid + lo, 16-bit types as they are; columns from c
 // on are zero.  A plane takes what the planes before it left, rounded to nearest; a value that would round to infinity is
 // cut to the largest number instead, and nothing is left of an infinity or a NaN.
+// A thread makes eight columns of a row.
 template <typename T>
-__global__ void __launch_bounds__(256) grouped_planes_kernel(const T* __restrict__ src, uint16_t* __restrict__ dst, uint64_t rows, int c, int cp, int planes) {
+__global__ void __launch_bounds__(256) grouped_planes_kernel(const T* __restrict__ src, uint16_t* __restrict__ dst, uint32_t rows, int c, int cp, int planes) {
   chain_release();
   chain_wait();
-  const uint64_t total = rows * cp;
-  for (uint64_t i = (uint64_t(blockIdx.x) * 256 + threadIdx.x) * 2; i < total; i += uint64_t(gridDim.x) * 512) {
-    const uint64_t r = i / cp;
-    const int col = static_cast<int>(i - r * cp);  // even, as cp is
-    uint16_t q[3][2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
+  const int packs = cp / 8, width = min(packs, 256), lanes = 256 / width;
+  const int cx = threadIdx.x % width, ry = threadIdx.x / width;
+  if (ry >= lanes) return;
+  const size_t plane = size_t(rows) * cp;
+  const bool whole = sizeof(T) == 4 && c % 4 == 0;
+  for (uint32_t r = blockIdx.x * lanes + ry; r < rows; r += gridDim.x * lanes) {
+    for (int q = cx; q < packs; q += width) {
+      const T* from = src + size_t(r) * c + q * 8;
+      uint16_t* to = dst + size_t(r) * cp + q * 8;
+      const int have = min(8, c - q * 8);
+      uint32_t out[3][4];
       if constexpr (sizeof(T) == 2) {
-        q[0][j] = col + j < c ? reinterpret_cast<const uint16_t*>(src)[r * c + col + j] : uint16_t(0);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(from);
+          out[0][i / 2] = (i < have ? uint32_t(h[i]) : 0u) | (i + 1 < have ? uint32_t(h[i + 1]) << 16 : 0u);
+        }
       } else {
-        float v = col + j < c ? src[r * c + col + j] : 0.f;
+        float v[8];
+        if (whole) {
+          const float4 a = __ldg(reinterpret_cast<const float4*>(from)), b = have == 8 ? __ldg(reinterpret_cast<const float4*>(from) + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = i < have ? from[i] : 0.f;
+        }
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
-          __nv_bfloat16 h = __float2bfloat16_rn(v);
-          if (__hisinf(h) && !isinf(v)) h = __ushort_as_bfloat16(static_cast<unsigned short>(v < 0.f ? 0xFF7Fu : 0x7F7Fu));
-          q[k][j] = __bfloat16_as_ushort(h);
-          v = isfinite(v) ? v - __bfloat162float(h) : 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            uint32_t two = 0;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float& x = v[i + j];
+              __nv_bfloat16 h = __float2bfloat16_rn(x);
+              if (__hisinf(h) && !isinf(x)) h = __ushort_as_bfloat16(static_cast<unsigned short>(x < 0.f ? 0xFF7Fu : 0x7F7Fu));
+              two |= uint32_t(__bfloat16_as_ushort(h)) << (16 * j);
+              x = isfinite(x) ? x - __bfloat162float(h) : 0.f;
+            }
+            out[k][i / 2] = two;
+          }
         }
       }
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        if (k < planes) *reinterpret_cast<uint4*>(to + k * plane) = make_uint4(out[k][0], out[k][1], out[k][2], out[k][3]);
     }
-    for (int k = 0; k < planes; ++k)
-      *reinterpret_cast<uint32_t*>(dst + uint64_t(k) * total + i) = uint32_t(q[k][0]) | uint32_t(q[k][1]) << 16;
   }
 }
 
@@ -846,11 +879,11 @@ static cudaError_t make_operand(Operand& o, const void* src, int64_t rows, int c
   uint16_t* dst = reinterpret_cast<uint16_t*>(at);
   at += plane_bytes(rows, c, dtype);
   o.base = dst;
-  const int64_t pairs = rows * o.cp / 2;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ceil_div(pairs, 256), int64_t(device_sm_count()) * 16));
+  const int64_t lanes = 256 / std::min(o.cp / 8, 256);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ceil_div(rows, lanes), int64_t(device_sm_count()) * 16));
   if (is_f32(dtype))
-    return launch_chained(grouped_planes_kernel<float>, dim3(grid), dim3(256), 0, s, static_cast<const float*>(src), dst, static_cast<uint64_t>(rows), c, o.cp, o.planes);
-  return launch_chained(grouped_planes_kernel<__half>, dim3(grid), dim3(256), 0, s, static_cast<const __half*>(src), dst, static_cast<uint64_t>(rows), c, o.cp, 1);
+    return launch_chained(grouped_planes_kernel<float>, dim3(grid), dim3(256), 0, s, static_cast<const float*>(src), dst, static_cast<uint32_t>(rows), c, o.cp, o.planes);
+  return launch_chained(grouped_planes_kernel<__half>, dim3(grid), dim3(256), 0, s, static_cast<const __half*>(src), dst, static_cast<uint32_t>(rows), c, o.cp, 1);
 }
 
 // columns of a tile over `extent` channels: all of them in steps of 32 up to `most`, else equal tiles in steps of 64
@@ -863,7 +896,8 @@ static int tile_columns(int extent, int most) {
 struct GroupedPlan {
   int mode, bn, split, pair;
   int64_t pieces;       // that the slab holds
-  int64_t slab_bytes, db_bytes;
+  int64_t slab_bytes, db_bytes, plan_bytes;
+  int64_t bytes() const { return slab_bytes + db_bytes + plan_bytes; }
   uint32_t min_part;
   int acc_stride;
   int64_t tiles;        // most tiles (those that the join kernel looks at)
@@ -873,19 +907,20 @@ struct GroupedPlan {
 static bool few_rows(const fgb_grouped_linear_call& c) { return c.n <= 64 * c.groups; }
 
 static int grouped_plan(const fgb_grouped_linear_call& c, int pass, GroupedPlan& p) {
-  const int64_t sms = device_sm_count(), terms = c.dtype == FGB_F32_IEEE ? 6 : c.dtype == FGB_F32_TF32 ? 3 : 1;
+  const int64_t sms = device_sm_count();
   const int64_t N = c.n, G = c.groups;
-  const int most = is_f32(c.dtype) ? 192 : 256;  // fp32: the blocks' sums of a tile are held in 3 x 32 registers
-  int64_t iterations, db_units = 0;
+  // fp32: the blocks' sums of a tile are held in 3 x 32 registers, and two stages of three planes in shared memory
+  auto most = [&](bool pair) { return !is_f32(c.dtype) ? 256 : pair ? 192 : 96; };
+  int64_t blocks, db_units = 0;
   p = GroupedPlan{};
   if (pass == 2) {
     p.mode = kWeight;
     p.pair = c.co > 128 && c.ci > 64;
-    p.bn = tile_columns(c.ci, most);
+    p.bn = tile_columns(c.ci, most(p.pair));
     const int64_t per = ceil_div(c.ci, p.bn) * ceil_div(c.co, p.pair ? 256 : 128);
     p.tiles = G * per;
-    iterations = (N / 64 + G) * per * terms;
-    p.split = 1, p.min_part = static_cast<uint32_t>(4 * terms);
+    blocks = (N / 64 + G) * per;
+    p.split = 1, p.min_part = 4;
     if (c.grad_bias != nullptr) db_units = p.tiles;
   } else {
     const int nout = pass == 0 ? c.co : c.ci, k = pass == 0 ? c.ci : c.co;
@@ -896,22 +931,23 @@ static int grouped_plan(const fgb_grouped_linear_call& c, int pass, GroupedPlan&
       p.bn = N <= 16 || N <= 4 * G ? 16 : N <= 16 * G ? 32 : 64;
       const int64_t m_tiles = ceil_div(nout, 128);
       p.tiles = std::min<int64_t>(N, N / p.bn + G) * m_tiles;
-      iterations = p.tiles * kb * terms;
-      if (p.tiles <= sms / 2 && kb >= 8) p.split = 1, p.min_part = static_cast<uint32_t>(4 * terms);
+      blocks = p.tiles * kb;
+      if (p.tiles <= sms / 2 && kb >= 8) p.split = 1, p.min_part = 4;
     } else {
       p.mode = kRows;
       p.pair = N >= 512 * G && nout > 64;
-      p.bn = tile_columns(nout, most);
+      p.bn = tile_columns(nout, most(p.pair));
       p.tiles = (N / (p.pair ? 256 : 128) + G) * ceil_div(nout, p.bn);
-      iterations = p.tiles * kb * terms;
+      blocks = p.tiles * kb;
     }
   }
-  if (iterations >= (int64_t(1) << 31) - 1) return FGB_E_SIZE;
+  if (blocks >= (int64_t(1) << 31) - 1) return FGB_E_SIZE;
   // two accumulators a tile; the products with ones take 32 columns more
   p.acc_stride = std::max(p.bn, 32) + (pass == 2 && c.grad_bias != nullptr ? 32 : 0);
   const int64_t tile_m = p.pair ? 256 : 128, workers = p.pair ? sms / 2 : sms;
   // a part has half of the wanted length at least (a tile is cut only where it is longer), and min_part at least
-  p.pieces = p.split ? std::min<int64_t>(2 * kGrMostUnits * workers, iterations / p.min_part) : 0;
+  p.pieces = p.split ? std::min<int64_t>(2 * kGrMostUnits * workers + 2, blocks / p.min_part) : 0;
+  p.plan_bytes = p.split ? schedule_bytes(G) : 0;
   p.slab_bytes = align256(p.pieces * tile_m * p.bn * 4);
   p.db_bytes = db_units > 0 ? align256((db_units + p.pieces) * tile_m * 4) : 0;
   return FGB_OK;
@@ -934,8 +970,8 @@ static int64_t backward_planes(const fgb_grouped_linear_call& c) {
 template <int kMode, typename T, bool kPair>
 static int launch_grouped(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMap& to, GroupedArgs& a, const GroupedPlan& p, cudaStream_t s) {
   const int prefix = static_cast<int>(schedule_bytes(a.ranges.count));
-  const int fixed = 1024 + kGrCtrlBytes + kGrStoreBytes + prefix;
-  const int stage = kGrPBytes + a.q_bytes;
+  const int fixed = 1024 + kGrCtrlBytes + kGrEpilogueWarps * (sizeof(T) == 4 ? 2048 : 4096) + prefix;
+  const int stage = a.planes * (kGrPBytes + a.q_bytes);
   a.stages = std::min(kGrMaxStages, (kGrSmemLimit - fixed) / stage);
   const size_t smem = size_t(fixed) + size_t(a.stages) * stage;
   static PerDeviceTable configured;
@@ -948,7 +984,7 @@ static int launch_grouped(const CUtensorMap& tp, const CUtensorMap& tq, const CU
     if constexpr (kMode != kRows) {
       const unsigned tiles = static_cast<unsigned>(p.tiles), x = std::min(tiles, 65535u * 8u);
       const unsigned y = static_cast<unsigned>(std::clamp<int64_t>(ceil_div(int64_t(device_sm_count()) * 8, tiles), 1, 64));
-      e = launch_chained(grouped_join_kernel<kMode, T>, dim3(x, y), dim3(kGrJoinThreads), size_t(prefix), s, a, grid, tiles);
+      e = launch_chained(grouped_join_kernel<kMode, T>, dim3(x, y), dim3(kGrJoinThreads), 0, s, a, tiles);
     }
   }
   return e != cudaSuccess ? cuda_status(e) : launch_status();
@@ -963,14 +999,15 @@ static int grouped_pass(const fgb_grouped_linear_call& c, int pass, const Operan
   a.ranges = RowRanges{c.offsets, c.offsets_bits == 64, static_cast<uint32_t>(c.n), static_cast<uint32_t>(c.groups)};
   a.bn = p.bn, a.tile_m = p.pair ? 256 : 128;
   const int half = p.pair ? p.bn / 2 : p.bn;
+  a.planes = planes_of(c.dtype);
   a.terms = c.dtype == FGB_F32_IEEE ? 6 : c.dtype == FGB_F32_TF32 ? 3 : 1;
   // the small products first: (lo hi) (hi lo) (mid mid) (mid hi) (hi mid) (hi hi), or the last three of them
   a.p_planes = a.terms == 6 ? 0x001102u : a.terms == 3 ? 0x001u : 0u, a.q_planes = a.terms == 6 ? 0x010120u : a.terms == 3 ? 0x010u : 0u;
   a.min_part = p.min_part;
-  a.piece_cost = static_cast<uint32_t>(ceil_div(10 * p.bn, 256));  // 128 KB a CTA written, then read: the time of some ten stages
+  a.piece_cost = 10.f * static_cast<float>(p.bn) / 256.f / static_cast<float>(a.terms);  // 128 KB a CTA written, then read: some ten stages' time
   a.acc_stride = p.acc_stride;
   a.acc_sets = 2 * p.acc_stride <= 512 ? 2 : 1;
-  a.slab = slab, a.db_parts = slab + p.slab_bytes / 4;
+  a.slab = slab, a.db_parts = slab + p.slab_bytes / 4, a.plan = reinterpret_cast<uint32_t*>(slab + (p.slab_bytes + p.db_bytes) / 4);
   a.status = c.status, a.mirror = status_mirror(c.status);
   const uint32_t fmt = features.dtype16 == FGB_F16 ? kFmtF16 : kFmtBF16;
   a.one_pair = features.dtype16 == FGB_F16 ? 0x3C003C00u : 0x3F803F80u;
@@ -1044,7 +1081,7 @@ extern "C" int64_t fgb_grouped_linear_workspace_bytes(const fgb_grouped_linear_c
   int64_t bytes = 256;
   if (!backward) {
     rc = grouped_plan(*c, 0, p);
-    bytes += p.slab_bytes + plane_bytes(c->n, c->ci, c->dtype) + plane_bytes(c->groups * c->co, c->ci, c->dtype);
+    bytes += p.bytes() + plane_bytes(c->n, c->ci, c->dtype) + plane_bytes(c->groups * c->co, c->ci, c->dtype);
     return rc != FGB_OK ? rc : bytes;
   }
   int64_t slab = 0;
@@ -1052,7 +1089,7 @@ extern "C" int64_t fgb_grouped_linear_workspace_bytes(const fgb_grouped_linear_c
     if (pass == 1 ? c->grad_x == nullptr : c->grad_weight == nullptr) continue;
     rc = grouped_plan(*c, pass, p);
     if (rc != FGB_OK) return rc;
-    slab = std::max(slab, p.slab_bytes + p.db_bytes);
+    slab = std::max(slab, p.bytes());
   }
   return bytes + slab + backward_planes(*c);
 }
@@ -1071,7 +1108,7 @@ extern "C" int fgb_grouped_linear_forward(const fgb_grouped_linear_call* c, void
   if (rc != FGB_OK) return rc;
   char* at = static_cast<char*>(c->workspace);
   float* slab = reinterpret_cast<float*>(at);
-  at += p.slab_bytes;
+  at += p.bytes();
   Operand x, w;
   cudaError_t e = make_operand(x, c->x, c->n, c->ci, c->dtype, at, s);
   if (e == cudaSuccess) e = make_operand(w, c->weight, c->groups * c->co, c->ci, c->dtype, at, s);
