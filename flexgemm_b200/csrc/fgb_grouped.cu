@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
   constexpr int kParamDtype = std::is_same<T, __half>::value ? FGB_F16 : std::is_same<T, __nv_bfloat16>::value ? FGB_BF16 : FGB_F32_IEEE;
   constexpr bool kBlocks = std::is_same<T, float>::value;  // the accumulator is emptied after every block of 64 k
   constexpr int kSums = kMode == kFew ? 1 : 3;             // blocks of 32 columns that a storing warp adds up
-  constexpr int kStore = kBlocks ? 2048 : 4096;            // a storing warp's buffers
+  constexpr int kStore = kBlocks ? 2048 : 4096;            // a storing warp's buffer: 32 rows of 64 or 128 bytes
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   GroupedSmem* ctl = reinterpret_cast<GroupedSmem*>(smem);
@@ -517,12 +517,9 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
   } else {
     // ------------------------------------------------------------------ stores
     const int quarter = warp & 3, group = warp >> 2;
-    uint8_t* stage = store + warp * kStore;  // 16-bit results: two buffers of 32 rows x 64 bytes
+    uint8_t* stage = store + warp * kStore;
     float* bias_buf = s_bias + warp * 128;
-    uint32_t buffer = 0;
     uint32_t set = 0, set_ph = 0;
-    // this warp's columns are [32 group, 32 group + 32) of every 64: at most 3 x 32 of them in fp32
-    uint32_t sum[kBlocks ? kSums : 1][32];
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t acc_empty[2] = {kPair ? cluster_map(smem_u32(&ctl->acc_empty[0]), 0) : 0u, kPair ? cluster_map(smem_u32(&ctl->acc_empty[1]), 0) : 0u};
     auto wait_full = [&]() {
@@ -539,36 +536,79 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
       }
       if (++set == static_cast<uint32_t>(p.acc_sets)) set = 0, set_ph ^= 1;
     };
-    while (walk.next(it)) {
+    // This warp's columns: the [kOwn group, kOwn group + kOwn) of every 2 kOwn.
+    constexpr int kOwn = kBlocks || kMode == kFew ? 32 : 64;
+    // The next unit, and the bias of its columns, are looked up while this one's accumulator is waited for and stored.
+    const bool with_bias = kMode == kRows && p.bias != nullptr;
+    float bias[4];
+    GroupedItem next;
+    auto look_up = [&]() {
+      const bool more = walk.next(next);
+      if (with_bias && more) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int in = kOwn == 32 ? group * 32 + b * 64 + lane : group * 64 + (b / 2) * 128 + (b % 2) * 32 + lane, c = static_cast<int>(n_tile_of(next)) * p.bn + in;
+          bias[b] = in < p.bn && c < p.n_extent ? load_param(p.bias, kParamDtype, int64_t(next.group) * p.n_extent + c) : 0.f;
+        }
+      }
+      return more;
+    };
+    for (bool more = look_up(); more;) {
+      it = next;
+      if (with_bias) {
+        __syncwarp();
+#pragma unroll
+        for (int b = 0; b < 4; ++b) bias_buf[b * 32 + lane] = bias[b];
+        __syncwarp();
+      }
+      more = look_up();
       const int in_tile = static_cast<int>(rank) * 128 + quarter * 32;  // the warp's first row within the tile
       const int m0 = static_cast<int>(m_tile_of(it)) * p.tile_m + in_tile, n0 = static_cast<int>(n_tile_of(it)) * p.bn;
       const bool whole = it.piece == kInvalid;
       const bool with_db = kMode == kWeight && p.db != nullptr && group == 0;
-      float db = 0.f;
-      uint32_t tmem = 0;
-      // 16-bit results go out by TMA (rows of other matrices are cut off by the map; rows of other groups by nothing, so all 32
-      // have to be the group's); else, and for pieces, by ordinary stores, for which both buffers have to be free
-      const bool by_tma = !kBlocks && kMode != kFew && whole && p.vec_ok && (kMode == kWeight || static_cast<int>(it.hi - it.lo) - m0 >= 32);
-      if (kMode != kFew && !by_tma) {
-        if (elect_one()) bulk_wait_read<0>();
-        __syncwarp();
-      }
-      if (kMode == kRows && p.bias != nullptr) {
-        __syncwarp();
+      float* piece = whole ? nullptr : p.slab + size_t(it.piece) * p.tile_m * p.bn;
+      const int64_t row0 = kMode == kRows ? int64_t(it.lo) + m0 : int64_t(it.group) * p.m_extent + m0;
+      const int rows = (kMode == kRows ? static_cast<int>(it.hi - it.lo) : p.m_extent) - m0;
+      auto add_bias = [&](uint32_t (&acc)[32], int b) {
+        if (!with_bias) return;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const int c = n0 + group * 32 + b * 64 + lane;
-          bias_buf[b * 32 + lane] = group * 32 + b * 64 < p.bn && c < p.n_extent ? load_param(p.bias, kParamDtype, int64_t(it.group) * p.n_extent + c) : 0.f;
+        for (int i = 0; i < 8; ++i) {
+          const float4 v = reinterpret_cast<const float4*>(bias_buf + b * 32)[i];
+          acc[4 * i] = __float_as_uint(__uint_as_float(acc[4 * i]) + v.x), acc[4 * i + 1] = __float_as_uint(__uint_as_float(acc[4 * i + 1]) + v.y);
+          acc[4 * i + 2] = __float_as_uint(__uint_as_float(acc[4 * i + 2]) + v.z), acc[4 * i + 3] = __float_as_uint(__uint_as_float(acc[4 * i + 3]) + v.w);
         }
-        __syncwarp();
-      }
+      };
+      // 32 columns by ordinary stores; `b`: their place among the warp's columns
+      auto put = [&](uint32_t (&acc)[32], int c0, int b) {
+        if constexpr (kMode == kFew) {
+          const int left = static_cast<int>(it.hi - it.lo) - n0;  // rows of the tile, and more
+          const float few_bias =
+              whole && p.bias != nullptr && m0 + lane < p.m_extent ? load_param(p.bias, kParamDtype, int64_t(it.group) * p.m_extent + m0 + lane) : 0.f;
+          T* out = static_cast<T*>(p.out) + int64_t(it.lo + n0) * p.out_ld + m0 + lane;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int r = c0 + i;
+            if (r < p.bn) {
+              if (piece != nullptr) piece[r * 128 + quarter * 32 + lane] = __uint_as_float(acc[i]);
+              else if (r < left && m0 + lane < p.m_extent) store_value(out + int64_t(r) * p.out_ld, __uint_as_float(acc[i]) + few_bias);
+            }
+          }
+        } else if (piece != nullptr) {
+          store_columns<float>(acc, stage, lane, c0, piece + size_t(in_tile) * p.bn, p.bn, 32, p.bn, 1);
+        } else {
+          add_bias(acc, b);
+          store_columns<T>(acc, stage, lane, c0, static_cast<T*>(p.out) + row0 * p.out_ld + n0, p.out_ld, rows, p.n_extent - n0, p.vec_ok);
+        }
+      };
       if constexpr (kBlocks) {
+        uint32_t sum[kSums][32];
+        float db = 0.f;
 #pragma unroll
         for (int b = 0; b < kSums; ++b)
 #pragma unroll
           for (int i = 0; i < 32; ++i) sum[b][i] = 0u;
         for (uint32_t at = it.from; at < it.to; ++at) {
-          tmem = wait_full();
+          const uint32_t tmem = wait_full();
 #pragma unroll
           for (int b = 0; b < kSums; ++b) {
             if (group * 32 + b * 64 < p.bn) {
@@ -587,92 +627,72 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
           }
           give_back();
         }
-      } else {
-        tmem = wait_full();
-        // the first of the unit's blocks whose turn it was, if there is one
-        if (with_db && it.from + (n_tile_of(it) + p.n_tiles - it.from % p.n_tiles) % p.n_tiles < it.to) {
-          uint32_t acc[32];
-          tmem_ld_32x32(tmem + p.bn, acc);
-          tmem_ld_wait();
-          db = __uint_as_float(acc[0]);
-        }
-      }
-      float* piece = whole ? nullptr : p.slab + size_t(it.piece) * p.tile_m * p.bn;
-      const int64_t row0 = kMode == kRows ? int64_t(it.lo) + m0 : int64_t(it.group) * p.m_extent + m0;
-      const int rows = (kMode == kRows ? static_cast<int>(it.hi - it.lo) : p.m_extent) - m0;
-      // bias (kRows): column c of the tile at bias_buf[c / 64 * 32 + c % 32], read ahead of the accumulator
-      auto add_bias = [&](uint32_t (&acc)[32], int c0) {
-        if (kMode != kRows || p.bias == nullptr) return;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 b = reinterpret_cast<const float4*>(bias_buf + c0 / 64 * 32)[i];
-          acc[4 * i] = __float_as_uint(__uint_as_float(acc[4 * i]) + b.x), acc[4 * i + 1] = __float_as_uint(__uint_as_float(acc[4 * i + 1]) + b.y);
-          acc[4 * i + 2] = __float_as_uint(__uint_as_float(acc[4 * i + 2]) + b.z), acc[4 * i + 3] = __float_as_uint(__uint_as_float(acc[4 * i + 3]) + b.w);
-        }
-      };
-      const float few_bias =
-          kMode == kFew && whole && p.bias != nullptr && m0 + lane < p.m_extent ? load_param(p.bias, kParamDtype, int64_t(it.group) * p.m_extent + m0 + lane) : 0.f;
-      auto put = [&](uint32_t (&acc)[32], int c0) {
-        if constexpr (kMode == kFew) {
-          const int left = static_cast<int>(it.hi - it.lo) - n0;  // rows of the tile, and more
-          T* out = static_cast<T*>(p.out) + int64_t(it.lo + n0) * p.out_ld + m0 + lane;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int r = c0 + i;
-            if (r < p.bn) {
-              if (piece != nullptr) piece[r * 128 + quarter * 32 + lane] = __uint_as_float(acc[i]);
-              else if (r < left && m0 + lane < p.m_extent) store_value(out + int64_t(r) * p.out_ld, __uint_as_float(acc[i]) + few_bias);
-            }
-          }
-        } else if (piece != nullptr) {
-          store_columns<float>(acc, stage, lane, c0, piece + size_t(in_tile) * p.bn, p.bn, 32, p.bn, 1);
-        } else if (by_tma) {
-          // the buffer before this one may still be read; 32 rows of 64 bytes in the order that the map's swizzle says
-          uint8_t* to = stage + buffer * 2048;
-          add_bias(acc, c0);
-          if (elect_one()) bulk_wait_read<1>();
-          __syncwarp();
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            float f[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(acc[g * 8 + i]);
-            if constexpr (!kBlocks) *reinterpret_cast<uint4*>(to + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4)) = Channels<T, 8>::pack(f);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (elect_one()) {
-            tma_store_3d(&tmap_o, smem_u32(to), n0 + c0, kMode == kRows ? static_cast<int>(it.lo) + m0 : m0, kMode == kRows ? 0 : static_cast<int>(it.group));
-            bulk_commit();
-          }
-          buffer ^= 1u;
-        } else {
-          add_bias(acc, c0);
-          store_columns<T>(acc, stage, lane, c0, static_cast<T*>(p.out) + row0 * p.out_ld + n0, p.out_ld, rows, p.n_extent - n0, p.vec_ok);
-        }
-      };
-      if (*abort_flag == 0u) {  // else nothing that was waited for is there, and the status word says so
-        if constexpr (kBlocks) {
+        if (*abort_flag == 0u) {  // else nothing that was waited for is there, and the status word says so
 #pragma unroll
           for (int b = 0; b < kSums; ++b)
-            if (group * 32 + b * 64 < p.bn) put(sum[b], group * 32 + b * 64);
-        } else {
-          // the next 32 columns are on their way while these are stored
-          uint32_t acc[2][32];
-          if (group * 32 < p.bn) tmem_ld_32x32(tmem + group * 32, acc[0]);
+            if (group * 32 + b * 64 < p.bn) put(sum[b], group * 32 + b * 64, b);
+          if (with_db) p.db_parts[size_t(it.unit) * p.tile_m + in_tile + lane] = db;
+        }
+      } else {
+        const uint32_t tmem = wait_full();
+        const bool fine = *abort_flag == 0u;
+        // the first of the unit's blocks whose turn it was, if there is one
+        if (with_db) {
+          float db = 0.f;
+          if (it.from + (n_tile_of(it) + p.n_tiles - it.from % p.n_tiles) % p.n_tiles < it.to) {
+            uint32_t acc[32];
+            tmem_ld_32x32(tmem + p.bn, acc);
+            tmem_ld_wait();
+            db = __uint_as_float(acc[0]);
+          }
+          if (fine) p.db_parts[size_t(it.unit) * p.tile_m + in_tile + lane] = db;
+        }
+        // 16-bit results go out by TMA, 64 columns at a time (rows of other matrices are cut off by the map; rows of other groups
+        // by nothing, so all 32 have to be the group's); else, and for pieces, by ordinary stores
+        const bool by_tma = kMode != kFew && whole && p.vec_ok && (kMode == kWeight || rows >= 32);
+        if (kMode != kFew) {  // the buffer may still be read
+          if (elect_one()) bulk_wait_read<0>();
+          __syncwarp();
+        }
 #pragma unroll
-          for (int b = 0; b < (kMode == kFew ? 1 : 4); ++b) {
-            const int c0 = group * 32 + b * 64;
-            if (c0 < p.bn) {
-              tmem_ld_wait();
-              if (kMode != kFew && c0 + 64 < p.bn) tmem_ld_32x32(tmem + c0 + 64, acc[(b + 1) % 2]);
-              put(acc[b % 2], c0);
+        for (int b = 0; b < (kMode == kFew ? 1 : 2); ++b) {
+          const int c0 = group * kOwn + b * 128;
+          if (c0 >= p.bn || !fine) continue;
+          uint32_t acc[2][32];
+          tmem_ld_32x32(tmem + c0, acc[0]);
+          if (kMode != kFew) tmem_ld_32x32(tmem + c0 + 32, acc[1]);  // columns beyond the tile are cut off below
+          tmem_ld_wait();
+          if (by_tma) {
+            // 32 rows of 128 bytes in the order that the map's swizzle says
+            if (b > 0) {
+              if (elect_one()) bulk_wait_read<0>();
+              __syncwarp();
             }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              add_bias(acc[h], b * 2 + h);
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(acc[h][g * 8 + i]);
+                *reinterpret_cast<uint4*>(stage + lane * 128 + (((h * 4 + g) ^ (lane & 7)) << 4)) = Channels<T, 8>::pack(f);
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (elect_one()) {
+              tma_store_3d(&tmap_o, smem_u32(stage), n0 + c0, kMode == kRows ? static_cast<int>(it.lo) + m0 : m0, kMode == kRows ? 0 : static_cast<int>(it.group));
+              bulk_commit();
+            }
+          } else {
+#pragma unroll
+            for (int h = 0; h < (kMode == kFew ? 1 : 2); ++h)
+              if (c0 + h * 32 < p.bn) put(acc[h], c0 + h * 32, b * 2 + h);
           }
         }
-        if (with_db) p.db_parts[size_t(it.unit) * p.tile_m + in_tile + lane] = db;
+        give_back();
       }
-      if constexpr (!kBlocks) give_back();
     }
     // rows of no group (forward and input gradient): zeros
     if constexpr (kMode != kWeight) {
@@ -1047,8 +1067,8 @@ static int grouped_pass(const fgb_grouped_linear_call& c, int pass, const Operan
   }
   if (rc != FGB_OK) return rc;
   a.vec_ok = a.out_ld * eb % 16 == 0;
-  if (a.vec_ok && eb == 2 && p.mode != kFew) {  // what is stored: 32 rows x 32 columns at a time
-    rc = pass == 2 ? make_rows_tmap_3d(&to, a.out, c.dtype, c.ci, c.co, G, 32, 32) : make_rows_tmap_3d(&to, a.out, c.dtype, a.out_ld, N, 1, 32, 32);
+  if (a.vec_ok && eb == 2 && p.mode != kFew) {  // what is stored: 32 rows x 64 columns at a time
+    rc = pass == 2 ? make_rows_tmap_3d(&to, a.out, c.dtype, c.ci, c.co, G, 64, 32) : make_rows_tmap_3d(&to, a.out, c.dtype, a.out_ld, N, 1, 64, 32);
     if (rc != FGB_OK) return rc;
   }
   a.idesc = make_idesc(fmt, a.tile_m, p.bn, a.p_mn, a.q_mn);

@@ -767,8 +767,7 @@ int make_rows_tmap(CUtensorMap* map, const void* rows, int64_t n_rows, int row_e
   });
 }
 
-// 3-D map over 16-bit elements [d2][d1][d0] (d0 a multiple of 8); box = b0 x b1 x 1, swizzled over 128 bytes, or 64 where a
-// row of the box has 64
+// 3-D map over 16-bit elements [d2][d1][d0] (d0 a multiple of 8); box = b0 x b1 x 1, 128B swizzle
 int make_rows_tmap_3d(CUtensorMap* map, const void* base, int dtype16, uint64_t d0, uint64_t d1, uint64_t d2, uint32_t b0, uint32_t b1) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (fn == nullptr) return FGB_E_DRIVER;
@@ -778,8 +777,7 @@ int make_rows_tmap_3d(CUtensorMap* map, const void* base, int dtype16, uint64_t 
   cuuint32_t box[3] = {b0, b1, 1u};
   cuuint32_t estr[3] = {1, 1, 1};
   return encode_tmap([&] {
-    return fn(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              b0 == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+    return fn(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   });
 }
