@@ -5,7 +5,9 @@
 //   dz    = dy act'(z),  dw = sum dz h,  db = sum dz  (all rows),   q = dz w
 //   dx    = r (q - mean(q) - h mean(q h))             (means as above)
 //
-// Three launches a direction, chained:
+// Short samples (at most 512 KB on average): one launch.  A team of threads -- a warp, a CTA, or a cluster of up to eight CTAs --
+// takes a sample: sums, statistics and the apply pass one after the other, the second read out of L1.  The teams keep their
+// own sums of the backward pass for dw and db, which a second launch adds up.  Else three launches a direction, chained:
 //   1. sums: a CTA takes a block of consecutive rows and adds, channel by channel, the rows of each sample that it meets
 //      there.  Forward it keeps mean and squared distance from the mean (not plain squares: a channel whose mean is far
 //      from zero keeps its digits), backward dz and dz h.
@@ -19,6 +21,7 @@
 #include "fgb_common.cuh"
 #include "fgb_device.cuh"
 #include "fgb_rows.cuh"
+#include "fgb_umma.cuh"
 
 namespace fgb {
 
@@ -37,6 +40,7 @@ struct NormArgs {
   RowRanges ranges;
   int C, G, cpg;         // channels, groups, channels per group
   uint32_t R, blocks;    // rows per block
+  uint32_t slots;        // backward: rows of `part` that make dw and db
   const void* w;
   const void* b;
   int param_dtype;
@@ -307,7 +311,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const NormArgs 
   chain_wait();
   if (kBackward && blockIdx.x >= join_ctas) {
     const int c = (blockIdx.x - join_ctas) * 8 + (threadIdx.x & 7), w = threadIdx.x >> 3;
-    const uint32_t slots = p.blocks + p.ranges.count - 1u;
+    const uint32_t slots = p.slots;
     float db = 0.f, dw = 0.f;
     if (c < p.C) {
 #pragma unroll 8
@@ -477,8 +481,292 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_apply_kernel(con
     if (r < begin || r >= end) Ch::store(out + size_t(r) * p.C, zero);
 }
 
+// ------------------------------------------------------------------ short samples
+struct SmallArgs {
+  int team;           // threads of a CTA that take a sample: 32, 64, 128 or 256
+  int cluster;        // CTAs that do (1 where a CTA has several teams)
+  uint32_t teams;     // samples at a time; team t takes the samples t, t + teams, ...
+  F2* columns;        // backward: [CTAs, or clusters][C] sums of dz and dz h
+};
+
+template <typename T, int kVec, bool kOne, bool kBackward, bool kSilu>
+__global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_small_kernel(const NormArgs p, const SmallArgs q) {
+  using Ch = Channels<T, kVec>;
+  using Raw = typename Ch::Raw;
+  using P = Pairs<T, kVec>;
+  constexpr bool kExact = sizeof(T) == 4;
+  constexpr int kPairs = P::kPairs;
+  extern __shared__ F2 s_mem[];  // of each team: sums [C], statistics [G], backward: columns [C]
+  __shared__ F2 s_sum[2 * kPairs][kNormThreads];
+  chain_release();
+  chain_wait();
+  p.ranges.check(p.status, p.mirror);
+  const int size = q.team, t = threadIdx.x % size, here = threadIdx.x / size, teams_here = kNormThreads / size;
+  const uint32_t rank = q.cluster > 1 ? cluster_ctarank() : 0u;
+  const uint32_t team = q.cluster > 1 ? blockIdx.x / q.cluster : blockIdx.x * teams_here + here;
+  F2* sums = s_mem + size_t(here) * ((kBackward ? 2 : 1) * p.C + p.G);
+  F2* stats = sums + p.C;
+  F2* columns = stats + p.G;
+  auto sync = [&]() {
+    if (size == 32) __syncwarp();
+    else if (size == kNormThreads) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(here + 1), "r"(size) : "memory");  // a barrier of the team's own
+  };
+  const int packs = p.C / kVec;
+  const double inv_cpg = 1.0 / p.cpg;
+  const T* x = static_cast<const T*>(p.x);
+  const T* dy = static_cast<const T*>(p.dy);
+  T* out = static_cast<T*>(p.out);
+  if constexpr (kBackward) {
+    for (int c = t; c < p.C; c += size) columns[c] = both(0.f);
+    sync();
+  }
+  for (uint32_t s = team; s < p.ranges.count; s += q.teams) {
+    const uint32_t lo = p.ranges.at(s), hi = max(lo, p.ranges.at(s + 1u)), len = hi - lo;
+    const uint32_t share = (len + q.cluster - 1u) / q.cluster, from = min(hi, lo + rank * share), to = min(hi, from + share);
+    // 1. sums of this CTA's rows, for each channel
+    for (int pack0 = 0; pack0 < packs; pack0 += size) {
+      const int width = min(size, packs - pack0), lanes = size / width;
+      const int cx = t % width, ry = t / width, c0 = (pack0 + cx) * kVec;
+      F2 sum0[kPairs], sum1[kPairs];
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) sum0[i] = sum1[i] = both(0.f);
+      if (ry < lanes && from < to) {
+        const size_t step = size_t(lanes) * p.C;
+        uint32_t r = from + ry;
+        const T* px = x + size_t(r) * p.C + c0;
+        if constexpr (!kBackward) {
+          // distances from the sample's first row, the same for all CTAs
+          P pivot;
+          pivot.unpack(Ch::load(x + size_t(lo) * p.C + c0));
+          auto add = [&](const Raw& raw) {
+            P v;
+            v.unpack(raw);
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) {
+              const F2 d = add2(v.v[i], neg2(pivot.v[i]));
+              sum0[i] = add2(sum0[i], d);
+              sum1[i] = fma2(d, d, sum1[i]);
+            }
+          };
+          constexpr int kRows = 8;
+          for (; r + (kRows - 1u) * lanes < to; r += kRows * lanes, px += kRows * step) {
+            Raw raw[kRows];
+#pragma unroll
+            for (int u = 0; u < kRows; ++u) raw[u] = Ch::load(px + u * step);
+#pragma unroll
+            for (int u = 0; u < kRows; ++u) add(raw[u]);
+          }
+#pragma unroll 4
+          for (; r < to; r += lanes, px += step) add(Ch::load(px));
+        } else {
+          ChannelParams<kVec, kOne> k;
+          k.load(p, c0);
+          k.load_stats(p, s, c0);
+          const T* pg = dy + size_t(r) * p.C + c0;
+          auto add = [&](const Raw& raw, const Raw& raw_dy) {
+            P v, g;
+            v.unpack(raw);
+            g.unpack(raw_dy);
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) {
+              const F2 h = k.h(v.v[i], i);
+              const F2 dz = activate_grad<kExact, kSilu>(g.v[i], k.z(h, i));
+              sum0[i] = add2(sum0[i], dz);
+              sum1[i] = fma2(dz, h, sum1[i]);
+            }
+          };
+          constexpr int kRows = 4;
+          for (; r + (kRows - 1u) * lanes < to; r += kRows * lanes, px += kRows * step, pg += kRows * step) {
+            Raw raw[kRows], raw_dy[kRows];
+#pragma unroll
+            for (int u = 0; u < kRows; ++u) raw[u] = Ch::load(px + u * step), raw_dy[u] = Ch::load(pg + u * step);
+#pragma unroll
+            for (int u = 0; u < kRows; ++u) add(raw[u], raw_dy[u]);
+          }
+#pragma unroll 2
+          for (; r < to; r += lanes, px += step, pg += step) add(Ch::load(px), Ch::load(pg));
+        }
+      }
+      for (int m = lanes; m > 1;) {
+        const int half = (m + 1) / 2;
+        if (ry >= half && ry < m) {
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) s_sum[i][threadIdx.x] = sum0[i], s_sum[kPairs + i][threadIdx.x] = sum1[i];
+        }
+        sync();
+        if (ry < m - half) {
+          const int at = threadIdx.x + half * width;
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) sum0[i] = add2(sum0[i], s_sum[i][at]), sum1[i] = add2(sum1[i], s_sum[kPairs + i][at]);
+        }
+        sync();
+        m = half;
+      }
+      if (ry == 0) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+          sums[c0 + i] = F2{i % 2 ? sum0[i / 2].y : sum0[i / 2].x, i % 2 ? sum1[i / 2].y : sum1[i / 2].x};
+      }
+    }
+    sync();
+    if (q.cluster > 1) cluster_sync_all();
+    // 2. the groups: a thread adds up a group, over the channels and the CTAs
+    auto total = [&](int c) {
+      F2 v = sums[c];
+      if (q.cluster > 1) {
+        v = both(0.f);
+        for (int i = 0; i < q.cluster; ++i) {
+          float2 w;
+          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(w.x), "=f"(w.y) : "r"(cluster_map(smem_u32(&sums[c]), i)) : "memory");
+          v = add2(v, F2{w.x, w.y});
+        }
+      }
+      return v;
+    };
+    // lanes that share a group: as many as it has channels, up to a warp's
+    int across = 1;
+    while (across < 32 && across < p.cpg) across *= 2;
+    for (int g0 = t / across; g0 < (p.G + size / across - 1) / (size / across) * (size / across); g0 += size / across) {  // whole warps
+      const bool has = g0 < p.G && len > 0u;
+      const int g = min(g0, p.G - 1);
+      double v0 = 0, v1 = 0;
+      if constexpr (!kBackward) {
+        // as the joins of the longer way: the first channel's mean is the pivot of the channels' means
+        const double inv_n = 1.0 / len;
+        const double pivot = has ? static_cast<double>(static_cast<float>(x[size_t(lo) * p.C + g * p.cpg])) : 0.0;
+        for (int i = t % across; i < p.cpg && has; i += across) {
+          const int c = g * p.cpg + i;
+          const F2 v = total(c);
+          const double mean = static_cast<double>(v.x) * inv_n, within = static_cast<double>(v.y) - v.x * mean;
+          const double d = static_cast<double>(static_cast<float>(x[size_t(lo) * p.C + c])) + mean - pivot;
+          v0 += d;
+          v1 += (within < 0 ? 0.0 : within) * inv_n + d * d;  // a NaN stays
+        }
+        for (int d = across / 2; d > 0; d >>= 1) v0 += __shfl_xor_sync(0xffffffffu, v0, d), v1 += __shfl_xor_sync(0xffffffffu, v1, d);
+        v0 *= inv_cpg, v1 *= inv_cpg;
+        const double var = v1 - v0 * v0 < 0 || !has ? 0.0 : v1 - v0 * v0;
+        if (t % across == 0 && g0 < p.G) {
+          const F2 st{has ? static_cast<float>(pivot + v0) : 0.f, 1.f / sqrtf(static_cast<float>(var + static_cast<double>(p.eps)))};
+          stats[g] = st;
+          if (rank == 0u) p.mean[size_t(s) * p.G + g] = st.x, p.rstd[size_t(s) * p.G + g] = st.y;
+        }
+      } else {
+        for (int i = t % across; i < p.cpg && has; i += across) {
+          const int c = g * p.cpg + i;
+          const F2 v = total(c);
+          const double w = p.w != nullptr ? load_param(p.w, p.param_dtype, c) : 1.f;
+          v0 += w * v.x;
+          v1 += w * v.y;
+          if (rank == 0u) columns[c] = add2(columns[c], v);
+        }
+        for (int d = across / 2; d > 0; d >>= 1) v0 += __shfl_xor_sync(0xffffffffu, v0, d), v1 += __shfl_xor_sync(0xffffffffu, v1, d);
+        const double inv_n = inv_cpg / len;
+        if (t % across == 0 && g0 < p.G) stats[g] = F2{static_cast<float>(v0 * inv_n), static_cast<float>(v1 * inv_n)};
+      }
+    }
+    sync();
+    if (q.cluster > 1) cluster_sync_all();  // the other CTAs have read this one's sums
+    // 3. apply
+    if (from < to && out != nullptr) {
+      for (int pack0 = 0; pack0 < packs; pack0 += size) {
+        const int width = min(size, packs - pack0), lanes = size / width;
+        const int cx = t % width, ry = t / width, c0 = (pack0 + cx) * kVec;
+        if (ry >= lanes) continue;
+        constexpr int kStats = ChannelParams<kVec, kOne>::kStats;
+        ChannelParams<kVec, kOne> k;
+        k.load(p, c0);
+        auto group_of = [&](int c) { return stats[(c0 + c) / p.cpg]; };
+        F2 minus_m1[kStats], m2[kStats];
+        if constexpr (kBackward) {
+          k.load_stats(p, s, c0);
+#pragma unroll
+          for (int i = 0; i < kStats; ++i) {
+            const F2 a = group_of(2 * i), b = kOne || kVec == 1 ? a : group_of(2 * i + 1);
+            minus_m1[i] = F2{-a.x, -b.x}, m2[i] = F2{a.y, b.y};
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kStats; ++i) {
+            const F2 a = group_of(2 * i), b = kOne || kVec == 1 ? a : group_of(2 * i + 1);
+            k.minus_mean[i] = F2{-a.x, -b.x}, k.r[i] = F2{a.y, b.y};
+          }
+        }
+        auto one = [&](const Raw& raw, const Raw& raw_dy) {
+          P v;
+          v.unpack(raw);
+          if constexpr (!kBackward) {
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) v.v[i] = activate<kExact, kSilu>(k.z(k.h(v.v[i], i), i));
+          } else {
+            P g;
+            g.unpack(raw_dy);
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) {
+              const F2 h = k.h(v.v[i], i), dz = activate_grad<kExact, kSilu>(g.v[i], k.z(h, i));
+              const F2 w = F2{__fmul_rn(dz.x, k.w[i].x), __fmul_rn(dz.y, k.w[i].y)};  // as in norm_apply_kernel
+              const int j = kOne ? 0 : i;
+              v.v[i] = mul2(k.r[j], fma2(neg2(h), m2[j], add2(w, minus_m1[j])));
+            }
+          }
+          return v.pack();
+        };
+        const size_t step = size_t(lanes) * p.C;
+        uint32_t r = from + ry;
+        size_t at = size_t(r) * p.C + c0;
+        constexpr int kRows = 4;
+        for (; r + (kRows - 1u) * lanes < to; r += kRows * lanes, at += kRows * step) {
+          Raw raw[kRows], raw_dy[kRows];
+#pragma unroll
+          for (int u = 0; u < kRows; ++u) {
+            raw[u] = Ch::load(x + at + u * step);
+            if (kBackward) raw_dy[u] = Ch::load(dy + at + u * step);
+          }
+#pragma unroll
+          for (int u = 0; u < kRows; ++u) Ch::store(out + at + u * step, one(raw[u], raw_dy[u]));
+        }
+        for (; r < to; r += lanes, at += step) {
+          const Raw raw = Ch::load(x + at);
+          Ch::store(out + at, one(raw, kBackward ? Ch::load(dy + at) : raw));
+        }
+      }
+    }
+    sync();  // sums and statistics are written again
+  }
+  if constexpr (kBackward) {
+    __syncthreads();
+    if (rank == 0u && q.columns != nullptr) {
+      // the CTA's teams in order
+      F2* to = q.columns + size_t(blockIdx.x / q.cluster) * p.C;
+      for (int c = threadIdx.x; c < p.C; c += kNormThreads) {
+        F2 v = both(0.f);
+        for (int i = 0; i < teams_here; ++i) v = add2(v, s_mem[size_t(i) * (2 * p.C + p.G) + p.C + p.G + c]);
+        to[c] = v;
+      }
+    }
+  }
+  // rows of no sample
+  if (out != nullptr) {
+    const uint32_t begin = p.ranges.at(0u), end = max(begin, p.ranges.at(p.ranges.count)), outside = begin + (p.ranges.n - end);
+    Raw zero{};
+    for (uint64_t i = uint64_t(blockIdx.x) * kNormThreads + threadIdx.x; i < uint64_t(outside) * packs; i += uint64_t(gridDim.x) * kNormThreads) {
+      const uint32_t r = static_cast<uint32_t>(i / packs), row = r < begin ? r : r - begin + end;
+      Ch::store(out + size_t(row) * p.C + (i - uint64_t(r) * packs) * kVec, zero);
+    }
+  }
+}
+
 // ------------------------------------------------------------------ host side
+// A sample on average up to this size goes the short way (all three passes in one launch): what eight CTAs hold in L1 between
+// the passes, with half of it to spare.
+constexpr int64_t kSmallBytes = 512 * 1024;
+constexpr int kSmallChannels = 2048;
+
 struct NormPlan {
+  bool small;         // the short way:
+  int team, cluster;  // threads of a CTA, and CTAs, for a sample
+  unsigned grid;
+  size_t small_smem;
   int vec;
   bool one;           // a pack lies in one group
   unsigned columns;   // CTAs along a row
@@ -491,6 +779,20 @@ static NormPlan norm_plan(const fgb_group_norm_call& c) {
   if (p.vec == 8 && c.c / c.groups % 8 != 0) p.vec = 4;  // eight channels of several groups would take too many registers
   p.one = c.c / c.groups % p.vec == 0;
   const int packs = c.c / p.vec;
+  const int64_t sms = device_sm_count(), mean_rows = c.n / c.samples, mean_bytes = mean_rows * c.c * elem_bytes(c.dtype);
+  p.small = mean_bytes <= kSmallBytes && c.c <= kSmallChannels;
+  // Eight packs a thread: that many loads are on their way at a time, and a sample's chain of steps takes the same few
+  // microseconds however many threads go through it, so small teams are more samples at a time.
+  p.team = 32;
+  auto team_smem = [&](int team) { return (kNormThreads / team) * (2 * size_t(c.c) + c.groups) * 8; };
+  while (p.team < kNormThreads && (mean_rows * packs > 8 * p.team || team_smem(p.team) > 48 * 1024 || p.team * c.samples * 2 <= 32 * sms)) p.team *= 2;
+  p.cluster = 1;
+  // 16 KB a CTA, or as many CTAs as there are SMs for each sample
+  while (p.small && p.team == kNormThreads && p.cluster < 8 && (int64_t(p.cluster) * 16384 < mean_bytes || p.cluster * c.samples * 2 <= sms)) p.cluster *= 2;
+  if (p.cluster > 1 && mean_bytes / p.cluster < 2048) p.cluster = 1;
+  const int64_t ctas = ceil_div(c.samples, kNormThreads / p.team);
+  p.grid = static_cast<unsigned>(std::min<int64_t>(ctas, std::max<int64_t>(sms * kNormCtas / p.cluster, 1)) * p.cluster);
+  p.small_smem = team_smem(p.team);
   p.columns = static_cast<unsigned>(ceil_div(packs, kNormThreads));
   const int width = packs < kNormThreads ? packs : kNormThreads, lanes = kNormThreads / width;
   // as many CTAs as run at a time, each thread at least eight rows
@@ -498,7 +800,7 @@ static NormPlan norm_plan(const fgb_group_norm_call& c) {
   const int64_t R = std::max<int64_t>(ceil_div(c.n, want), int64_t(lanes) * 8);
   p.R = static_cast<uint32_t>(R);
   p.blocks = static_cast<uint32_t>(std::max<int64_t>(ceil_div(c.n, R), 1));
-  p.joined_off = align256((int64_t(p.blocks) + c.samples - 1) * 2 * c.c * 4);
+  p.joined_off = p.small ? align256(int64_t(p.grid / p.cluster) * c.c * 8) : align256((int64_t(p.blocks) + c.samples - 1) * 2 * c.c * 4);
   p.bytes = p.joined_off + align256(c.samples * c.groups * 8);
   return p;
 }
@@ -519,6 +821,20 @@ template <typename T, int kVec, bool kOne, bool kSilu>
 static int norm_run_act(const NormArgs& a, const NormPlan& p, bool backward, bool want_out, bool want_param, cudaStream_t s) {
   const dim3 grid(p.blocks, p.columns);
   LaunchErrors chain;
+  if (p.small) {
+    const SmallArgs q{p.team, p.cluster, p.grid / p.cluster * (kNormThreads / p.team), want_param ? a.part : nullptr};
+    auto kernel = backward ? norm_small_kernel<T, kVec, kOne, true, kSilu> : norm_small_kernel<T, kVec, kOne, false, kSilu>;
+    static PerDeviceTable configured[2];
+    const int rc = ensure_dynamic_smem(configured[backward], kernel, p.small_smem);
+    if (rc != FGB_OK) return rc;
+    chain.add(launch_chained_clusters(kernel, dim3(p.grid), dim3(kNormThreads), p.small_smem, p.cluster, s, a, q));
+    if (want_param) {
+      NormArgs cols = a;
+      cols.slots = p.grid / p.cluster;
+      chain.add(launch_chained(norm_join_kernel<32, true>, dim3(static_cast<unsigned>(ceil_div(a.C, 8))), dim3(kNormThreads), 0, s, cols, 0u));
+    }
+    return chain.first != cudaSuccess ? cuda_status(chain.first) : launch_status();
+  }
   const int64_t units = int64_t(a.ranges.count) * a.G;
   // a CTA a (sample, group) where the samples cover many blocks, a warp where they are short
   const bool warps = int64_t(p.blocks) * a.cpg / a.ranges.count < 64;
@@ -557,7 +873,7 @@ static int norm_call(const fgb_group_norm_call* c, bool backward, cudaStream_t s
   a.x = c->x, a.dy = c->grad_out, a.out = c->out;
   a.ranges = RowRanges{c->offsets_bits ? c->offsets : nullptr, c->offsets_bits == 64, static_cast<uint32_t>(c->n), static_cast<uint32_t>(c->samples)};
   a.C = c->c, a.G = c->groups, a.cpg = c->c / c->groups;
-  a.R = p.R, a.blocks = p.blocks;
+  a.R = p.R, a.blocks = p.blocks, a.slots = p.blocks + static_cast<uint32_t>(c->samples) - 1u;
   a.w = c->weight, a.b = c->bias, a.param_dtype = c->param_dtype, a.act = c->act, a.eps = c->eps;
   a.mean = c->mean, a.rstd = c->rstd;
   a.part = static_cast<F2*>(c->workspace);

@@ -79,6 +79,13 @@ CASES = [
     ([30, 30], 1028, 4, 2),
     ([6000], 36, 9, 0),
     ([3000, 5000], 512, 32, 0),
+    # samples too long for one launch
+    ([20000, 0, 3], 36, 9, 50),
+    ([12000, 5000], 100, 5, 7),
+    ([40000], 16, 16, 0),
+    ([900], 2056, 8, 0),
+    ([30000, 1], 33, 3, 1),
+    ([70000], 6, 1, 0),
 ]
 
 
