@@ -31,7 +31,7 @@ Printed JSON (one line, rank 0): the metric and, beside it,
   local gradient recomputed on rank 0).
 
 --impl reference times the CPU algorithm alone, with all host threads.
---workload res1024_batch8 | res1024_map [--unsorted] | residual_stack [--fused] | pipeline_microbench
+--workload res1024_batch8 | res1024_map [--unsorted] | residual_stack [--fused | --norm] | pipeline_microbench
 run one of the side workloads alone (what the ncu captures under profiles/ use).
 --quick skips the side workloads of the default run.
 """
@@ -340,13 +340,16 @@ def sweep_report(dev, peaks, iters: int = 8):
             "tf32_peak": "half of the measured bf16 peak", "points": points}
 
 
-def residual_stack_steps(dev, fused: bool, steps: int, warmup: int = 3):
+def residual_stack_steps(dev, fused: bool, steps: int, warmup: int = 3, norm: bool = False):
     """Residual stack: 8 blocks [conv, SiLU, conv] + skip on 4 shells at RES=64,
     C=512, bf16, one shared neighbour cache, forward + backward of the mean.
-    ``fused``: SiLU and the skip addition run in the conv kernels' epilogue."""
+    ``fused``: SiLU and the skip addition run in the conv kernels' epilogue.
+    ``norm``: the blocks are [group norm + SiLU, conv] twice + skip (32 groups,
+    ``sparse_group_norm``) instead."""
     from flexgemm_b200 import workloads
     from flexgemm_b200.kernels import cuda as K
-    from flexgemm_b200.ops import spconv
+    from flexgemm_b200.ops import spconv, utils
+    from flexgemm_b200.ops.group_norm import sparse_group_norm
     from flexgemm_b200.ops.spconv import SubMConv3dFunction as F
     B, res, C, blocks = 4, 64, 512, 8
     dt = torch.bfloat16
@@ -358,11 +361,20 @@ def residual_stack_steps(dev, fused: bool, steps: int, warmup: int = 3):
     bs = [torch.zeros(C, dtype=dt, device=dev).requires_grad_(True) for _ in range(2 * blocks)]
     cache = F._compute_neighbor_cache(coords, shape, (3, 3, 3), (1, 1, 1), True)
     pairs = int(cache["valid_signal_i"].shape[0])
+    offsets = utils.sample_offsets(coords, B)
+    scales = [torch.ones(C, dtype=dt, device=dev).requires_grad_(True) for _ in range(2 * blocks)] if norm else []
+    shifts = [torch.zeros(C, dtype=dt, device=dev).requires_grad_(True) for _ in range(2 * blocks)] if norm else []
 
     def step():
         h = x0.detach().requires_grad_(True)
         for i in range(blocks):
-            if fused:
+            if norm:
+                y = h
+                for k in (2 * i, 2 * i + 1):
+                    y = sparse_group_norm(y, offsets, 32, scales[k], shifts[k], activation="silu")
+                    y, _ = spconv.sparse_submanifold_conv3d(y, coords, shape, ws[k], bs[k], neighbor_cache=cache)
+                h = h + y
+            elif fused:
                 y, _ = spconv.sparse_submanifold_conv3d_fused(h, coords, shape, ws[2 * i], bs[2 * i], neighbor_cache=cache, activation="silu")
                 h, _ = spconv.sparse_submanifold_conv3d_fused(y, coords, shape, ws[2 * i + 1], bs[2 * i + 1], neighbor_cache=cache, residual=h)
             else:
@@ -371,7 +383,7 @@ def residual_stack_steps(dev, fused: bool, steps: int, warmup: int = 3):
                 y, _ = spconv.sparse_submanifold_conv3d(y, coords, shape, ws[2 * i + 1], bs[2 * i + 1], neighbor_cache=cache)
                 h = h + y
         h.float().mean().backward()
-        for t in ws + bs:
+        for t in ws + bs + scales + shifts:
             t.grad = None
 
     for _ in range(warmup):
@@ -907,15 +919,16 @@ def run_residual_stack(args):
     peaks = load_peaks()
     spconv.set_algorithm(spconv.Algorithm.MASKED_IMPLICIT_GEMM_SPLITK)
     sampler = ClockSampler(dev.index).start()
-    r = residual_stack_steps(dev, args.fused, args.steps, max(args.warmup, 3))
+    r = residual_stack_steps(dev, args.fused, args.steps, max(args.warmup, 3), args.norm)
     clocks = sampler.stop()
     peak = float(peaks["bf16_tflops"])
     emit({
         "metric": "residual stack fwd+bwd useful TFLOP/s (16 submconvs, C=512 bf16, 4 x RES=64)", "value": r["tflops"], "unit": "TFLOP/s",
         "n_gpus": 1, "steps": args.steps, "warmup": max(args.warmup, 3), "ms_per_step": r["ms"], "higher_is_better": True,
         "scaling": "weak", "vs_baseline": None, "dtype": "bf16", "data": "synthetic",
-        "config": {"workload": f"8 x ([conv, SiLU, conv] + skip), N={r['n_voxels']} voxels, L={r['pairs']} pairs per conv, shared cache; "
-                               f"elementwise work {'in the conv epilogues' if args.fused else 'as torch kernels'}",
+        "config": {"workload": f"8 x ({'[group norm + SiLU, conv] x 2' if args.norm else '[conv, SiLU, conv]'} + skip), N={r['n_voxels']} voxels, "
+                               f"L={r['pairs']} pairs per conv, shared cache; "
+                               f"elementwise work {'in the conv epilogues' if args.fused else 'in the group norms' if args.norm else 'as torch kernels'}",
                    "l2": "activations of one layer (41 MB) fit the 126 MB L2; no flush: the stack streams 16 layers of them"},
         "roofline": {"bound": "tensor", "achieved": r["tflops"], "peak": peak, "unit": "TFLOP/s", "frac": r["tflops"] / peak, "traffic": None,
                      "algorithmic_flops_per_step": r["flops_per_step"], "peak_source": peaks["source"]},
@@ -999,6 +1012,7 @@ def main():
                          "with SiLU and skip additions between them; pipeline_microbench: operand streams and MMAs of one fprop stage per SM")
     ap.add_argument("--unsorted", action="store_true", help="res1024_map: shuffle the rows (hash-table path)")
     ap.add_argument("--fused", action="store_true", help="residual_stack: SiLU and skip additions in the conv epilogues")
+    ap.add_argument("--norm", action="store_true", help="residual_stack: blocks of [group norm + SiLU, conv] twice + skip")
     args = ap.parse_args()
     claim_stdout()
     if args.impl == "reference":
