@@ -801,7 +801,8 @@ static NormPlan norm_plan(const fgb_group_norm_call& c) {
   p.R = static_cast<uint32_t>(R);
   p.blocks = static_cast<uint32_t>(std::max<int64_t>(ceil_div(c.n, R), 1));
   p.joined_off = p.small ? align256(int64_t(p.grid / p.cluster) * c.c * 8) : align256((int64_t(p.blocks) + c.samples - 1) * 2 * c.c * 4);
-  p.bytes = p.joined_off + align256(c.samples * c.groups * 8);
+  // one launch forward needs nothing between its passes
+  p.bytes = p.small ? (c.grad_out != nullptr ? p.joined_off : 0) : p.joined_off + align256(c.samples * c.groups * 8);
   return p;
 }
 
@@ -863,11 +864,12 @@ static int norm_call(const fgb_group_norm_call* c, bool backward, cudaStream_t s
   if (rc != FGB_OK) return rc;
   if (c->offsets_bits != 0 && !c->offsets) return FGB_E_NULL;
   const bool want_param = backward && (c->grad_weight != nullptr || c->grad_bias != nullptr);
-  if (!c->mean || !c->rstd || !c->workspace) return FGB_E_NULL;
+  if (!c->mean || !c->rstd) return FGB_E_NULL;
   if (c->n > 0 && (!c->x || (backward ? !c->grad_out : !c->out))) return FGB_E_NULL;
   if ((reinterpret_cast<uintptr_t>(c->x) | reinterpret_cast<uintptr_t>(c->grad_out) | reinterpret_cast<uintptr_t>(c->out)) & 15) return FGB_E_ALIGN;
   if (reinterpret_cast<uintptr_t>(c->workspace) & 255) return FGB_E_ALIGN;
   const NormPlan p = norm_plan(*c);
+  if (p.bytes > 0 && !c->workspace) return FGB_E_NULL;
   if (c->workspace_bytes < static_cast<int64_t>(p.bytes)) return FGB_E_WORKSPACE;
   NormArgs a{};
   a.x = c->x, a.dy = c->grad_out, a.out = c->out;

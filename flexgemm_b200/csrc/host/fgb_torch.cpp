@@ -1188,14 +1188,14 @@ struct NormShape {
   int act = 0;
   float eps = 0.f;
 };
-fgb_group_norm_call norm_call(const Tensor& x, const Tensor& offsets, const Tensor& weight, const Tensor& bias, const Tensor& mean, const Tensor& rstd,
+fgb_group_norm_call norm_call(const Tensor& x, const Tensor& offsets, const Tensor& weight, const Tensor& bias, const Tensor& stats /* mean, rstd */,
                               const NormShape& k, DeviceState& ds) {
   fgb_group_norm_call c{};
   c.x = ptr(x);
   c.offsets = offsets.defined() ? offsets.const_data_ptr() : nullptr;
   c.offsets_bits = !offsets.defined() ? 0 : offsets.scalar_type() == at::kLong ? 64 : 32;
   c.weight = weight.defined() ? ptr(weight) : nullptr, c.bias = bias.defined() ? ptr(bias) : nullptr;
-  c.mean = static_cast<float*>(mean.data_ptr()), c.rstd = static_cast<float*>(rstd.data_ptr());
+  c.mean = static_cast<float*>(stats.data_ptr()), c.rstd = c.mean + k.samples * k.groups;
   c.n = k.n, c.samples = k.samples;
   c.c = static_cast<int32_t>(x.size(-1)), c.groups = static_cast<int32_t>(k.groups);
   c.dtype = dtype_code(x.scalar_type(), false);
@@ -1206,17 +1206,17 @@ fgb_group_norm_call norm_call(const Tensor& x, const Tensor& offsets, const Tens
 }
 
 struct GroupNormBackward : public torch::autograd::Node {
-  torch::autograd::SavedVariable x_, weight_, bias_, offsets_, mean_, rstd_;
+  torch::autograd::SavedVariable x_, weight_, bias_, offsets_, stats_;
   NormShape shape;
   std::string name() const override { return "SparseGroupNormBackward"; }
   void release_variables() override {
-    for (auto* v : {&x_, &weight_, &bias_, &offsets_, &mean_, &rstd_}) v->reset_data();
+    for (auto* v : {&x_, &weight_, &bias_, &offsets_, &stats_}) v->reset_data();
   }
   variable_list apply(variable_list&& grads) override {
     variable_list out(3);
     if (!grads[0].defined()) return out;
     const Tensor x = x_.unpack(), weight = weight_.unpack(), bias = bias_.unpack(), offsets = offsets_.unpack();
-    const Tensor mean = mean_.unpack(), rstd = rstd_.unpack();
+    const Tensor stats = stats_.unpack();
     const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1) && weight.defined(),
                need_b = task_should_compute_output(2) && bias.defined();
     {
@@ -1226,7 +1226,7 @@ struct GroupNormBackward : public torch::autograd::Node {
       DeviceState& ds = device_state(x.device().index());
       poll(ds, stream);
       const Tensor g = grad_rows(grads[0], x.scalar_type());
-      fgb_group_norm_call c = norm_call(x, offsets, weight, bias, mean, rstd, shape, ds);
+      fgb_group_norm_call c = norm_call(x, offsets, weight, bias, stats, shape, ds);
       c.grad_out = ptr(g);
       if (need_x) out[0] = new_tensor(x.sizes(), x.scalar_type(), x.device()), c.out = out[0].data_ptr();
       if (need_w) out[1] = new_tensor(weight.sizes(), weight.scalar_type(), x.device()), c.grad_weight = out[1].data_ptr();
@@ -1271,16 +1271,16 @@ PyObject* py_group_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const auto stream = c10::cuda::getCurrentCUDAStream(x.device().index());
   DeviceState& ds = device_state(x.device().index());
   poll(ds, stream);
-  Tensor out, mean, rstd;
+  Tensor out, stats;
   {
     at::AutoDispatchBelowADInplaceOrView below;
     out = new_tensor(x.sizes(), x.scalar_type(), x.device());
-    mean = new_tensor({k.samples, k.groups}, at::kFloat, x.device());
-    rstd = new_tensor({k.samples, k.groups}, at::kFloat, x.device());
-    fgb_group_norm_call c = norm_call(x, offsets, weight, bias, mean, rstd, k, ds);
+    stats = new_tensor({2, k.samples, k.groups}, at::kFloat, x.device());
+    fgb_group_norm_call c = norm_call(x, offsets, weight, bias, stats, k, ds);
     c.out = out.data_ptr();
     c.workspace_bytes = check_bytes(api.fgb_group_norm_workspace_bytes(&c), "fgb_group_norm_workspace_bytes");
-    const c10::DataPtr ws = scratch(c.workspace_bytes);
+    c10::DataPtr ws;
+    if (c.workspace_bytes > 0) ws = scratch(c.workspace_bytes);
     c.workspace = ws.get();
     check(api.fgb_group_norm_forward(&c, stream), "fgb_group_norm_forward");
   }
@@ -1292,7 +1292,7 @@ PyObject* py_group_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (weight.defined()) node->weight_ = SavedVariable(weight, false);
     if (bias.defined()) node->bias_ = SavedVariable(bias, false);
     if (offsets.defined()) node->offsets_ = SavedVariable(offsets, false);
-    node->mean_ = SavedVariable(mean, false), node->rstd_ = SavedVariable(rstd, false);
+    node->stats_ = SavedVariable(stats, false);
     node->shape = k;
     torch::autograd::set_history(out, node);
   }

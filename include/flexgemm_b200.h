@@ -753,10 +753,11 @@ typedef struct fgb_group_norm_call {
   int32_t param_dtype;    /* of weight, bias and their gradients: dtype, or FGB_F32_IEEE */
   int32_t act;            /* FGB_ACT_* */
   float eps;
-  void* workspace;
+  void* workspace;        /* may be null where the query below says 0 bytes */
   int64_t workspace_bytes;
   int32_t* status;
 } fgb_group_norm_call;
+/* of the backward call where grad_out is set, else of the forward one */
 int64_t fgb_group_norm_workspace_bytes(const fgb_group_norm_call* call);
 int fgb_group_norm_forward(const fgb_group_norm_call* call, void* stream);
 int fgb_group_norm_backward(const fgb_group_norm_call* call, void* stream);

@@ -122,12 +122,15 @@ def test_group_norm_entry_points_refuse(lib):
     def rc(fn=lib.fgb_group_norm_forward, **kw):
         call = NormCall(**{**good, **kw})
         return fn(ctypes.byref(call), None)
-    assert lib.fgb_group_norm_workspace_bytes(ctypes.byref(NormCall(**good))) > 0
+    assert lib.fgb_group_norm_workspace_bytes(ctypes.byref(NormCall(**{**good, "n": 100000, "samples": 1}))) > 0
+    assert lib.fgb_group_norm_workspace_bytes(ctypes.byref(NormCall(**good))) == 0   # one launch: nothing between its passes
+    assert lib.fgb_group_norm_workspace_bytes(ctypes.byref(NormCall(**{**good, "grad_out": 1 << 25}))) > 0
     assert lib.fgb_group_norm_workspace_bytes(None) == -1 and lib.fgb_group_norm_forward(None, None) == -1
     for kw, code in ((dict(dtype=9), -3), (dict(param_dtype=_cabi.BF16), -3), (dict(act=7), -3), (dict(offsets_bits=16), -3), (dict(n=-1), -2),
                      (dict(n=1 << 31), -2), (dict(samples=0), -2), (dict(samples=1 << 24), -2), (dict(groups=7), -2), (dict(c=0), -2),
                      (dict(offsets_bits=0), -2), (dict(samples=(1 << 24) - 1, c=65536, groups=65536), -2), (dict(offsets=None), -1), (dict(x=None), -1), (dict(out=None), -1),
-                     (dict(mean=None), -1), (dict(workspace=None), -1), (dict(x=(1 << 20) + 8), -4), (dict(workspace=(1 << 24) + 16), -4), (dict(workspace_bytes=10), -5)):
+                     (dict(mean=None), -1), (dict(workspace=None, n=100000, samples=1), -1), (dict(x=(1 << 20) + 8), -4), (dict(workspace=(1 << 24) + 16), -4),
+                     (dict(workspace_bytes=10, n=100000, samples=1), -5)):
         assert rc(**kw) == code, kw
     assert rc(lib.fgb_group_norm_backward) == -1   # no grad_out
 
