@@ -136,6 +136,7 @@ struct Channels {
     return raw;
   }
   static __device__ __forceinline__ void store(T* p, const Raw& raw) { *reinterpret_cast<Raw*>(p) = raw; }
+  static __device__ __forceinline__ void store_streaming(T* p, const Raw& raw) { __stcs(reinterpret_cast<Raw*>(p), raw); }
 };
 
 // the widest pack that divides a row of C channels: 16 bytes, else 8 or 4, else one channel
