@@ -253,11 +253,6 @@ struct GroupedWalk {
   }
 };
 
-// A value that all lanes of the warp have, in a form that tells the compiler so: TMA and MMA instructions take their operands
-// from registers that are uniform over the warp, and the loops around them have to be uniform for such registers to be used.
-// The loads' and the products' loop took 860 cycles a stage of a 512-cycle product without it.
-__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
-
 template <typename T>
 __device__ __forceinline__ void store_value(T* p, float v) {
   if constexpr (std::is_same<T, float>::value) *p = v;
@@ -374,18 +369,18 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
   // the bias gradient's products: of a block of k in one of the tiles that read the same rows of dy, in turn
   auto ones_in = [&](const GroupedItem& t, uint32_t kb) { return kMode == kWeight && p.db != nullptr && kb % p.n_tiles == n_tile_of(t); };
 
-  const uint32_t stage0 = uniform(smem_u32(stages));
+  const uint32_t stage0 = smem_u32(stages);
   if (warp == 8) {
     // ------------------------------------------------------------------ loads
     uint32_t s = 0, ph = 0;
     const int G = static_cast<int>(p.ranges.count);
-    const uint32_t full_own = uniform(smem_u32(&ctl->full[0])), full_leader = kPair ? uniform(cluster_map(full_own, 0)) : full_own;
-    while (__any_sync(0xffffffffu, walk.next(it))) {
+    const uint32_t full_own = smem_u32(&ctl->full[0]), full_leader = kPair ? cluster_map(full_own, 0) : full_own;
+    while (walk.next(it)) {
       // first row (or channel) of the tile along m and n, first k
-      const int m0 = static_cast<int>(uniform(m_tile_of(it) * p.tile_m + rank * 128u)), n0 = static_cast<int>(uniform(n_tile_of(it) * p.bn + rank * half));
-      const int lo = static_cast<int>(uniform(it.lo)), g = static_cast<int>(uniform(it.group)), len = static_cast<int>(uniform(it.hi - it.lo));
-      const int k_end = static_cast<int>(uniform(it.to * 64u));
-      for (int k0 = static_cast<int>(uniform(it.from * 64u)); k0 < k_end; k0 += 64) {
+      const int m0 = static_cast<int>(m_tile_of(it) * p.tile_m + rank * 128u), n0 = static_cast<int>(n_tile_of(it) * p.bn + rank * half);
+      const int lo = static_cast<int>(it.lo), g = static_cast<int>(it.group), len = static_cast<int>(it.hi - it.lo);
+      const int k_end = static_cast<int>(it.to * 64u);
+      for (int k0 = static_cast<int>(it.from * 64u); k0 < k_end; k0 += 64) {
         const bool cleared = kMode == kWeight && k0 + 64 > len && (len & 15) != 0;  // see the products
         wait(&ctl->empty[s], ph ^ 1);
         if (elect_one()) {
@@ -427,14 +422,14 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
   } else if (warp == 9) {
     // ------------------------------------------------------------------ products
     uint32_t s = 0, ph = 0, set = 0, set_ph = 0;
-    const bool leader = uniform(rank) == 0u;
+    const bool leader = rank == 0u;
     const uint64_t p_step = kMode == kWeight || p.p_mn ? 128u : 2u, q_step = kMode == kWeight || p.q_mn ? 128u : 2u;
     const uint32_t p_lbo = kMode == kWeight || p.p_mn ? 8192u : 16u, q_lbo = kMode == kWeight || p.q_mn ? 8192u : 16u;
-    const uint64_t d_ones = make_smem_desc(uniform(smem_u32(ones)), 16, 1024);
+    const uint64_t d_ones = make_smem_desc(smem_u32(ones), 16, 1024);
     const uint64_t dp0 = make_smem_desc(stage0, p_lbo, 1024), dq0 = make_smem_desc(stage0 + kGrPBytes, q_lbo, 1024);
-    const uint32_t tmem0 = uniform(tmem_base), peer_full0 = kPair ? uniform(cluster_map(smem_u32(&ctl->peer_full[0]), 0)) : 0u;
-    const uint32_t empty0 = uniform(smem_u32(&ctl->empty[0])), acc_full0 = uniform(smem_u32(&ctl->acc_full[0]));
-    const uint32_t empty1 = kPair ? uniform(cluster_map(empty0, 1)) : 0u, acc_full1 = kPair ? uniform(cluster_map(acc_full0, 1)) : 0u;
+    const uint32_t tmem0 = tmem_base, peer_full0 = kPair ? cluster_map(smem_u32(&ctl->peer_full[0]), 0) : 0u;
+    const uint32_t empty0 = smem_u32(&ctl->empty[0]), acc_full0 = smem_u32(&ctl->acc_full[0]);
+    const uint32_t empty1 = kPair ? cluster_map(empty0, 1) : 0u, acc_full1 = kPair ? cluster_map(acc_full0, 1) : 0u;
     auto product = [&](uint32_t acc, uint64_t dp, uint64_t dq, uint32_t idesc, uint32_t add) {
       if constexpr (kPair) umma_ss_pair(acc, dp, dq, idesc, add);
       else umma_ss<false>(acc, dp, dq, idesc, add);
@@ -448,10 +443,10 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
       }
     };
     uint32_t own_ph = 0, peer_ph = 0;  // a bit for each stage: the phases of the barriers that only cleared blocks use
-    while (__any_sync(0xffffffffu, walk.next(it))) {
-      const uint32_t n_blocks = uniform(it.to - it.from);
-      uint32_t left = uniform((kMode == kWeight ? it.hi - it.lo : static_cast<uint32_t>(p.k_extent)) - it.from * 64u);  // k from here on
-      uint32_t turn = kMode == kWeight ? uniform((it.from + p.n_tiles - n_tile_of(it)) % p.n_tiles) : 0u;  // 0: the ones' products are ours
+    while (walk.next(it)) {
+      const uint32_t n_blocks = it.to - it.from;
+      uint32_t left = (kMode == kWeight ? it.hi - it.lo : static_cast<uint32_t>(p.k_extent)) - it.from * 64u;  // k from here on
+      uint32_t turn = kMode == kWeight ? (it.from + p.n_tiles - n_tile_of(it)) % p.n_tiles : 0u;  // 0: the ones' products are ours
       uint32_t any_ones = 0, acc = 0;
       for (uint32_t kb = 0; kb < n_blocks; ++kb) {
         const uint32_t valid = min(left, 64u), steps = (valid + 15u) / 16u;
