@@ -45,8 +45,8 @@ constexpr int kGrThreads = 320;
 constexpr int kGrEpilogueWarps = 8;
 constexpr int kGrMaxStages = 12;
 constexpr int kGrMaxGroups = 2048;
-constexpr int kGrCtrlBytes = 1024 + 4096;  // barriers; a block of ones (kWeight) or the storing warps' bias (kRows)
-constexpr int kGrSmemLimit = 226 * 1024;  // of dynamic shared memory, beside 1 KB of static
+constexpr int kGrSmemLimit = 227 * 1024;  // all of it dynamic
+constexpr int kGrOnesBytes = 2048;        // 16 columns of 64 k
 constexpr int kGrPBytes = 128 * 128;
 
 enum { kRows = 0, kFew = 1, kWeight = 2 };
@@ -87,7 +87,19 @@ struct GroupedSmem {
   uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem_base, abort_flag;
 };
-static_assert(sizeof(GroupedSmem) <= 1024, "control block too large");
+
+// Shared memory: the stages (a multiple of 1024 bytes, as the ones behind them need it), the storing warps' buffers, a block of ones
+// (kWeight) or those warps' bias (kRows), the barriers, the schedule.  Packed, so that a pair of CTAs has six stages of 32 KB:
+// the products wait for loads half as long as with five.
+template <int kMode, typename T>
+__host__ __device__ constexpr int grouped_store_bytes() {  // of a storing warp: 32 rows of 64 or 128 bytes
+  return sizeof(T) == 4 ? 2048 : 4096;
+}
+template <int kMode, typename T>
+__host__ __device__ constexpr int grouped_extra_bytes() {
+  return kMode == kWeight ? kGrOnesBytes : kMode == kRows ? kGrEpilogueWarps * 128 * static_cast<int>(sizeof(T)) : 0;
+}
+static_assert(sizeof(GroupedSmem) % 8 == 0, "the schedule follows the barriers");
 
 // The rows and tiles of group g, and the blocks of k of a tile; `offsets` are those of the groups in shared memory
 struct GroupSize {
@@ -126,12 +138,15 @@ struct GroupedSchedule {
   uint32_t* offsets;
   uint32_t unit;
 };
-inline int64_t schedule_bytes(int64_t groups) { return align256((groups + 1) * 12 + 4); }
+inline int64_t schedule_bytes(int64_t groups) { return (groups + 1) * 12 + 4; }
 template <int kMode>
-__device__ __forceinline__ GroupedSchedule plan_groups(const GroupedArgs& p, uint32_t* s_first, uint32_t ctas) {
-  __shared__ unsigned long long s_total;
-  __shared__ uint32_t s_units[32], s_pieces[32], s_longest[32], s_shortest[32];
-  __shared__ uint32_t s_best;
+__device__ __forceinline__ GroupedSchedule plan_groups(const GroupedArgs& p, uint32_t* s_first, uint32_t* scratch, uint32_t ctas) {
+  uint32_t* s_units = scratch;
+  uint32_t* s_pieces = scratch + 32;
+  uint32_t* s_longest = scratch + 64;
+  uint32_t* s_shortest = scratch + 96;
+  unsigned long long& s_total = *reinterpret_cast<unsigned long long*>(scratch + 128);
+  uint32_t& s_best = scratch[130];
   const uint32_t G = p.ranges.count, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
   GroupedSchedule plan{s_first, s_first + G + 1u, s_first + 2u * (G + 1u), 0xFFFFFFFFu};
   bool bad = false;
@@ -224,30 +239,37 @@ struct GroupedItem {
   uint32_t unit;
 };
 
-// walks the units of a CTA: every role goes through the same sequence
+// walks the units of a CTA: every role goes through the same sequence (whole warps)
 template <int kMode>
 struct GroupedWalk {
   const GroupedArgs& p;
   const GroupedSchedule& plan;
-  uint32_t at, step, total;
+  uint32_t at, step, total, group = 0;
   __device__ __forceinline__ GroupedWalk(const GroupedArgs& p_, const GroupedSchedule& plan_, uint32_t ctas, uint32_t cta)
       : p(p_), plan(plan_), at(cta), step(ctas), total(plan_.first[p_.ranges.count]) {}
   __device__ __forceinline__ bool next(GroupedItem& it) {
     if (at >= total) return false;
-    uint32_t lo = 0, hi = p.ranges.count - 1u;  // the last group that begins at or before `at`: not an empty one
-    while (lo < hi) {
-      const uint32_t mid = (lo + hi + 1u) / 2u;
-      if (plan.first[mid] <= at) lo = mid;
-      else hi = mid - 1u;
+    // the last group that begins at or before `at` (not an empty one): `at` only grows, and 32 groups are looked at at a time
+    for (uint32_t passed = 32u; passed == 32u; group += passed) {
+      const uint32_t ahead = group + 1u + (threadIdx.x & 31u);
+      passed = __popc(__ballot_sync(0xffffffffu, ahead < p.ranges.count && plan.first[ahead] <= at));
     }
+    const uint32_t lo = group;
     const GroupSize z = group_size<kMode>(p, plan.offsets, lo);
-    const uint32_t length = part_length(p, z.whole, plan.unit), local = at - plan.first[lo], part = local / z.tiles;
+    const uint32_t length = part_length(p, z.whole, plan.unit), local = at - plan.first[lo], part = length < z.whole ? local / z.tiles : 0u;
     it.group = lo;
     it.tile = local - part * z.tiles;
     it.from = part * length, it.to = min(z.whole, it.from + length);
     it.lo = z.lo, it.hi = z.hi;
     it.piece = length < z.whole ? plan.piece[lo] + local : kInvalid;
     it.unit = at;
+    at += step;
+    return true;
+  }
+  // all that the products of kRows have to know of a unit: it is a whole tile
+  __device__ __forceinline__ bool next_whole(GroupedItem& it) {
+    if (at >= total) return false;
+    it.from = 0u, it.to = static_cast<uint32_t>(p.k_blocks);
     at += step;
     return true;
   }
@@ -306,16 +328,20 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
   constexpr int kParamDtype = std::is_same<T, __half>::value ? FGB_F16 : std::is_same<T, __nv_bfloat16>::value ? FGB_BF16 : FGB_F32_IEEE;
   constexpr bool kBlocks = std::is_same<T, float>::value;  // the accumulator is emptied after every block of 64 k
   constexpr int kSums = kMode == kFew ? 1 : 3;             // blocks of 32 columns that a storing warp adds up
-  constexpr int kStore = kBlocks ? 2048 : 4096;            // a storing warp's buffer: 32 rows of 64 or 128 bytes
+  constexpr int kStore = grouped_store_bytes<kMode, T>();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  GroupedSmem* ctl = reinterpret_cast<GroupedSmem*>(smem);
-  uint8_t* ones = smem + 1024;
-  float* s_bias = reinterpret_cast<float*>(smem + 1024);  // of the storing warps' columns: 128 each
-  uint8_t* stages = smem + kGrCtrlBytes;  // multiples of 1024 from here on
-  const int plane_bytes = kGrPBytes + p.q_bytes, stage_bytes = p.planes * plane_bytes;  // of a plane: P, then Q
+  if ((smem_u32(smem_raw) & 1023u) != 0u) {  // the operands' swizzle needs it; no static shared memory is in the way
+    if (threadIdx.x == 0) report(p.status, FGB_S_WAIT_TIMEOUT);
+    return;
+  }
+  uint8_t* stages = smem_raw;
+  const int planes = kBlocks ? p.planes : 1, terms = kBlocks ? p.terms : 1;
+  const int plane_bytes = kGrPBytes + p.q_bytes, stage_bytes = planes * plane_bytes;  // of a plane: P, then Q
   uint8_t* store = stages + size_t(p.stages) * stage_bytes;
-  uint32_t* first = reinterpret_cast<uint32_t*>(store + kGrEpilogueWarps * kStore);
+  uint8_t* ones = store + kGrEpilogueWarps * kStore;
+  T* s_bias = reinterpret_cast<T*>(ones);  // of the storing warps' columns: 128 each
+  GroupedSmem* ctl = reinterpret_cast<GroupedSmem*>(ones + grouped_extra_bytes<kMode, T>());
+  uint32_t* first = reinterpret_cast<uint32_t*>(ctl + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = kPair ? cluster_ctarank() : 0u;
   const int half = kPair ? p.bn / 2 : p.bn;  // columns whose operand this CTA holds
@@ -338,7 +364,7 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
     mbar_init_fence();
   }
   if (kMode == kWeight) {
-    for (int i = tid; i < 512; i += kGrThreads) reinterpret_cast<uint32_t*>(ones)[i] = p.one_pair;
+    for (int i = tid; i < kGrOnesBytes / 4; i += kGrThreads) reinterpret_cast<uint32_t*>(ones)[i] = p.one_pair;
     fence_proxy_async_smem();
   }
   if (warp == 8 && lane == 0) {
@@ -354,7 +380,7 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
     }
   }
   chain_wait();
-  const GroupedSchedule plan = plan_groups<kMode>(p, first, workers);
+  const GroupedSchedule plan = plan_groups<kMode>(p, first, reinterpret_cast<uint32_t*>(store), workers);
   tc_fence_before_sync();
   __syncthreads();
   if constexpr (kPair) cluster_sync_all();
@@ -372,18 +398,19 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
   const uint32_t stage0 = smem_u32(stages);
   if (warp == 8) {
     // ------------------------------------------------------------------ loads
+    // One elected lane goes through all blocks of a unit (elect picks the same lane each time).
     uint32_t s = 0, ph = 0;
     const int G = static_cast<int>(p.ranges.count);
     const uint32_t full_own = smem_u32(&ctl->full[0]), full_leader = kPair ? cluster_map(full_own, 0) : full_own;
     while (walk.next(it)) {
-      // first row (or channel) of the tile along m and n, first k
-      const int m0 = static_cast<int>(m_tile_of(it) * p.tile_m + rank * 128u), n0 = static_cast<int>(n_tile_of(it) * p.bn + rank * half);
-      const int lo = static_cast<int>(it.lo), g = static_cast<int>(it.group), len = static_cast<int>(it.hi - it.lo);
-      const int k_end = static_cast<int>(it.to * 64u);
-      for (int k0 = static_cast<int>(it.from * 64u); k0 < k_end; k0 += 64) {
-        const bool cleared = kMode == kWeight && k0 + 64 > len && (len & 15) != 0;  // see the products
-        wait(&ctl->empty[s], ph ^ 1);
-        if (elect_one()) {
+      if (elect_one()) {
+        // first row (or channel) of the tile along m and n, first k
+        const int m0 = static_cast<int>(m_tile_of(it) * p.tile_m + rank * 128u), n0 = static_cast<int>(n_tile_of(it) * p.bn + rank * half);
+        const int lo = static_cast<int>(it.lo), g = static_cast<int>(it.group), len = static_cast<int>(it.hi - it.lo);
+        const int k_end = static_cast<int>(it.to * 64u);
+        for (int k0 = static_cast<int>(it.from * 64u); k0 < k_end; k0 += 64) {
+          const bool cleared = kMode == kWeight && k0 + 64 > len && (len & 15) != 0;  // see the products
+          wait(&ctl->empty[s], ph ^ 1);
           // Pairs: both CTAs' bytes count on the leader's barrier, so that it has one to wait for -- but for a block that
           // either has to clear rows of first.
           const bool shared = kPair && !cleared;
@@ -394,7 +421,7 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
             else tma_load_3d(dst, map, &ctl->full[s], c0, c1, c2);
           };
           uint32_t pd = stage0 + s * stage_bytes;
-          for (int i = 0; i < p.planes; ++i, pd += plane_bytes) {
+          for (int i = 0; i < planes; ++i, pd += plane_bytes) {
             const uint32_t qd = pd + kGrPBytes;
             if constexpr (kMode == kRows) {
               load(pd, &tmap_p, k0, lo + m0, i);
@@ -415,18 +442,26 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
               for (int c = 0; c * 64 < half; ++c) load(qd + c * 8192, &tmap_q, n0 + c * 64, lo + k0, i);
             }
           }
+          if (++s == static_cast<uint32_t>(p.stages)) s = 0, ph ^= 1;
         }
-        if (++s == static_cast<uint32_t>(p.stages)) s = 0, ph ^= 1;
       }
+      __syncwarp();
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------------ products
-    uint32_t s = 0, ph = 0, set = 0, set_ph = 0;
+    // One elected lane goes through all blocks of a unit and carries the ring's and the accumulators' state; the descriptors
+    // move by one addition, and the next block's barrier is looked at behind the products.  With the whole warp in the loop and
+    // a lane elected for each block the instructions around four products took 690 cycles, more than their 512: 131072 rows of
+    // 16 groups, 1024 x 1024: 229 us, 217 with this loop, 210 with a sixth stage.  The whole warp clears rows, in the last block of a group (kWeight).
     const bool leader = rank == 0u;
-    const uint64_t p_step = kMode == kWeight || p.p_mn ? 128u : 2u, q_step = kMode == kWeight || p.q_mn ? 128u : 2u;
+    const uint32_t p_step = kMode == kWeight || p.p_mn ? 128u : 2u, q_step = kMode == kWeight || p.q_mn ? 128u : 2u;
     const uint32_t p_lbo = kMode == kWeight || p.p_mn ? 8192u : 16u, q_lbo = kMode == kWeight || p.q_mn ? 8192u : 16u;
     const uint64_t d_ones = make_smem_desc(smem_u32(ones), 16, 1024);
+    // the low half of a descriptor holds the address: it moves, the high half stays
     const uint64_t dp0 = make_smem_desc(stage0, p_lbo, 1024), dq0 = make_smem_desc(stage0 + kGrPBytes, q_lbo, 1024);
+    const uint64_t dp_high = dp0 >> 32 << 32, dq_high = dq0 >> 32 << 32;
+    const uint32_t dp_low = static_cast<uint32_t>(dp0), dq_low = static_cast<uint32_t>(dq0);
+    const uint32_t stage_step = static_cast<uint32_t>(stage_bytes) >> 4, plane_step = static_cast<uint32_t>(plane_bytes) >> 4;
     const uint32_t tmem0 = tmem_base, peer_full0 = kPair ? cluster_map(smem_u32(&ctl->peer_full[0]), 0) : 0u;
     const uint32_t empty0 = smem_u32(&ctl->empty[0]), acc_full0 = smem_u32(&ctl->acc_full[0]);
     const uint32_t empty1 = kPair ? cluster_map(empty0, 1) : 0u, acc_full1 = kPair ? cluster_map(acc_full0, 1) : 0u;
@@ -442,78 +477,96 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
         umma_commit(bar0 + 8u * i);
       }
     };
-    uint32_t own_ph = 0, peer_ph = 0;  // a bit for each stage: the phases of the barriers that only cleared blocks use
-    while (walk.next(it)) {
+    // the elected lane's: stage, its phase and offset; accumulator set; whose turn it is to multiply with ones (0: ours)
+    uint32_t s = 0, ph = 0, at = 0, set = 0, set_ph = 0, acc = 0, turn = 0, any_ones = 0;
+    bool ready = false;  // the stage has been seen full
+    auto block = [&](bool begins, bool ends, uint32_t steps, bool look_ahead) {
+      if (begins) {  // a new accumulator
+        wait(&ctl->acc_empty[set], set_ph ^ 1);
+        tc_fence_after_sync();
+        acc = tmem0 + set * p.acc_stride;
+        any_ones = 0;
+      }
+      const bool with_ones = kMode == kWeight && p.db != nullptr && turn == 0u;
+      for (int term = 0; term < terms; ++term) {
+        const uint32_t pp = (p.p_planes >> (4 * term)) & 15u, pq = (p.q_planes >> (4 * term)) & 15u;
+        const uint32_t da = dp_low + at + (kBlocks ? pp * plane_step : 0u), db = dq_low + at + (kBlocks ? pq * plane_step : 0u);
+        const bool ones_now = with_ones && (!kBlocks || pq == 0u);  // once for each plane of dy
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+          if (kMode == kWeight && k >= steps) break;  // elsewhere what is behind the last k has been filled with zeros
+          product(acc, dp_high | (da + k * p_step), dq_high | (db + k * q_step), p.idesc, k == 0 && term == 0 && begins ? 0u : 1u);
+          if (ones_now) product(acc + p.bn, dp_high | (da + k * p_step), d_ones, p.idesc_ones, k == 0 ? any_ones : 1u);
+        }
+        if (ones_now) any_ones = 1u;
+      }
+      commit(empty0, empty1, s);
+      if (ends) {  // the accumulator is done
+        commit(acc_full0, acc_full1, set);
+        if (++set == static_cast<uint32_t>(p.acc_sets)) set = 0, set_ph ^= 1;
+      }
+      at += stage_step;
+      if (++s == static_cast<uint32_t>(p.stages)) s = 0, at = 0, ph ^= 1;
+      if (kMode == kWeight && ++turn == static_cast<uint32_t>(p.n_tiles)) turn = 0u;
+      ready = look_ahead && mbar_try_wait(&ctl->full[s], ph);
+    };
+    // the whole warp's: blocks before the unit; a bit for each stage: the phases of the barriers that only cleared blocks use
+    uint32_t done = 0, own_ph = 0, peer_ph = 0;
+    while (kMode == kRows ? walk.next_whole(it) : walk.next(it)) {
       const uint32_t n_blocks = it.to - it.from;
-      uint32_t left = (kMode == kWeight ? it.hi - it.lo : static_cast<uint32_t>(p.k_extent)) - it.from * 64u;  // k from here on
-      uint32_t turn = kMode == kWeight ? (it.from + p.n_tiles - n_tile_of(it)) % p.n_tiles : 0u;  // 0: the ones' products are ours
-      uint32_t any_ones = 0, acc = 0;
-      for (uint32_t kb = 0; kb < n_blocks; ++kb) {
-        const uint32_t valid = min(left, 64u), steps = (valid + 15u) / 16u;
-        const bool cleared = kMode == kWeight && (valid & 15u) != 0u;
-        const bool with_ones = kMode == kWeight && p.db != nullptr && turn == 0u;
-        const bool begins = kBlocks || kb == 0u;  // a new accumulator
-        if (begins && leader) {
-          wait(&ctl->acc_empty[set], set_ph ^ 1);
-          tc_fence_after_sync();
-          acc = tmem0 + set * p.acc_stride;
-          any_ones = 0;
+      const uint32_t valid = kMode == kWeight ? min(it.hi - it.lo - (it.to - 1u) * 64u, 64u) : 64u;  // k of the last block
+      const uint32_t steps = (valid + 15u) / 16u;
+      const bool cleared = kMode == kWeight && (valid & 15u) != 0u;
+      const uint32_t plain = n_blocks - (cleared ? 1u : 0u);
+      if (leader) {
+        if (elect_one()) {
+          turn = kMode == kWeight ? (it.from + p.n_tiles - n_tile_of(it)) % p.n_tiles : 0u;
+          for (uint32_t kb = 0; kb < plain; ++kb) {
+            if (!ready) wait(&ctl->full[s], ph);
+            block(kBlocks || kb == 0u, kBlocks || kb + 1u == n_blocks, kb + 1u == n_blocks ? steps : 4u, kb + 1u < plain);
+          }
+        }
+        __syncwarp();
+      }
+      if (cleared) {
+        // rows of other groups in the last step: cleared in both operands
+        const uint32_t stage = (done + plain) % static_cast<uint32_t>(p.stages);
+        if (leader) {
+          wait(&ctl->full[stage], (done + plain) / static_cast<uint32_t>(p.stages) & 1u);
+        } else {
+          wait(&ctl->full[stage], own_ph >> stage & 1u);
+          own_ph ^= 1u << stage;
+        }
+        __syncwarp();
+        const uint32_t chunks = static_cast<uint32_t>(stage_bytes) / 8192u, rows = steps * 16u - valid;
+        uint8_t* from = stages + size_t(stage) * stage_bytes;
+        for (uint32_t c = 0; c < chunks; ++c)
+          for (uint32_t r = lane >> 3; r < rows; r += 4u)
+            *reinterpret_cast<uint4*>(from + c * 8192u + (valid + r) * 128u + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if constexpr (kPair) {
+          // the peer's ordinary stores: cluster scope on both sides, here only (a wait of that scope takes some 1000 cycles)
+          if (leader) mbar_wait_cluster(&ctl->peer_full[stage], peer_ph >> stage & 1u, abort_flag);
+          else if (lane == 0) mbar_arrive_cluster_release(peer_full0 + 8u * stage);
+          peer_ph ^= 1u << stage;
+          __syncwarp();
         }
         if (leader) {
-          wait(&ctl->full[s], ph);
-        } else if (cleared) {
-          wait(&ctl->full[s], own_ph >> s & 1u);
-          own_ph ^= 1u << s;
-        }
-        if (cleared) {
-          // rows of other groups in the last step: cleared in both operands
-          __syncwarp();
-          const uint32_t chunks = static_cast<uint32_t>(stage_bytes) / 8192u, rows = steps * 16u - valid;
-          uint8_t* at = stages + size_t(s) * stage_bytes;
-          for (uint32_t c = 0; c < chunks; ++c)
-            for (uint32_t r = lane >> 3; r < rows; r += 4u)
-              *reinterpret_cast<uint4*>(at + c * 8192u + (valid + r) * 128u + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if constexpr (kPair) {
-            // the peer's ordinary stores: cluster scope on both sides, here only (a wait of that scope takes some 1000 cycles)
-            if (leader) mbar_wait_cluster(&ctl->peer_full[s], peer_ph >> s & 1u, abort_flag);
-            else if (lane == 0) mbar_arrive_cluster_release(peer_full0 + 8u * s);
-            peer_ph ^= 1u << s;
-            __syncwarp();
+          if (elect_one()) {
+            if (plain == 0u) turn = (it.from + p.n_tiles - n_tile_of(it)) % p.n_tiles;
+            block(kBlocks || plain == 0u, true, steps, false);
           }
+          __syncwarp();
         }
-        if (leader && elect_one()) {
-          const uint64_t dp = dp0 + ((s * stage_bytes) >> 4), dq = dq0 + ((s * stage_bytes) >> 4);
-          for (int term = 0; term < p.terms; ++term) {
-            const uint32_t pp = (p.p_planes >> (4 * term)) & 15u, pq = (p.q_planes >> (4 * term)) & 15u;
-            const uint64_t da = dp + ((pp * plane_bytes) >> 4), db = dq + ((pq * plane_bytes) >> 4);
-            const uint32_t add = begins && term == 0 ? 0u : 1u;
-            const bool ones_now = with_ones && pq == 0u;  // once for each plane of dy
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) {
-              if (k < steps) {
-                product(acc, da + k * p_step, db + k * q_step, p.idesc, k == 0 ? add : 1u);
-                if (ones_now) product(acc + p.bn, da + k * p_step, d_ones, p.idesc_ones, k == 0 ? any_ones : 1u);
-              }
-            }
-            if (ones_now) any_ones = 1u;
-          }
-          commit(empty0, empty1, s);
-          if (kBlocks || kb + 1u == n_blocks) commit(acc_full0, acc_full1, set);  // the accumulator is done
-        }
-        if (with_ones) any_ones = 1u;
-        if (++s == static_cast<uint32_t>(p.stages)) s = 0, ph ^= 1;
-        left -= 64u;
-        if (kMode == kWeight && ++turn == static_cast<uint32_t>(p.n_tiles)) turn = 0u;
-        if ((kBlocks || kb + 1u == n_blocks) && ++set == static_cast<uint32_t>(p.acc_sets)) set = 0, set_ph ^= 1;
       }
+      done += n_blocks;
     }
   } else {
     // ------------------------------------------------------------------ stores
     const int quarter = warp & 3, group = warp >> 2;
     uint8_t* stage = store + warp * kStore;
-    float* bias_buf = s_bias + warp * 128;
+    T* bias_buf = s_bias + warp * 128;
     uint32_t set = 0, set_ph = 0;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t acc_empty[2] = {kPair ? cluster_map(smem_u32(&ctl->acc_empty[0]), 0) : 0u, kPair ? cluster_map(smem_u32(&ctl->acc_empty[1]), 0) : 0u};
@@ -553,7 +606,7 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
       if (with_bias) {
         __syncwarp();
 #pragma unroll
-        for (int b = 0; b < 4; ++b) bias_buf[b * 32 + lane] = bias[b];
+        for (int b = 0; b < 4; ++b) bias_buf[b * 32 + lane] = static_cast<T>(bias[b]);  // as it was given
         __syncwarp();
       }
       more = look_up();
@@ -564,13 +617,15 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
       float* piece = whole ? nullptr : p.slab + size_t(it.piece) * p.tile_m * p.bn;
       const int64_t row0 = kMode == kRows ? int64_t(it.lo) + m0 : int64_t(it.group) * p.m_extent + m0;
       const int rows = (kMode == kRows ? static_cast<int>(it.hi - it.lo) : p.m_extent) - m0;
+      constexpr int kBias = 16 / sizeof(T);
       auto add_bias = [&](uint32_t (&acc)[32], int b) {
         if (!with_bias) return;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 v = reinterpret_cast<const float4*>(bias_buf + b * 32)[i];
-          acc[4 * i] = __float_as_uint(__uint_as_float(acc[4 * i]) + v.x), acc[4 * i + 1] = __float_as_uint(__uint_as_float(acc[4 * i + 1]) + v.y);
-          acc[4 * i + 2] = __float_as_uint(__uint_as_float(acc[4 * i + 2]) + v.z), acc[4 * i + 3] = __float_as_uint(__uint_as_float(acc[4 * i + 3]) + v.w);
+        for (int i = 0; i < 32; i += kBias) {
+          float v[kBias];
+          Channels<T, kBias>::unpack(*reinterpret_cast<const typename Channels<T, kBias>::Raw*>(bias_buf + b * 32 + i), v);
+#pragma unroll
+          for (int j = 0; j < kBias; ++j) acc[i + j] = __float_as_uint(__uint_as_float(acc[i + j]) + v[j]);
         }
       };
       // 32 columns by ordinary stores; `b`: their place among the warp's columns
@@ -962,7 +1017,7 @@ static int grouped_plan(const fgb_grouped_linear_call& c, int pass, GroupedPlan&
   const int64_t tile_m = p.pair ? 256 : 128, workers = p.pair ? sms / 2 : sms;
   // a part has half of the wanted length at least (a tile is cut only where it is longer), and min_part at least
   p.pieces = p.split ? std::min<int64_t>(2 * kGrMostUnits * workers + 2, blocks / p.min_part) : 0;
-  p.plan_bytes = p.split ? schedule_bytes(G) : 0;
+  p.plan_bytes = p.split ? align256(schedule_bytes(G)) : 0;
   p.slab_bytes = align256(p.pieces * tile_m * p.bn * 4);
   p.db_bytes = db_units > 0 ? align256((db_units + p.pieces) * tile_m * 4) : 0;
   return FGB_OK;
@@ -985,7 +1040,7 @@ static int64_t backward_planes(const fgb_grouped_linear_call& c) {
 template <int kMode, typename T, bool kPair>
 static int launch_grouped(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMap& to, GroupedArgs& a, const GroupedPlan& p, cudaStream_t s) {
   const int prefix = static_cast<int>(schedule_bytes(a.ranges.count));
-  const int fixed = 1024 + kGrCtrlBytes + kGrEpilogueWarps * (sizeof(T) == 4 ? 2048 : 4096) + prefix;
+  const int fixed = kGrEpilogueWarps * grouped_store_bytes<kMode, T>() + grouped_extra_bytes<kMode, T>() + static_cast<int>(sizeof(GroupedSmem)) + prefix;
   const int stage = a.planes * (kGrPBytes + a.q_bytes);
   a.stages = std::min(kGrMaxStages, (kGrSmemLimit - fixed) / stage);
   const size_t smem = size_t(fixed) + size_t(a.stages) * stage;
