@@ -5,7 +5,7 @@
 //   dz    = dy act'(z),  dw = sum dz h,  db = sum dz  (all rows),   q = dz w
 //   dx    = r (q - mean(q) - h mean(q h))             (means as above)
 //
-// Short samples (at most 512 KB on average): one launch.  A team of threads -- a warp, a CTA, or a cluster of up to eight CTAs --
+// Short samples: one launch.  A team of threads -- a warp, a CTA, or a cluster of up to eight CTAs --
 // takes a sample: sums, statistics and the apply pass one after the other, the second read out of L1.  The teams keep their
 // own sums of the backward pass for dw and db, which a second launch adds up.  Else three launches a direction, chained:
 //   1. sums: a CTA takes a block of consecutive rows and adds, channel by channel, the rows of each sample that it meets
@@ -757,9 +757,11 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_small_kernel(con
 }
 
 // ------------------------------------------------------------------ host side
-// A sample on average up to this size goes the short way (all three passes in one launch): what eight CTAs hold in L1 between
-// the passes, with half of it to spare.
-constexpr int64_t kSmallBytes = 512 * 1024;
+// A sample on average up to this size goes the short way (all passes in one launch).  Forward it is what eight CTAs hold in L1
+// between the passes, with half of it to spare; backward there are two tensors to keep, and dw and db cost a launch anyway.
+// us, short / long way (bf16): forward 16 samples of 2048 x 128 (512 KB): 16.2 / 21.2, 64 of 4096 x 128: 58.0 / 57.1; backward 2000
+// of 30 x 256 (15 KB): 64 / 81, 64 of 300 x 128 (77 KB): 24.5 / 25.9, 300 of 256 x 256 (131 KB): 74 / 58, 16 of 2048 x 128: 30 / 22.
+constexpr int64_t kSmallForward = 512 * 1024, kSmallBackward = 48 * 1024;
 constexpr int kSmallChannels = 2048;
 
 struct NormPlan {
@@ -775,20 +777,22 @@ struct NormPlan {
 };
 static NormPlan norm_plan(const fgb_group_norm_call& c) {
   NormPlan p;
+  const bool backward = c.grad_out != nullptr || c.grad_weight != nullptr || c.grad_bias != nullptr;  // without rows there is no grad_out
   p.vec = row_pack(c.c, elem_bytes(c.dtype));
   if (p.vec == 8 && c.c / c.groups % 8 != 0) p.vec = 4;  // eight channels of several groups would take too many registers
   p.one = c.c / c.groups % p.vec == 0;
   const int packs = c.c / p.vec;
   const int64_t sms = device_sm_count(), mean_rows = c.n / c.samples, mean_bytes = mean_rows * c.c * elem_bytes(c.dtype);
-  p.small = mean_bytes <= kSmallBytes && c.c <= kSmallChannels;
+  p.small = mean_bytes <= (backward ? kSmallBackward : kSmallForward) && c.c <= kSmallChannels;
   // Eight packs a thread: that many loads are on their way at a time, and a sample's chain of steps takes the same few
   // microseconds however many threads go through it, so small teams are more samples at a time.
   p.team = 32;
   auto team_smem = [&](int team) { return (kNormThreads / team) * (2 * size_t(c.c) + c.groups) * 8; };
   while (p.team < kNormThreads && (mean_rows * packs > 8 * p.team || team_smem(p.team) > 48 * 1024 || p.team * c.samples * 2 <= 32 * sms)) p.team *= 2;
   p.cluster = 1;
-  // 16 KB a CTA, or as many CTAs as there are SMs for each sample
-  while (p.small && p.team == kNormThreads && p.cluster < 8 && (int64_t(p.cluster) * 16384 < mean_bytes || p.cluster * c.samples * 2 <= sms)) p.cluster *= 2;
+  // Clusters where samples are fewer than SMs, or for more than 64 KB a CTA.  A cluster's barriers cost more than its threads save
+  // where there are samples for all SMs: 600 samples of 100 x 256 took 98 us in clusters of 16 KB a CTA, 31 in single CTAs.
+  while (p.small && p.team == kNormThreads && p.cluster < 8 && (int64_t(p.cluster) * 65536 < mean_bytes || p.cluster * c.samples * 2 <= sms)) p.cluster *= 2;
   if (p.cluster > 1 && mean_bytes / p.cluster < 2048) p.cluster = 1;
   const int64_t ctas = ceil_div(c.samples, kNormThreads / p.team);
   p.grid = static_cast<unsigned>(std::min<int64_t>(ctas, std::max<int64_t>(sms * kNormCtas / p.cluster, 1)) * p.cluster);
@@ -802,7 +806,7 @@ static NormPlan norm_plan(const fgb_group_norm_call& c) {
   p.blocks = static_cast<uint32_t>(std::max<int64_t>(ceil_div(c.n, R), 1));
   p.joined_off = p.small ? align256(int64_t(p.grid / p.cluster) * c.c * 8) : align256((int64_t(p.blocks) + c.samples - 1) * 2 * c.c * 4);
   // one launch forward needs nothing between its passes
-  p.bytes = p.small ? (c.grad_out != nullptr ? p.joined_off : 0) : p.joined_off + align256(c.samples * c.groups * 8);
+  p.bytes = p.small ? (backward ? p.joined_off : 0) : p.joined_off + align256(c.samples * c.groups * 8);
   return p;
 }
 
@@ -837,7 +841,8 @@ static int norm_run_act(const NormArgs& a, const NormPlan& p, bool backward, boo
     return chain.first != cudaSuccess ? cuda_status(chain.first) : launch_status();
   }
   const int64_t units = int64_t(a.ranges.count) * a.G;
-  // a CTA a (sample, group) where the samples cover many blocks, a warp where they are short
+  // A CTA a (sample, group) where the samples cover many blocks, a warp where they are short: 166000 x 256 of 2 samples, forward,
+  // 62 us by CTAs, 81 by warps; of 128 samples 73 and 66.
   const bool warps = int64_t(p.blocks) * a.cpg / a.ranges.count < 64;
   const uint32_t join = static_cast<uint32_t>(warps ? ceil_div(units, kNormThreads / 32) : units);
   if (!backward) {

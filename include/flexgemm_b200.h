@@ -757,7 +757,8 @@ typedef struct fgb_group_norm_call {
   int64_t workspace_bytes;
   int32_t* status;
 } fgb_group_norm_call;
-/* of the backward call where grad_out is set, else of the forward one */
+/* of the backward call where grad_out, grad_weight or grad_bias is set, else
+ * of the forward one */
 int64_t fgb_group_norm_workspace_bytes(const fgb_group_norm_call* call);
 int fgb_group_norm_forward(const fgb_group_norm_call* call, void* stream);
 int fgb_group_norm_backward(const fgb_group_norm_call* call, void* stream);

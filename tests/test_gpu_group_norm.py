@@ -305,6 +305,17 @@ def test_no_rows():
     assert out.shape == (0, 8) and x.grad.shape == (0, 8) and not w.grad.any()
 
 
+@pytest.mark.parametrize("C, samples", [(512, 3), (2056, 40), (96, 2000)])
+def test_parameters_without_rows(C, samples):
+    from flexgemm_b200.ops.group_norm import sparse_group_norm
+    x = torch.zeros(0, C, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    w, b = (torch.ones(C, dtype=torch.bfloat16, device=DEV, requires_grad=True) for _ in range(2))
+    out = sparse_group_norm(x, torch.zeros(samples + 1, dtype=torch.int32, device=DEV), 8, w, b, activation="silu")
+    gw, gb = torch.autograd.grad(out, (w, b), torch.zeros_like(out))
+    torch.cuda.synchronize()
+    assert not gw.any() and not gb.any()
+
+
 def test_input_changed_before_backward_is_refused():
     from flexgemm_b200.ops.group_norm import sparse_group_norm
     x = torch.randn(40, 8, device=DEV, requires_grad=True)

@@ -114,6 +114,16 @@ class NormCall(ctypes.Structure):
                [("eps", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("status", ctypes.c_void_p)]
 
 
+def test_group_norm_workspace_without_rows(lib):
+    """The gradients of weight and bias go through the workspace also where there is no row, and so no grad_out."""
+    call = dict(mean=1 << 20, rstd=1 << 20, n=0, samples=3, offsets_bits=32, offsets=1 << 20, c=512, groups=8, dtype=_cabi.F16, param_dtype=_cabi.F16, eps=1e-5)
+    size = lambda **kw: lib.fgb_group_norm_workspace_bytes(ctypes.byref(NormCall(**{**call, **kw})))
+    need = size(grad_out=1 << 20)
+    assert size() == 0 and need >= 512 * 8
+    assert size(grad_weight=1 << 20) == size(grad_bias=1 << 20) == need
+    assert lib.fgb_group_norm_backward(ctypes.byref(NormCall(**{**call, "grad_weight": 1 << 20})), None) == -1
+
+
 def test_group_norm_entry_points_refuse(lib):
     """Pointers are numbers here: every call is refused before a launch."""
     good = dict(x=1 << 20, out=1 << 21, offsets=1 << 22, mean=1 << 23, rstd=1 << 23, n=100, samples=3, offsets_bits=32, c=64, groups=8,
