@@ -973,8 +973,10 @@ struct GroupedPlan {
   int64_t tiles;        // most tiles (those that the join kernel looks at)
 };
 
-// A tile of few rows where a group has at most 64 on average: see the note on kFew above.
-static bool few_rows(const fgb_grouped_linear_call& c) { return c.n <= 64 * c.groups; }
+// A tile of few rows where a group has at most 16 on average: see the note on kFew above.  us of a forward call and an input
+// gradient, few rows / tiles of 128 (bf16): 8 rows of 8 groups, 4096 -> 1024: 19.7 and 14.0 / 31.2 and 19.9; 1024 rows of
+// 64 groups, 2048 -> 1024: 49.3 and 47.5 / 49.7 and 49.8; with 32 rows a group 256 of 8, 4096 -> 1024: 21.0 and 15.5 / 20.5 and 13.2.
+static bool few_rows(const fgb_grouped_linear_call& c) { return c.n <= 16 * c.groups; }
 
 static int grouped_plan(const fgb_grouped_linear_call& c, int pass, GroupedPlan& p) {
   const int64_t sms = device_sm_count();
@@ -985,7 +987,9 @@ static int grouped_plan(const fgb_grouped_linear_call& c, int pass, GroupedPlan&
   p = GroupedPlan{};
   if (pass == 2) {
     p.mode = kWeight;
-    p.pair = c.co > 128 && c.ci > 64;
+    // A pair reads less for the same products, and has half as many tiles to deal out.  us, single / pair: 131072 rows of 16
+    // groups, 1024 x 1024: 285 / 244; 39872 of 4, 512 x 512: 41.7 / 40.6; 4096 of 16, 1024 x 1024: 23.9 / 26.6.
+    p.pair = c.co > 128 && c.ci > 64 && N >= 2048 * G;
     p.bn = tile_columns(c.ci, most(p.pair));
     const int64_t per = ceil_div(c.ci, p.bn) * ceil_div(c.co, p.pair ? 256 : 128);
     p.tiles = G * per;
@@ -997,16 +1001,25 @@ static int grouped_plan(const fgb_grouped_linear_call& c, int pass, GroupedPlan&
     const int64_t kb = ceil_div(k, 64);
     if (few_rows(c)) {
       p.mode = kFew;
-      // most groups in one tile, and no more columns than that takes
-      p.bn = N <= 16 || N <= 4 * G ? 16 : N <= 16 * G ? 32 : 64;
+      // most groups in one tile: tiles of 16 rows made 2048 rows of 64 groups, 1024 -> 1024, 51.8 us, tiles of 32 34.9
+      p.bn = N <= 16 || N <= 4 * G ? 16 : 32;
       const int64_t m_tiles = ceil_div(nout, 128);
       p.tiles = std::min<int64_t>(N, N / p.bn + G) * m_tiles;
       blocks = p.tiles * kb;
-      if (p.tiles <= sms / 2 && kb >= 8) p.split = 1, p.min_part = 4;
+      // A second launch that adds pieces up takes some 5 us.  24 rows of 2 groups to 512 channels, whole / cut: 1024 channels
+      // 8.8 / 13.7 us, 4096 17.6 / 17.3 (16384 cut: 22.8).
+      if (p.tiles <= sms / 2 && kb > 64) p.split = 1, p.min_part = 4;
     } else {
       p.mode = kRows;
-      p.pair = N >= 512 * G && nout > 64;
-      p.bn = tile_columns(nout, most(p.pair));
+      // tiles as they come out on average; the pairs' are twice as many rows
+      auto tiles = [&](int rows, int64_t columns) { return (N / rows + (G + 1) / 2) * ceil_div(nout, columns); };
+      // Pairs where there are two rounds of tiles and more.  us of a forward call, single / pair: 131072 rows of 16 groups,
+      // 1024 -> 1024: 264 / 233; 166000 of 4, 256 -> 256: 41.7 / 39.1 (one lane a block, see the products); 20000 of 4: 10.7 /
+      // 11.0; 10000 of 4: 7.8 / 8.6.
+      p.pair = N >= 512 * G && nout > 64 && tiles(256, most(true)) >= sms;
+      // Half as many columns where half of the SMs had no tile: 4096 rows of 2 groups, 512 -> 512, 9.2 us with 256, 7.6 with 128;
+      // 8192 of 2: 10.1 / 11.0.
+      p.bn = tile_columns(nout, !p.pair && !is_f32(c.dtype) && 2 * tiles(128, 256) <= sms ? 128 : most(p.pair));
       p.tiles = (N / (p.pair ? 256 : 128) + G) * ceil_div(nout, p.bn);
       blocks = p.tiles * kb;
     }
