@@ -98,6 +98,21 @@ def test_matches_plain_form(lengths, C, groups, spare, dtype):
         assert not out[ends[-1]:].any() and not grads[0][ends[-1]:].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("lengths,C,groups", [
+    ([7] * 30 + [3000, 0, 2500] + [7] * 500 + [2800, 4000] + [1] * 20, 96, 12),
+    ([9000, 1] + [3] * 700 + [5000], 8, 2),
+    ([4100] * 9 + [0] * 3000 + [2], 33, 3),
+    ([2] * 900 + [20000], 64, 8),
+])
+def test_long_samples_among_short_ones(lengths, C, groups, dtype):
+    x, dy, w, b, ends = problem(lengths, C, dtype, spare=5, seed=C)
+    out, grads = check(x, dy, w, b, ends, groups, "silu")
+    again = run(x, dy, w, b, ends.to(DEV), groups, "silu")
+    assert torch.equal(out, again[0]) and all(torch.equal(u, v) for u, v in zip(grads, again[1]))
+    assert not out[ends[-1]:].any() and not grads[0][ends[-1]:].any()
+
+
 @pytest.mark.parametrize("w_on,b_on", [(False, False), (True, False), (False, True)])
 def test_without_parameters(w_on, b_on):
     x, dy, w, b, ends = problem([40, 300], 24, torch.float16, seed=3)
