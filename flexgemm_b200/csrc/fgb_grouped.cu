@@ -55,6 +55,7 @@ struct GroupedArgs {
   RowRanges ranges;
   int bn;               // columns of a tile
   int tile_m;           // rows of it: 128, or 256 of a pair of CTAs
+  int row_shift;        // kRows, kFew: log2 of the rows that a tile has of a group (tile_m; bn)
   int n_tiles;          // tiles along the channels that are not rows: kRows along n, kFew along m, kWeight along n
   int m_tiles;          // kWeight: tiles along co
   int k_blocks;         // kRows, kFew: blocks of 64 along k
@@ -111,8 +112,7 @@ __device__ __forceinline__ GroupSize group_size(const GroupedArgs& p, const uint
   s.lo = offsets[g];
   s.hi = offsets[g + 1u];
   const uint32_t len = s.hi - s.lo;
-  if constexpr (kMode == kRows) s.tiles = (len + p.tile_m - 1u) / p.tile_m * p.n_tiles;
-  else if constexpr (kMode == kFew) s.tiles = (len + p.bn - 1u) / p.bn * p.n_tiles;
+  if constexpr (kMode != kWeight) s.tiles = ((len + (1u << p.row_shift) - 1u) >> p.row_shift) * p.n_tiles;
   else s.tiles = len > 0u ? p.n_tiles * p.m_tiles : 0u;
   s.whole = kMode == kWeight ? (len + 63u) / 64u : static_cast<uint32_t>(p.k_blocks);
   return s;
@@ -123,7 +123,9 @@ __device__ __forceinline__ uint32_t part_length(const GroupedArgs& p, uint32_t w
   const uint32_t parts = min((whole + unit - 1u) / unit, max(whole / p.min_part, 1u));
   return (whole + parts - 1u) / parts;
 }
-__device__ __forceinline__ uint32_t parts_of(uint32_t whole, uint32_t length) { return length == 0u ? 0u : (whole + length - 1u) / length; }
+__device__ __forceinline__ uint32_t parts_of(uint32_t whole, uint32_t length) {
+  return length == 0u ? 0u : length == whole ? 1u : (whole + length - 1u) / length;
+}
 
 // What every CTA works out at its start: first[g] = units of the groups before g, piece[g] = pieces of tiles before g, the
 // groups' offsets, and the length that parts should have.  The whole CTA calls it (and waits at its end).
@@ -140,13 +142,7 @@ struct GroupedSchedule {
 };
 inline int64_t schedule_bytes(int64_t groups) { return (groups + 1) * 12 + 4; }
 template <int kMode>
-__device__ __forceinline__ GroupedSchedule plan_groups(const GroupedArgs& p, uint32_t* s_first, uint32_t* scratch, uint32_t ctas) {
-  uint32_t* s_units = scratch;
-  uint32_t* s_pieces = scratch + 32;
-  uint32_t* s_longest = scratch + 64;
-  uint32_t* s_shortest = scratch + 96;
-  unsigned long long& s_total = *reinterpret_cast<unsigned long long*>(scratch + 128);
-  uint32_t& s_best = scratch[130];
+__device__ __forceinline__ GroupedSchedule plan_groups(const GroupedArgs& p, uint32_t* s_first, float* costs, uint32_t ctas) {
   const uint32_t G = p.ranges.count, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
   GroupedSchedule plan{s_first, s_first + G + 1u, s_first + 2u * (G + 1u), 0xFFFFFFFFu};
   bool bad = false;
@@ -154,7 +150,6 @@ __device__ __forceinline__ GroupedSchedule plan_groups(const GroupedArgs& p, uin
     plan.offsets[g] = p.ranges.at(g);
     bad |= g < G && !p.ranges.good(g);
   }
-  if (p.min_part != 0u && threadIdx.x < 32u) s_units[lane] = s_pieces[lane] = s_longest[lane] = 0u, s_shortest[lane] = 0xFFFFFFFFu;
   // ranges that overlap could ask for more tiles than there is room for: nothing is done
   bad = __syncthreads_or(bad) != 0;
   if (bad && threadIdx.x == 0) {
@@ -162,43 +157,37 @@ __device__ __forceinline__ GroupedSchedule plan_groups(const GroupedArgs& p, uin
     mirror_code(p.mirror, FGB_S_BAD_OFFSETS);
   }
   if (p.min_part != 0u && !bad) {
-    if (warp == 0) {
-      unsigned long long total = 0;
+    // every warp: all blocks of k
+    unsigned long long total = 0;
+    for (uint32_t g = lane; g < G; g += 32u) {
+      const GroupSize z = group_size<kMode>(p, plan.offsets, g);
+      total += static_cast<unsigned long long>(z.tiles) * z.whole;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    const float share = static_cast<float>(total) / static_cast<float>(ctas);
+    auto unit_of = [&](uint32_t i) { return i == 31u ? 0xFFFFFFFFu : max(static_cast<uint32_t>(ceilf(share * 2.f * exp2f(-2.5849625f / 30.f * static_cast<float>(i)))), 1u); };
+    for (uint32_t i = warp; i < 32u; i += blockDim.x / 32u) {
+      const uint32_t unit = unit_of(i);
+      uint32_t units = 0, pieces = 0, longest = 0, shortest = 0xFFFFFFFFu;
       for (uint32_t g = lane; g < G; g += 32u) {
         const GroupSize z = group_size<kMode>(p, plan.offsets, g);
-        total += static_cast<unsigned long long>(z.tiles) * z.whole;
+        if (z.tiles == 0u) continue;
+        const uint32_t len = part_length(p, z.whole, unit), parts = parts_of(z.whole, len);
+        units += parts * z.tiles;
+        if (parts > 1u) pieces += parts * z.tiles;
+        longest = max(longest, len), shortest = min(shortest, len);
       }
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-      if (lane == 0) s_total = total;
+      units = __reduce_add_sync(0xffffffffu, units), pieces = __reduce_add_sync(0xffffffffu, pieces);
+      longest = __reduce_max_sync(0xffffffffu, longest), shortest = __reduce_min_sync(0xffffffffu, shortest);
+      const float len = static_cast<float>(longest);
+      const float most = longest == shortest ? static_cast<float>((units + ctas - 1u) / ctas) * len : fmaxf(share + 0.5f * len, len);
+      if (lane == 0u) costs[i] = most + static_cast<float>(pieces) / static_cast<float>(ctas) * p.piece_cost;
     }
     __syncthreads();
-    const float share = static_cast<float>(s_total) / static_cast<float>(ctas);
-    const uint32_t unit = lane == 31u ? 0xFFFFFFFFu : static_cast<uint32_t>(ceilf(share * 2.f * exp2f(-2.5849625f / 30.f * static_cast<float>(lane))));
-    uint32_t units = 0, pieces = 0, longest = 0, shortest = 0xFFFFFFFFu;
-    for (uint32_t g = warp; g < G; g += blockDim.x / 32u) {
-      const GroupSize z = group_size<kMode>(p, plan.offsets, g);
-      if (z.tiles == 0u) continue;
-      const uint32_t len = part_length(p, z.whole, max(unit, 1u)), parts = parts_of(z.whole, len);
-      units += parts * z.tiles;
-      if (parts > 1u) pieces += parts * z.tiles;
-      longest = max(longest, len), shortest = min(shortest, len);
-    }
-    atomicAdd(&s_units[lane], units);
-    atomicAdd(&s_pieces[lane], pieces);
-    atomicMax(&s_longest[lane], longest);
-    atomicMin(&s_shortest[lane], shortest);
-    __syncthreads();
-    if (warp == 0) {
-      const float len = static_cast<float>(s_longest[lane]);
-      const float most = s_longest[lane] == s_shortest[lane] ? static_cast<float>((s_units[lane] + ctas - 1u) / ctas) * len : fmaxf(share + 0.5f * len, len);
-      const float cost = most + static_cast<float>(s_pieces[lane]) / static_cast<float>(ctas) * p.piece_cost;
-      // the cheapest, of equally cheap ones the longest
-      const uint32_t least = __reduce_min_sync(0xffffffffu, __float_as_uint(cost));
-      if (static_cast<uint32_t>(__ffs(__ballot_sync(0xffffffffu, __float_as_uint(cost) == least)) - 1) == lane) s_best = max(unit, 1u);
-    }
-    __syncthreads();
-    plan.unit = s_best;
+    // the cheapest, of equally cheap ones the longest
+    const uint32_t cost = __float_as_uint(costs[lane]), least = __reduce_min_sync(0xffffffffu, cost);
+    plan.unit = unit_of(static_cast<uint32_t>(__ffs(__ballot_sync(0xffffffffu, cost == least)) - 1));
   }
   for (uint32_t g = threadIdx.x; g < G; g += blockDim.x) {
     const GroupSize z = group_size<kMode>(p, plan.offsets, g);
@@ -379,11 +368,13 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
       tmem_relinquish();
     }
   }
+  // some 1000 cycles until the other CTA knows these barriers: the plan is made meanwhile
+  if constexpr (kPair) cluster_arrive();
   chain_wait();
-  const GroupedSchedule plan = plan_groups<kMode>(p, first, reinterpret_cast<uint32_t*>(store), workers);
+  const GroupedSchedule plan = plan_groups<kMode>(p, first, reinterpret_cast<float*>(store), workers);
   tc_fence_before_sync();
   __syncthreads();
-  if constexpr (kPair) cluster_sync_all();
+  if constexpr (kPair) cluster_wait();
   tc_fence_after_sync();
   const uint32_t tmem_base = ctl->tmem_base;
   GroupedWalk<kMode> walk(p, plan, workers, worker);
@@ -1081,6 +1072,7 @@ static int grouped_pass(const fgb_grouped_linear_call& c, int pass, const Operan
   GroupedArgs a{};
   a.ranges = RowRanges{c.offsets, c.offsets_bits == 64, static_cast<uint32_t>(c.n), static_cast<uint32_t>(c.groups)};
   a.bn = p.bn, a.tile_m = p.pair ? 256 : 128;
+  for (const int rows = p.mode == kFew ? a.bn : a.tile_m; (1 << a.row_shift) < rows;) ++a.row_shift;
   const int half = p.pair ? p.bn / 2 : p.bn;
   a.planes = planes_of(c.dtype);
   a.terms = c.dtype == FGB_F32_IEEE ? 6 : c.dtype == FGB_F32_TF32 ? 3 : 1;
