@@ -1178,7 +1178,7 @@ bool offsets_arg_ok(const Tensor& t, const Tensor& rows) {
 }
 // gradient of an output: in the output's layout and type
 Tensor grad_rows(const Tensor& g, at::ScalarType dtype) {
-  Tensor r = (g.scalar_type() == dtype ? g : g.to(dtype)).contiguous();
+  Tensor r = (g.scalar_type() == dtype ? g : g.to(dtype)).contiguous().resolve_neg();
   return aligned(r) ? r : r.clone();
 }
 

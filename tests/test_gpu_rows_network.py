@@ -126,6 +126,20 @@ def test_samples_do_not_see_one_another():
         assert (alone - whole[mine.to(DEV)]).abs().max().item() <= 1e-3 * scale
 
 
+def test_negated_gradients():
+    """A gradient that says only by a flag that it is negated."""
+    from flexgemm_b200.ops.embedding import sparse_embedding
+    from flexgemm_b200.ops.group_norm import sparse_group_norm
+    from flexgemm_b200.ops.grouped_linear import sparse_grouped_linear
+    x = torch.randn(70, 16, device=DEV, requires_grad=True)
+    w = torch.randn(2, 16, 16, device=DEV, requires_grad=True)
+    ends = torch.tensor([0, 30, 70], device=DEV)
+    for out, leaf in ((sparse_embedding(torch.arange(70, device=DEV), x, 2.0), x), (sparse_group_norm(x, ends, 4), x), (sparse_grouped_linear(x, ends, w), w)):
+        dy = torch.randn_like(out)
+        want = torch.autograd.grad(out, leaf, -dy, retain_graph=True)[0]
+        assert torch.equal(torch.autograd.grad(out, leaf, torch._neg_view(dy))[0], want)
+
+
 def test_two_streams_at_once():
     coords, labels, params, grad, shape = make(6)
     p = {k: v.to(DEV) for k, v in params.items()}
