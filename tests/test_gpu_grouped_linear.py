@@ -93,6 +93,34 @@ def test_matches_plain_form(lengths, ci, co, spare, dtype):
     check(*problem(lengths, ci, co, dtype, spare, seed=ci + co, bias=ci != 64))
 
 
+VARIANTS = [
+    # pairs of CTAs: forward, input gradient, weight gradient (rows cleared in both CTAs), narrower last tiles
+    ([4500, 300], 72, 2056, 0),
+    ([3001, 1700], 2056, 72, 7),
+    ([9001], 1040, 640, 0),
+    ([2100, 0, 4200], 136, 2824, 1),
+    # few rows, cut along 4104 or 4200 channels
+    ([3, 5, 0, 9], 4104, 24, 0),
+    ([2, 7], 40, 4200, 3),
+    ([11], 8200, 136, 0),
+    # tiles of half as many columns
+    ([200, 130], 80, 520, 0),
+    # searches past more than 32 groups, few rows and many
+    ([1] * 40 + [0] * 100 + [3] * 40 + [200], 24, 40, 2),
+    ([0] * 40 + [2000] + [0] * 33 + [1900, 0], 64, 96, 0),
+    # all rows in one of many groups
+    ([0] * 60 + [900] + [0] * 20, 64, 72, 0),
+    # the plan of many groups
+    ([2, 1, 0, 3] * 500, 16, 24, 5),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lengths,ci,co,spare", VARIANTS)
+def test_variants(lengths, ci, co, spare, dtype):
+    check(*problem(lengths, ci, co, dtype, spare, seed=ci, bias=ci != 40))
+
+
 @pytest.mark.parametrize("lengths,ci,co", [([300, 500], 64, 72), ([4, 9], 128, 256), ([90], 20, 12)])
 def test_float32_with_tf32_allowed(lengths, ci, co):
     from flexgemm_b200.kernels import config
