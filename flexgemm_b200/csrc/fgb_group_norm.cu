@@ -482,14 +482,21 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_apply_kernel(con
 }
 
 // ------------------------------------------------------------------ short samples
+// Ragged samples may be long ones in between, and a team would be at one long after all others are done.  Teams leave samples of
+// more than long_rows rows out, and a second launch (kLong) takes them in clusters of kLongCtas CTAs; neighbours, which are often
+// alike, go to different clusters.  us, in one launch / in two (bf16, 96 channels): 2000 samples of 7 rows around one of 50000, forward
+// 2591 / 159, backward 7374 / 321; 2000 samples of 20 rows 14.5 / 16.9 and 28.2 / 31.5.  Lengths that scatter like exp(N(0, 1)) (80000
+// rows of fp32 in 2048 samples, forward + backward): 110 to 162 / 130.
+constexpr int kLongCtas = 8, kLongClusters = 18;
 struct SmallArgs {
-  int team;           // threads of a CTA that take a sample: 32, 64, 128 or 256
-  int cluster;        // CTAs that do (1 where a CTA has several teams)
-  uint32_t teams;     // samples at a time; team t takes the samples t, t + teams, ...
-  F2* columns;        // backward: [CTAs, or clusters][C] sums of dz and dz h
+  int team;            // threads of a CTA that take a sample: 32, 64, 128 or 256
+  int cluster;         // CTAs that do (1 where a CTA has several teams)
+  uint32_t teams;      // samples at a time; team t takes the samples t, t + teams, ...
+  uint32_t long_rows;  // see above
+  F2* columns;         // backward: [CTAs, or clusters][C] sums of dz and dz h
 };
 
-template <typename T, int kVec, bool kOne, bool kBackward, bool kSilu>
+template <typename T, int kVec, bool kOne, bool kBackward, bool kSilu, bool kLong>
 __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_small_kernel(const NormArgs p, const SmallArgs q) {
   using Ch = Channels<T, kVec>;
   using Raw = typename Ch::Raw;
@@ -521,8 +528,8 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_small_kernel(con
     for (int c = t; c < p.C; c += size) columns[c] = both(0.f);
     sync();
   }
-  for (uint32_t s = team; s < p.ranges.count; s += q.teams) {
-    const uint32_t lo = p.ranges.at(s), hi = max(lo, p.ranges.at(s + 1u)), len = hi - lo;
+  auto sample = [&](uint32_t s, uint32_t lo, uint32_t hi) {
+    const uint32_t len = hi - lo;
     const uint32_t share = (len + q.cluster - 1u) / q.cluster, from = min(hi, lo + rank * share), to = min(hi, from + share);
     // 1. sums of this CTA's rows, for each channel
     for (int pack0 = 0; pack0 < packs; pack0 += size) {
@@ -732,6 +739,32 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_small_kernel(con
       }
     }
     sync();  // sums and statistics are written again
+  };
+  if constexpr (!kLong) {
+    for (uint32_t s = team; s < p.ranges.count; s += q.teams) {
+      const uint32_t lo = p.ranges.at(s), hi = max(lo, p.ranges.at(s + 1u));
+      if (hi - lo <= q.long_rows) sample(s, lo, hi);
+    }
+  } else {
+    // 256 of the cluster's samples are looked at at a time; all its CTAs find the same
+    __shared__ uint32_t s_long[kNormThreads / 32];
+    for (uint64_t s0 = team; s0 < p.ranges.count; s0 += uint64_t(kNormThreads) * q.teams) {
+      const uint64_t k = s0 + uint64_t(threadIdx.x) * q.teams;
+      bool is_long = false;
+      if (k < p.ranges.count) {
+        const uint32_t lo = p.ranges.at(static_cast<uint32_t>(k)), hi = p.ranges.at(static_cast<uint32_t>(k) + 1u);
+        is_long = hi > lo && hi - lo > q.long_rows;
+      }
+      const uint32_t found = __ballot_sync(0xffffffffu, is_long);
+      if ((threadIdx.x & 31u) == 0u) s_long[threadIdx.x / 32u] = found;
+      __syncthreads();
+      for (uint32_t word = 0; word < kNormThreads / 32; ++word)
+        for (uint32_t left = s_long[word]; left != 0u; left &= left - 1u) {
+          const uint32_t s = static_cast<uint32_t>(s0) + (word * 32u + __ffs(left) - 1u) * q.teams, lo = p.ranges.at(s);
+          sample(s, lo, max(lo, p.ranges.at(s + 1u)));
+        }
+      __syncthreads();
+    }
   }
   if constexpr (kBackward) {
     __syncthreads();
@@ -746,7 +779,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_small_kernel(con
     }
   }
   // rows of no sample
-  if (out != nullptr) {
+  if (!kLong && out != nullptr) {
     const uint32_t begin = p.ranges.at(0u), end = max(begin, p.ranges.at(p.ranges.count)), outside = begin + (p.ranges.n - end);
     Raw zero{};
     for (uint64_t i = uint64_t(blockIdx.x) * kNormThreads + threadIdx.x; i < uint64_t(outside) * packs; i += uint64_t(gridDim.x) * kNormThreads) {
@@ -768,7 +801,9 @@ struct NormPlan {
   bool small;         // the short way:
   int team, cluster;  // threads of a CTA, and CTAs, for a sample
   unsigned grid;
-  size_t small_smem;
+  uint32_t long_rows;
+  int long_clusters;  // of the second launch; 0: there is none
+  size_t small_smem, long_smem;
   int vec;
   bool one;           // a pack lies in one group
   unsigned columns;   // CTAs along a row
@@ -796,7 +831,10 @@ static NormPlan norm_plan(const fgb_group_norm_call& c) {
   if (p.cluster > 1 && mean_bytes / p.cluster < 2048) p.cluster = 1;
   const int64_t ctas = ceil_div(c.samples, kNormThreads / p.team);
   p.grid = static_cast<unsigned>(std::min<int64_t>(ctas, std::max<int64_t>(sms * kNormCtas / p.cluster, 1)) * p.cluster);
-  p.small_smem = team_smem(p.team);
+  p.small_smem = team_smem(p.team), p.long_smem = team_smem(kNormThreads);
+  // 128 packs a thread, some 10 us of a team
+  p.long_rows = p.cluster == 1 && c.offsets_bits != 0 ? static_cast<uint32_t>(128 * p.team / packs) : 0xFFFFFFFFu;
+  p.long_clusters = p.small && p.long_rows < c.n ? static_cast<int>(std::min<int64_t>(kLongClusters, c.samples)) : 0;
   p.columns = static_cast<unsigned>(ceil_div(packs, kNormThreads));
   const int width = packs < kNormThreads ? packs : kNormThreads, lanes = kNormThreads / width;
   // as many CTAs as run at a time, each thread at least eight rows
@@ -804,7 +842,7 @@ static NormPlan norm_plan(const fgb_group_norm_call& c) {
   const int64_t R = std::max<int64_t>(ceil_div(c.n, want), int64_t(lanes) * 8);
   p.R = static_cast<uint32_t>(R);
   p.blocks = static_cast<uint32_t>(std::max<int64_t>(ceil_div(c.n, R), 1));
-  p.joined_off = p.small ? align256(int64_t(p.grid / p.cluster) * c.c * 8) : align256((int64_t(p.blocks) + c.samples - 1) * 2 * c.c * 4);
+  p.joined_off = p.small ? align256((int64_t(p.grid / p.cluster) + p.long_clusters) * c.c * 8) : align256((int64_t(p.blocks) + c.samples - 1) * 2 * c.c * 4);
   // one launch forward needs nothing between its passes
   p.bytes = p.small ? (backward ? p.joined_off : 0) : p.joined_off + align256(c.samples * c.groups * 8);
   return p;
@@ -827,15 +865,24 @@ static int norm_run_act(const NormArgs& a, const NormPlan& p, bool backward, boo
   const dim3 grid(p.blocks, p.columns);
   LaunchErrors chain;
   if (p.small) {
-    const SmallArgs q{p.team, p.cluster, p.grid / p.cluster * (kNormThreads / p.team), want_param ? a.part : nullptr};
-    auto kernel = backward ? norm_small_kernel<T, kVec, kOne, true, kSilu> : norm_small_kernel<T, kVec, kOne, false, kSilu>;
-    static PerDeviceTable configured[2];
-    const int rc = ensure_dynamic_smem(configured[backward], kernel, p.small_smem);
+    const uint32_t slots = p.grid / p.cluster;
+    const SmallArgs q{p.team, p.cluster, slots * (kNormThreads / p.team), p.long_rows, want_param ? a.part : nullptr};
+    auto kernel = backward ? norm_small_kernel<T, kVec, kOne, true, kSilu, false> : norm_small_kernel<T, kVec, kOne, false, kSilu, false>;
+    static PerDeviceTable configured[2], configured_long[2];
+    int rc = ensure_dynamic_smem(configured[backward], kernel, p.small_smem);
     if (rc != FGB_OK) return rc;
     chain.add(launch_chained_clusters(kernel, dim3(p.grid), dim3(kNormThreads), p.small_smem, p.cluster, s, a, q));
+    if (p.long_clusters > 0) {
+      const unsigned clusters = static_cast<unsigned>(p.long_clusters);
+      const SmallArgs l{kNormThreads, kLongCtas, clusters, p.long_rows, want_param ? a.part + size_t(slots) * a.C : nullptr};
+      auto rest = backward ? norm_small_kernel<T, kVec, kOne, true, kSilu, true> : norm_small_kernel<T, kVec, kOne, false, kSilu, true>;
+      rc = ensure_dynamic_smem(configured_long[backward], rest, p.long_smem);
+      if (rc != FGB_OK) return rc;
+      chain.add(launch_chained_clusters(rest, dim3(clusters * kLongCtas), dim3(kNormThreads), p.long_smem, kLongCtas, s, a, l));
+    }
     if (want_param) {
       NormArgs cols = a;
-      cols.slots = p.grid / p.cluster;
+      cols.slots = slots + static_cast<uint32_t>(p.long_clusters);
       chain.add(launch_chained(norm_join_kernel<32, true>, dim3(static_cast<unsigned>(ceil_div(a.C, 8))), dim3(kNormThreads), 0, s, cols, 0u));
     }
     return chain.first != cudaSuccess ? cuda_status(chain.first) : launch_status();
