@@ -281,12 +281,19 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_join_kernel(const EmbGr
   const int cx = threadIdx.x & 7, ry = threadIdx.x >> 3;
   const int c0 = static_cast<int>(blockIdx.y) * kJoinCols + cx * 4;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (uint32_t k = q + ry; k <= last; k += 32u) {
-    const float* from = p.slab + (size_t(k) * 2 + (k == q ? 1 : 0)) * p.C + c0;
+  for (uint32_t k0 = q + ry; k0 <= last; k0 += 4u * 32u) {
+    float v[4][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (c0 + i < p.C) acc[i] += from[i];
+    for (uint32_t u = 0; u < 4u; ++u) {
+      const uint32_t k = k0 + u * 32u;
+      const float* from = p.slab + (size_t(k) * 2 + (k == q ? 1 : 0)) * p.C + c0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[u][i] = k <= last && c0 + i < p.C ? from[i] : 0.f;
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < 4u; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] += v[u][i];
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) s_sum[ry][cx * 4 + i] = acc[i];

@@ -287,25 +287,36 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_sums_kernel(cons
 
 // ------------------------------------------------------------------ 2. join
 template <int kThreads>
-__device__ __forceinline__ double sum_of_threads(double v, double* s_red) {
+__device__ __forceinline__ void sum_of_threads(double& v0, double& v1, double (*s_red)[2]) {  // once a kernel
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  for (int d = 16; d > 0; d >>= 1) v0 += __shfl_xor_sync(0xffffffffu, v0, d), v1 += __shfl_xor_sync(0xffffffffu, v1, d);
   if constexpr (kThreads > 32) {
+    if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5][0] = v0, s_red[threadIdx.x >> 5][1] = v1;
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0;
+    const int w = threadIdx.x & (kThreads / 32 - 1);
+    v0 = s_red[w][0], v1 = s_red[w][1];
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) v += s_red[w];
+    for (int d = kThreads / 64; d > 0; d >>= 1) v0 += __shfl_xor_sync(0xffffffffu, v0, d), v1 += __shfl_xor_sync(0xffffffffu, v1, d);
   }
-  return v;
+}
+
+// Entries k0, k0 + step, ... below `end` of a column of the slots, zeros behind: all on their way at once.  (Whole batches and a
+// remainder loop waited for each entry of the remainder, which is mostly all there is.)
+constexpr int kJoinLoads = 8;
+__device__ __forceinline__ void load_join(F2 (&v)[kJoinLoads], const F2* column, int C, uint32_t k0, uint32_t step, uint32_t end) {
+#pragma unroll
+  for (int u = 0; u < kJoinLoads; ++u) {
+    const uint32_t k = k0 + u * step;
+    v[u] = F2{0.f, 0.f};
+    if (k < end) v[u] = column[size_t(k) * C];
+  }
 }
 
 // kThreads threads of the CTA's 256 take one (sample, group); backward: the CTAs from `join_ctas` on add up eight columns each.
 // A unit's entries are (block, channel of the group): a thread keeps to one channel and takes every few blocks.
 template <int kThreads, bool kBackward>
 __global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const NormArgs p, uint32_t join_ctas) {
-  __shared__ double s_red[kNormThreads / 32];
+  __shared__ double s_red[kNormThreads / 32][2];
   __shared__ float s_col[2][32][8];
   chain_release();
   chain_wait();
@@ -314,10 +325,11 @@ __global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const NormArgs 
     const uint32_t slots = p.slots;
     float db = 0.f, dw = 0.f;
     if (c < p.C) {
-#pragma unroll 8
-      for (uint32_t k = w; k < slots; k += 32u) {
-        const F2 v = p.part[size_t(k) * p.C + c];
-        db += v.x, dw += v.y;
+      for (uint32_t k0 = w; k0 < slots; k0 += 32u * kJoinLoads) {
+        F2 v[kJoinLoads];
+        load_join(v, p.part + c, p.C, k0, 32u, slots);
+#pragma unroll
+        for (int u = 0; u < kJoinLoads; ++u) db += v[u].x, dw += v[u].y;
       }
     }
     s_col[0][w][threadIdx.x & 7] = db;
@@ -333,14 +345,14 @@ __global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const NormArgs 
     }
     return;
   }
-  const uint64_t unit = uint64_t(blockIdx.x) * (kNormThreads / kThreads) + threadIdx.x / kThreads;
-  if (unit >= uint64_t(p.ranges.count) * p.G) return;  // whole warps; with 256 threads a unit whole CTAs
-  const uint32_t s = static_cast<uint32_t>(unit / p.G), g = static_cast<uint32_t>(unit % p.G), t = threadIdx.x % kThreads;
+  const uint32_t unit = blockIdx.x * (kNormThreads / kThreads) + threadIdx.x / kThreads;  // samples * groups < 2^31
+  if (unit >= p.ranges.count * static_cast<uint32_t>(p.G)) return;  // whole warps; with 256 threads a unit whole CTAs
+  const uint32_t s = unit / p.G, g = unit - s * p.G, t = threadIdx.x % kThreads;
   const uint32_t lo = p.ranges.at(s), hi = max(lo, p.ranges.at(s + 1u));
   const uint32_t j0 = lo / p.R, blocks = lo < hi ? (hi - 1u) / p.R - j0 + 1u : 0u;
   const uint32_t cpg = p.cpg, across = min(cpg, static_cast<uint32_t>(kThreads)), down = kThreads / across;
   const uint32_t c_own = t % across, k_own = t / across;
-  const double count = static_cast<double>(hi - lo) * cpg;
+  const double inv_count = 1.0 / (static_cast<double>(hi - lo) * cpg);  // unused where there are no rows
   const F2* part = p.part + size_t(j0 + s) * p.C + g * cpg;
   double v0 = 0, v1 = 0;
   if constexpr (!kBackward) {
@@ -349,47 +361,53 @@ __global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const NormArgs 
     const double pivot = blocks > 0u ? part[0].x : 0.f;
     if (k_own < down) {
       for (uint32_t c = c_own; c < cpg; c += across) {
-#pragma unroll 8
-        for (uint32_t k = k_own; k < blocks; k += down) {
-          const F2 v = part[size_t(k) * p.C + c];
-          const double rows = static_cast<double>(min(hi, (j0 + k + 1u) * p.R) - max(lo, (j0 + k) * p.R)), d = v.x - pivot;
-          v0 += rows * d;
-          v1 += v.y + rows * d * d;
+        for (uint32_t k0 = k_own; k0 < blocks; k0 += down * kJoinLoads) {
+          F2 v[kJoinLoads];
+          load_join(v, part + c, p.C, k0, down, blocks);
+#pragma unroll
+          for (int u = 0; u < kJoinLoads; ++u) {
+            const uint32_t k = k0 + u * down;
+            if (k >= blocks) break;
+            const double rows = static_cast<double>(min(hi, (j0 + k + 1u) * p.R) - max(lo, (j0 + k) * p.R)), d = v[u].x - pivot;
+            v0 += rows * d;
+            v1 += v[u].y + rows * d * d;
+          }
         }
       }
     }
     double mean = 0, var = 0;
     if (blocks > 0u) {
-      v0 = sum_of_threads<kThreads>(v0, s_red) / count;
-      v1 = sum_of_threads<kThreads>(v1, s_red) / count;
+      sum_of_threads<kThreads>(v0, v1, s_red);
+      v0 *= inv_count, v1 *= inv_count;
       mean = pivot + v0, var = v1 - v0 * v0;
       if (var < 0) var = 0;
     }
     if (t == 0) {
       p.mean[unit] = static_cast<float>(mean);
-      p.rstd[unit] = static_cast<float>(1.0 / sqrt(var + static_cast<double>(p.eps)));
+      p.rstd[unit] = static_cast<float>(rsqrt(var + static_cast<double>(p.eps)));
     }
   } else {
     if (k_own < down) {
       for (uint32_t c = c_own; c < cpg; c += across) {
         const double w = p.w != nullptr ? load_param(p.w, p.param_dtype, g * cpg + c) : 1.f;
         double q0 = 0, q1 = 0;
-#pragma unroll 8
-        for (uint32_t k = k_own; k < blocks; k += down) {
-          const F2 v = part[size_t(k) * p.C + c];
-          q0 += v.x, q1 += v.y;
+        for (uint32_t k0 = k_own; k0 < blocks; k0 += down * kJoinLoads) {
+          F2 v[kJoinLoads];
+          load_join(v, part + c, p.C, k0, down, blocks);
+#pragma unroll
+          for (int u = 0; u < kJoinLoads; ++u) q0 += v[u].x, q1 += v[u].y;
         }
         v0 += w * q0;
         v1 += w * q1;
       }
     }
     if (blocks > 0u) {
-      v0 = sum_of_threads<kThreads>(v0, s_red) / count;
-      v1 = sum_of_threads<kThreads>(v1, s_red) / count;
+      sum_of_threads<kThreads>(v0, v1, s_red);
+      v0 *= inv_count, v1 *= inv_count;
     }
     if (t == 0) {
-      p.joined[unit * 2] = static_cast<float>(v0);
-      p.joined[unit * 2 + 1] = static_cast<float>(v1);
+      p.joined[size_t(unit) * 2] = static_cast<float>(v0);
+      p.joined[size_t(unit) * 2 + 1] = static_cast<float>(v1);
     }
   }
 }

@@ -819,11 +819,16 @@ __global__ void __launch_bounds__(kGrJoinThreads) grouped_join_kernel(const __gr
     for (uint32_t q = q0 + threadIdx.x; q < q1; q += kGrJoinThreads) {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (pieces > 0u) {
-        v = __ldcg(reinterpret_cast<const float4*>(from) + q);
-#pragma unroll 8
-        for (uint32_t k = 1; k < pieces; ++k) {
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(from + apart * k) + q);
-          v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+        // eight at a time on their way, also where there are fewer
+        for (uint32_t k0 = 0; k0 < pieces; k0 += 8u) {
+          float4 x[8];
+#pragma unroll
+          for (uint32_t u = 0; u < 8u; ++u) {
+            x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k0 + u < pieces) x[u] = __ldcg(reinterpret_cast<const float4*>(from + apart * (k0 + u)) + q);
+          }
+#pragma unroll
+          for (uint32_t u = 0; u < 8u; ++u) v.x += x[u].x, v.y += x[u].y, v.z += x[u].z, v.w += x[u].w;
         }
       }
       const uint32_t e = q * 4u;
