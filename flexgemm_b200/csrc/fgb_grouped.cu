@@ -804,9 +804,18 @@ __global__ void __launch_bounds__(kGrJoinThreads) grouped_join_kernel(const __gr
       if (m < static_cast<uint32_t>(p.m_extent)) {
         float v = 0.f;
         const float* share = p.db_parts + (size_t(first[g]) + tile) * p.tile_m + threadIdx.x;
-        for (uint32_t k = 0; k < pieces; ++k)
-#pragma unroll 4
-          for (int n = 0; n < p.n_tiles; ++n) v += share[(size_t(k) * z.tiles + n) * p.tile_m];
+        // eight at a time on their way
+        const uint32_t n_tiles = static_cast<uint32_t>(p.n_tiles), shares = pieces * n_tiles;
+        for (uint32_t i0 = 0; i0 < shares; i0 += 8u) {
+          float x[8];
+#pragma unroll
+          for (uint32_t u = 0; u < 8u; ++u) {
+            const uint32_t k = (i0 + u) / n_tiles, n = i0 + u - k * n_tiles;
+            x[u] = i0 + u < shares ? share[(size_t(k) * z.tiles + n) * p.tile_m] : 0.f;
+          }
+#pragma unroll
+          for (uint32_t u = 0; u < 8u; ++u) v += x[u];
+        }
         store_value(static_cast<T*>(p.db) + int64_t(g) * p.m_extent + m, v);
       }
     }
