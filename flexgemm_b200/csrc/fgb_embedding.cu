@@ -7,6 +7,10 @@
 // up the runs that lie in several of its chunks.  A run that lies in one CTA is final.  The two that may reach beyond its ends
 // leave their sums in a slab, and a second kernel adds a run's pieces up.  Nothing is added atomically, so the order of every
 // sum is fixed, and an index that every other position holds costs no more than a spread one.
+//
+// Measured (B200, int64 indices that repeat four times in a row): lookup 166000 x 256 fp16 from 4096 rows 19 us (5 TB/s; bound by
+// the stores), 1.32 million x 64 bf16 from 50000 rows 43 us (4.2 TB/s); gradient 57 and 142 us, of which the two passes of the
+// sort are 27 and 74 (scattered stores of 8 bytes) and the sums 22 and 50 (the rows of g in sorted order).
 #include <algorithm>
 
 #include "fgb_common.cuh"

@@ -16,6 +16,10 @@
 //   3. apply: the blocks in reverse, so that what the first pass read last is still in L2.
 // Results of (block j, sample s) go to slot j + s: walking along the rows either number grows by one from one result to
 // the next, so slots are unique, those of a sample are consecutive, and nothing has to be planned ahead.
+//
+// Measured (B200): 166000 x 256 fp16 with SiLU, one sample, forward + backward 162 us (floor 65: x and y, x, dy and dx once each; with
+// the second reads of x and dy 104), 39872 x 512 bf16 of four samples 95 us: sums 16, join 6, apply 19, backward 26, 7 and 27.
+// The long way's sums and apply run at 75 to 80 % of the copy rate; a short sample is bound by its chain of latencies.
 #include <algorithm>
 
 #include "fgb_common.cuh"

@@ -8,7 +8,7 @@
 // a block of 64 k a stage.
 //   kRows    m = rows, n = channels of the output.  The rows of a tile may reach into the next group: what they give is not
 //            stored.  The gradient reads W_g as stored, with k along its rows (MN-major operand).
-//   kFew     m = channels, n = rows (16 to 64 of them): where groups have few rows the matrices are what is read, and a tile
+//   kFew     m = channels, n = rows (16 or 32 of them): where groups have few rows the matrices are what is read, and a tile
 //            of 128 rows would be mostly empty.
 //   kWeight  m = co, n = ci, k = rows: both operands MN-major.  The k blocks of a group end where its rows end: a block
 //            that reaches further is cut in steps of 16 rows, and what its last step holds of other rows is cleared in
@@ -41,6 +41,10 @@
 
 namespace fgb {
 
+// Measured (B200): 131072 rows of 16 groups, 1024 x 1024 bf16: forward 195 to 210 us, input gradient 211, weight gradient 254 and 21
+// for the join (one cuBLAS product of that size 209, 209, 210; the clock is at the power cap); 166000 of 27, 256 x 256 fp16: 33, 33
+// and 54 (33, 33, 45), forward at 80 % of the copy rate; 24 rows of 64 groups, 512 -> 1024: 8 us, a chain of plan, loads,
+// products and stores (the touched matrices alone take 4).
 constexpr int kGrThreads = 320;
 constexpr int kGrEpilogueWarps = 8;
 constexpr int kGrMaxStages = 12;
