@@ -90,6 +90,7 @@ _PROTOTYPES = {
     "fgb_sparse_conv_wgrad": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int, _P, c_int64, _P, _P]),
     "fgb_sparse_conv_workspace_bytes": (c_int64, [c_int, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int]),
     "fgb_sample_offsets": (c_int, [_P, c_int64, c_int64, _P, _P, _P]),
+    "fgb_sample_offsets_host": (c_int, [_P, c_int64, c_int64, _P]),
     "fgb_group_norm_workspace_bytes": (c_int64, [_P]),
     "fgb_group_norm_forward": (c_int, [_P, _P]),
     "fgb_group_norm_backward": (c_int, [_P, _P]),

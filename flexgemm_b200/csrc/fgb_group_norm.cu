@@ -971,7 +971,18 @@ static int norm_call(const fgb_group_norm_call* c, bool backward, cudaStream_t s
 }
 
 // ------------------------------------------------------------------ row ranges of the samples
-// A row whose batch index is larger than the one before begins the samples in between; the last row ends those behind it.
+// A row whose batch index is larger than the one before begins the samples in between; the last row ends those behind it:
+// entries behind index `before`, up to `upto`.  Both may be any number (padding often has the largest one): they are cut to the
+// samples that there are before anything is added to them.
+struct OffsetEntries {
+  int first, last;
+};
+__host__ __device__ __forceinline__ OffsetEntries offset_entries(int before, int upto, int batch) {
+  const int b = before < -1 ? -1 : before > batch ? batch : before;
+  return OffsetEntries{b + 1, upto < batch ? upto : batch};
+}
+__host__ __device__ __forceinline__ bool batch_index_ok(int before, int b, int batch) { return b >= 0 && b < batch && b >= before; }
+
 __global__ void __launch_bounds__(256) sample_offsets_kernel(const int4* __restrict__ coords, uint32_t n, uint32_t batch, int32_t* __restrict__ offsets,
                                                              int32_t* status, int32_t* mirror) {
   chain_release();
@@ -982,15 +993,17 @@ __global__ void __launch_bounds__(256) sample_offsets_kernel(const int4* __restr
       for (uint32_t k = i; k <= batch; k += gridDim.x * 256u) offsets[k] = 0;
     return;
   }
-  const int b = __ldg(&coords[i]).x, before = i > 0u ? __ldg(&coords[i - 1u]).x : -1;
-  if (b < 0 || b >= static_cast<int>(batch) || b < before) {
+  const int b = __ldg(&coords[i]).x, before = i > 0u ? __ldg(&coords[i - 1u]).x : -1, most = static_cast<int>(batch);
+  if (!batch_index_ok(before, b, most)) {
     report(status, FGB_S_BAD_OFFSETS);
     mirror_code(mirror, FGB_S_BAD_OFFSETS);
   }
-  const int most = static_cast<int>(batch);
-  for (int k = max(before, -1) + 1; k <= min(b, most); ++k) offsets[k] = static_cast<int32_t>(i);
-  if (i == n - 1u)
-    for (int k = max(b, -1) + 1; k <= most; ++k) offsets[k] = static_cast<int32_t>(n);
+  const OffsetEntries begun = offset_entries(before, b, most);
+  for (int k = begun.first; k <= begun.last; ++k) offsets[k] = static_cast<int32_t>(i);
+  if (i == n - 1u) {
+    const OffsetEntries rest = offset_entries(b, most, most);
+    for (int k = rest.first; k <= rest.last; ++k) offsets[k] = static_cast<int32_t>(n);
+  }
 }
 
 }  // namespace fgb
@@ -1015,4 +1028,21 @@ extern "C" int fgb_sample_offsets(const int32_t* coords, int64_t n, int64_t batc
                                        reinterpret_cast<const int4*>(coords), static_cast<uint32_t>(n), static_cast<uint32_t>(batch), offsets, status,
                                        status_mirror(status));
   return e != cudaSuccess ? cuda_status(e) : launch_status();
+}
+
+// The kernel's rows one after the other, on host memory
+extern "C" int fgb_sample_offsets_host(const int32_t* coords, int64_t n, int64_t batch, int32_t* offsets) {
+  using namespace fgb;
+  if (n < 0 || n >= (int64_t(1) << 31) || batch < 1 || batch >= (int64_t(1) << 24)) return FGB_E_SIZE;
+  if (!offsets || (n > 0 && !coords)) return FGB_E_NULL;
+  const int most = static_cast<int>(batch);
+  int status = 0, before = -1;
+  for (int64_t i = 0; i <= n; ++i) {
+    const int b = i < n ? coords[i * 4] : most;  // what is behind the last row ends the samples that are left
+    if (i < n && !batch_index_ok(before, b, most)) status = FGB_S_BAD_OFFSETS;
+    const OffsetEntries e = offset_entries(before, b, most);
+    for (int k = e.first; k <= e.last; ++k) offsets[k] = static_cast<int32_t>(i);
+    before = b;
+  }
+  return status;
 }

@@ -730,6 +730,8 @@ int fgb_resize_rows(const void* src, void* dst, int64_t rows_in, int64_t rows_ou
  * that are grouped by ascending b, as the convolutions take and give them.
  * coords: int32 [n, 4], 16-byte aligned. */
 int fgb_sample_offsets(const int32_t* coords, int64_t n, int64_t batch, int32_t* offsets, int32_t* status, void* stream);
+/* The same on host memory, with the kernel's index arithmetic: 0, or FGB_S_BAD_OFFSETS where that would be recorded. */
+int fgb_sample_offsets_host(const int32_t* coords, int64_t n, int64_t batch, int32_t* offsets);
 
 /* Group norm, channels last: with mean m and variance v over the rows of a
  * sample and the c / groups channels of a group,

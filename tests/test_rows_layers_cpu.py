@@ -107,6 +107,38 @@ def test_sample_offsets_refuses(lib):
             sample_offsets(c, bad)
 
 
+def offsets_on_host(lib, batch_indices, batch):
+    """The entries, what is recorded, and whether all else was left alone."""
+    import numpy as np
+    coords = np.zeros((len(batch_indices), 4), np.int32)
+    coords[:, 0] = batch_indices
+    buffer = np.full(batch + 1 + 32, -7, np.int32)
+    entries = buffer[16:-16]
+    code = lib.fgb_sample_offsets_host(coords.ctypes.data, len(coords), batch, entries.ctypes.data)
+    return entries.tolist(), code, bool((buffer[:16] == -7).all() and (buffer[-16:] == -7).all())
+
+
+def test_sample_offsets_arithmetic(lib):
+    """The kernel's rows replayed on the host.  Batch indices at the ends of int32, as padding often has them: they are
+    recorded, and nothing is written but the entries (an index that is added to before it is cut would wrap, and write from
+    2^31 entries in front of them on)."""
+    low, high = -2 ** 31, 2 ** 31 - 1
+    for lengths in ([7], [0, 3, 0, 0, 9, 1, 0], [0, 0], [3] * 9):
+        rows = [b for b, k in enumerate(lengths) for _ in range(k)]
+        want = [sum(lengths[:b]) for b in range(len(lengths) + 1)]
+        assert offsets_on_host(lib, rows, len(lengths)) == (want, 0, True)
+    values = [low, low + 1, -2, -1, 0, 1, 2, 3, 4, 2 ** 24, high - 1, high]
+    for a in values:
+        for b in values:
+            for rows in ([a], [a, b], [0, a, b], [a, b, 1], [a, 0, b]):
+                entries, code, alone = offsets_on_host(lib, rows, 3)
+                good = rows == sorted(rows) and rows[0] >= 0 and rows[-1] < 3
+                assert alone and code == (0 if good else _cabi.S_BAD_OFFSETS), rows
+                assert all(0 <= e <= len(rows) for e in entries), rows
+    assert offsets_on_host(lib, [0, 1, high, high], 2) == ([0, 1, 2], _cabi.S_BAD_OFFSETS, True)
+    assert lib.fgb_sample_offsets_host(None, 1, 1, None) == -1 and lib.fgb_sample_offsets_host(None, 0, 0, None) == -2
+
+
 class NormCall(ctypes.Structure):
     _fields_ = [(k, ctypes.c_void_p) for k in ("x", "grad_out", "out", "offsets", "weight", "bias", "mean", "rstd", "grad_weight", "grad_bias")] + \
                [("n", ctypes.c_int64), ("samples", ctypes.c_int64)] + \
