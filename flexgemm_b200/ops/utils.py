@@ -56,11 +56,21 @@ def sample_offsets(coords: torch.Tensor, batch: int) -> torch.Tensor:
         raise ValueError(f"1 to 2^24 - 1 samples are supported, got {batch}")
     if coords.shape[0] >= 2 ** 31:
         raise ValueError("at most 2^31 - 1 rows are supported")
+    coords = _int32_coords(coords, batch)
     require_cuda(coords, "coords")
     out = _native.ext().sample_offsets(coords, batch)
     if out is None:
-        out = _native.ext().sample_offsets(kernel_layout(coords.int()), batch)
+        out = _native.ext().sample_offsets(kernel_layout(coords), batch)
     return out
+
+
+def _int32_coords(coords: torch.Tensor, batch: int) -> torch.Tensor:
+    """Other integers are cut to the samples before they are cast: one of 2^32 must not come out as sample 0."""
+    if coords.dtype == torch.int32:
+        return coords
+    if coords.dtype not in (torch.int64, torch.int16, torch.int8, torch.uint8):
+        raise TypeError(f"unsupported coords dtype {coords.dtype}: expected int32")
+    return (coords.clamp(-1, batch) if coords.dtype == torch.int64 else coords).int()
 
 
 def require_cuda(t: torch.Tensor, name: str = "feats") -> None:

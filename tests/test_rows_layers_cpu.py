@@ -107,6 +107,18 @@ def test_sample_offsets_refuses(lib):
             sample_offsets(c, bad)
 
 
+def test_sample_offsets_of_other_types(lib):
+    from flexgemm_b200.ops import utils
+    for dtype in (torch.float32, torch.float16, torch.bool):
+        with pytest.raises(TypeError):
+            utils.sample_offsets(torch.zeros(5, 4, dtype=dtype), 1)
+    b = [-2 ** 40, -2 ** 32, -1, 0, 1, 2, 3, 2 ** 31, 2 ** 32, 2 ** 32 + 1, 2 ** 63 - 1]
+    got = utils._int32_coords(torch.tensor(b).view(-1, 1).expand(-1, 4), 3)
+    assert got.dtype == torch.int32 and got[:, 0].tolist() == [-1, -1, -1, 0, 1, 2, 3, 3, 3, 3, 3]
+    for dtype in (torch.int16, torch.int8, torch.uint8):
+        assert utils._int32_coords(torch.tensor([[0, 1, 2, 3]], dtype=dtype), 1).tolist() == [[0, 1, 2, 3]]
+
+
 def offsets_on_host(lib, batch_indices, batch):
     """The entries, what is recorded, and whether all else was left alone."""
     import numpy as np
