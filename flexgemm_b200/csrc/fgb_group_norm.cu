@@ -167,6 +167,80 @@ struct ChannelParams {
   __device__ __forceinline__ F2 z(F2 h, int i) const { return fma2(h, w[i], b[i]); }
 };
 
+// Mean and squared distance from it of the rows r, r + lanes, ... below `end` (px: row r), channel by channel; returns their number.
+// What cancels in sum d^2 - (sum d)^2 / n grows with n and with the distance of the pivot, from which d is taken, to the mean:
+// with the first row as the pivot of all, an outlier there, or zeros in front of a large mean, cost the variance of 50000 rows 4e-3 of
+// its value.  So the first row is the pivot of eight rows, and the mean so far, which an outlier among them moves by an eighth, that of
+// the next kRunRows, and so on.  The squared distance of the rows before a run waits in shared memory (`park`, a place of the thread's own
+// for each pair): 8 registers that the loop of 16-bit packs of eight does not have.
+constexpr uint32_t kBatchRows = 8, kRunRows = 64;
+template <typename T, int kVec>
+__device__ __forceinline__ float moments_of_rows(const T* px, uint32_t r, uint32_t end, uint32_t lanes, size_t step, F2 (&mean)[Pairs<T, kVec>::kPairs],
+                                                 F2 (&m2)[Pairs<T, kVec>::kPairs], F2* park) {
+  using Ch = Channels<T, kVec>;
+  using Raw = typename Ch::Raw;
+  using P = Pairs<T, kVec>;
+  constexpr int kPairs = P::kPairs;
+  if (r >= end) return 0.f;
+  uint32_t left = (end - r + lanes - 1u) / lanes;
+  float n = 0.f;
+  F2 minus_pivot[kPairs];
+  {
+    P pivot;
+    pivot.unpack(Ch::load(px));
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) minus_pivot[i] = neg2(pivot.v[i]);
+  }
+  while (left > 0u) {
+    const uint32_t rows = min(left, n == 0.f ? kBatchRows : kRunRows);
+    F2 sum0[kPairs], sum1[kPairs];
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) sum0[i] = sum1[i] = both(0.f);
+    auto add = [&](const Raw& raw) {
+      P v;
+      v.unpack(raw);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        const F2 d = add2(v.v[i], minus_pivot[i]);
+        sum0[i] = add2(sum0[i], d);
+        sum1[i] = fma2(d, d, sum1[i]);
+      }
+    };
+    uint32_t k = 0;
+    for (; k + kBatchRows <= rows; k += kBatchRows, px += kBatchRows * step) {
+      Raw raw[kBatchRows];
+#pragma unroll
+      for (uint32_t u = 0; u < kBatchRows; ++u) raw[u] = Ch::load(px + u * step);
+#pragma unroll
+      for (uint32_t u = 0; u < kBatchRows; ++u) add(raw[u]);
+    }
+#pragma unroll 4
+    for (; k < rows; ++k, px += step) add(Ch::load(px));
+    left -= rows;
+    // the run's mean lies `d` from the pivot; its squared distance is not below zero (a NaN stays)
+    const float count = static_cast<float>(rows), total = n + count, inv = __fdividef(1.f, count), share = n == 0.f ? 1.f : __fdividef(count, total);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const F2 d = mul2(sum0[i], both(inv)), w = fma2(neg2(sum0[i]), d, sum1[i]);
+      F2 before = F2{w.x < 0.f ? 0.f : w.x, w.y < 0.f ? 0.f : w.y};
+      if (n > 0.f) before = fma2(mul2(d, d), both(n * share), add2(park[i * kNormThreads], before));
+      park[i * kNormThreads] = before;
+      minus_pivot[i] = fma2(neg2(d), both(share), minus_pivot[i]);
+    }
+    n = total;
+  }
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) mean[i] = neg2(minus_pivot[i]), m2[i] = park[i * kNormThreads];
+  return n;
+}
+// Joins the rows of (mean, m2, n) with those of (mean_b, m2_b, n_b), of which there are none where n_b is zero
+__device__ __forceinline__ void join_moments(F2& mean, F2& m2, float n, F2 mean_b, F2 m2_b, float n_b) {
+  const float share = __fdividef(n_b, n + n_b);  // exact to two last bits, as good as the products that follow
+  const F2 d = add2(mean_b, neg2(mean));
+  mean = fma2(d, both(share), mean);
+  m2 = fma2(mul2(d, d), both(n * share), add2(m2, m2_b));
+}
+
 // ------------------------------------------------------------------ 1. sums
 template <typename T, int kVec, bool kOne, bool kBackward, bool kSilu>
 __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_sums_kernel(const NormArgs p) {
@@ -176,6 +250,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_sums_kernel(cons
   constexpr bool kExact = sizeof(T) == 4;
   constexpr int kPairs = P::kPairs;
   __shared__ F2 s_sum[2 * kPairs][kNormThreads];
+  __shared__ float s_rows[kNormThreads];
   chain_release();
   chain_wait();
   if constexpr (!kBackward) p.ranges.check(p.status, p.mirror);
@@ -195,38 +270,14 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_sums_kernel(cons
   const T* dy = static_cast<const T*>(p.dy) + c0;
   for (uint32_t s = first; s <= last; ++s) {
     const uint32_t lo = max(p.ranges.at(s), row0), hi = min(p.ranges.at(s + 1u), row1);
-    F2 sum0[kPairs], sum1[kPairs], minus_pivot[kPairs];
+    F2 sum0[kPairs], sum1[kPairs];  // forward: mean and squared distance from it
+    float rows = 0.f;               // forward: that they are of
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) sum0[i] = sum1[i] = minus_pivot[i] = both(0.f);
+    for (int i = 0; i < kPairs; ++i) sum0[i] = sum1[i] = both(0.f);
     if (lo < hi && active) {
       const size_t step = size_t(lanes) * p.C;
       if constexpr (!kBackward) {
-        // distances from the range's first row: what cancels in sum1 - sum0^2 / n is at most its share of the rows
-        P pivot;
-        pivot.unpack(Ch::load(x + size_t(lo) * p.C));
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) minus_pivot[i] = neg2(pivot.v[i]);
-        auto add = [&](const Raw& raw) {
-          P v;
-          v.unpack(raw);
-#pragma unroll
-          for (int i = 0; i < kPairs; ++i) {
-            const F2 d = add2(v.v[i], minus_pivot[i]);
-            sum0[i] = add2(sum0[i], d);
-            sum1[i] = fma2(d, d, sum1[i]);
-          }
-        };
-        constexpr int kRows = 8;
-        uint32_t r = lo + ry;
-        const T* px = x + size_t(r) * p.C;
-        for (; r + (kRows - 1u) * lanes < hi; r += kRows * lanes, px += kRows * step) {
-          Raw raw[kRows];
-#pragma unroll
-          for (int u = 0; u < kRows; ++u) raw[u] = Ch::load(px + u * step);
-#pragma unroll
-          for (int u = 0; u < kRows; ++u) add(raw[u]);
-        }
-        for (; r < hi; r += lanes, px += step) add(Ch::load(px));
+        rows = moments_of_rows<T, kVec>(x + size_t(lo + ry) * p.C, lo + ry, hi, lanes, step, sum0, sum1, &s_sum[0][threadIdx.x]);
       } else {
         k.load_stats(p, s, c0);
         auto add = [&](const Raw& raw, const Raw& raw_dy) {
@@ -261,30 +312,27 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_sums_kernel(cons
       if (active && ry >= half && ry < m) {
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) s_sum[i][threadIdx.x] = sum0[i], s_sum[kPairs + i][threadIdx.x] = sum1[i];
+        if constexpr (!kBackward) s_rows[threadIdx.x] = rows;
       }
       __syncthreads();
       if (ry < m - half) {
         const int from = threadIdx.x + half * width;
+        if constexpr (kBackward) {
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) sum0[i] = add2(sum0[i], s_sum[i][from]), sum1[i] = add2(sum1[i], s_sum[kPairs + i][from]);
+          for (int i = 0; i < kPairs; ++i) sum0[i] = add2(sum0[i], s_sum[i][from]), sum1[i] = add2(sum1[i], s_sum[kPairs + i][from]);
+        } else if (s_rows[from] > 0.f) {
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) join_moments(sum0[i], sum1[i], rows, s_sum[i][from], s_sum[kPairs + i][from], s_rows[from]);
+          rows += s_rows[from];
+        }
       }
       __syncthreads();
       m = half;
     }
     if (ry == 0) {
       F2* out = p.part + size_t(j + s) * p.C + c0;
-      const float n = lo < hi ? static_cast<float>(hi - lo) : 1.f;
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        const float v0 = i % 2 ? sum0[i / 2].y : sum0[i / 2].x, v1 = i % 2 ? sum1[i / 2].y : sum1[i / 2].x;
-        if constexpr (kBackward) {
-          out[i] = F2{v0, v1};
-        } else {
-          const float d = v0 / n, within = fmaf(-v0, d, v1);
-          // mean and squared distance from it (not below zero; a NaN stays)
-          out[i] = F2{d - (i % 2 ? minus_pivot[i / 2].y : minus_pivot[i / 2].x), within < 0.f ? 0.f : within};
-        }
-      }
+      for (int i = 0; i < kVec; ++i) out[i] = F2{i % 2 ? sum0[i / 2].y : sum0[i / 2].x, i % 2 ? sum1[i / 2].y : sum1[i / 2].x};
     }
   }
 }
@@ -525,8 +573,9 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_small_kernel(con
   using P = Pairs<T, kVec>;
   constexpr bool kExact = sizeof(T) == 4;
   constexpr int kPairs = P::kPairs;
-  extern __shared__ F2 s_mem[];  // of each team: sums [C], statistics [G], backward: columns [C]
+  extern __shared__ F2 s_mem[];  // of each team: sums [C] (forward: mean and squared distance from it), statistics [G], backward: columns [C]
   __shared__ F2 s_sum[2 * kPairs][kNormThreads];
+  __shared__ float s_rows[kNormThreads];
   chain_release();
   chain_wait();
   p.ranges.check(p.status, p.mirror);
@@ -558,6 +607,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_small_kernel(con
       const int width = min(size, packs - pack0), lanes = size / width;
       const int cx = t % width, ry = t / width, c0 = (pack0 + cx) * kVec;
       F2 sum0[kPairs], sum1[kPairs];
+      float rows = 0.f;
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) sum0[i] = sum1[i] = both(0.f);
       if (ry < lanes && from < to) {
@@ -565,29 +615,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_small_kernel(con
         uint32_t r = from + ry;
         const T* px = x + size_t(r) * p.C + c0;
         if constexpr (!kBackward) {
-          // distances from the sample's first row, the same for all CTAs
-          P pivot;
-          pivot.unpack(Ch::load(x + size_t(lo) * p.C + c0));
-          auto add = [&](const Raw& raw) {
-            P v;
-            v.unpack(raw);
-#pragma unroll
-            for (int i = 0; i < kPairs; ++i) {
-              const F2 d = add2(v.v[i], neg2(pivot.v[i]));
-              sum0[i] = add2(sum0[i], d);
-              sum1[i] = fma2(d, d, sum1[i]);
-            }
-          };
-          constexpr int kRows = 8;
-          for (; r + (kRows - 1u) * lanes < to; r += kRows * lanes, px += kRows * step) {
-            Raw raw[kRows];
-#pragma unroll
-            for (int u = 0; u < kRows; ++u) raw[u] = Ch::load(px + u * step);
-#pragma unroll
-            for (int u = 0; u < kRows; ++u) add(raw[u]);
-          }
-#pragma unroll 4
-          for (; r < to; r += lanes, px += step) add(Ch::load(px));
+          rows = moments_of_rows<T, kVec>(px, r, to, lanes, step, sum0, sum1, &s_sum[0][threadIdx.x]);
         } else {
           ChannelParams<kVec, kOne> k;
           k.load(p, c0);
@@ -622,12 +650,19 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_small_kernel(con
         if (ry >= half && ry < m) {
 #pragma unroll
           for (int i = 0; i < kPairs; ++i) s_sum[i][threadIdx.x] = sum0[i], s_sum[kPairs + i][threadIdx.x] = sum1[i];
+          if constexpr (!kBackward) s_rows[threadIdx.x] = rows;
         }
         sync();
         if (ry < m - half) {
           const int at = threadIdx.x + half * width;
+          if constexpr (kBackward) {
 #pragma unroll
-          for (int i = 0; i < kPairs; ++i) sum0[i] = add2(sum0[i], s_sum[i][at]), sum1[i] = add2(sum1[i], s_sum[kPairs + i][at]);
+            for (int i = 0; i < kPairs; ++i) sum0[i] = add2(sum0[i], s_sum[i][at]), sum1[i] = add2(sum1[i], s_sum[kPairs + i][at]);
+          } else if (s_rows[at] > 0.f) {
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) join_moments(sum0[i], sum1[i], rows, s_sum[i][at], s_sum[kPairs + i][at], s_rows[at]);
+            rows += s_rows[at];
+          }
         }
         sync();
         m = half;
@@ -641,16 +676,10 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_small_kernel(con
     sync();
     if (q.cluster > 1) cluster_sync_all();
     // 2. the groups: a thread adds up a group, over the channels and the CTAs
-    auto total = [&](int c) {
-      F2 v = sums[c];
-      if (q.cluster > 1) {
-        v = both(0.f);
-        for (int i = 0; i < q.cluster; ++i) {
-          float2 w;
-          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(w.x), "=f"(w.y) : "r"(cluster_map(smem_u32(&sums[c]), i)) : "memory");
-          v = add2(v, F2{w.x, w.y});
-        }
-      }
+    auto sum_of = [&](int c, int i) {  // CTA i's
+      if (q.cluster == 1) return sums[c];
+      F2 v;
+      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_map(smem_u32(&sums[c]), i)) : "memory");
       return v;
     };
     // lanes that share a group: as many as it has channels, up to a warp's
@@ -661,19 +690,21 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_small_kernel(con
       const int g = min(g0, p.G - 1);
       double v0 = 0, v1 = 0;
       if constexpr (!kBackward) {
-        // as the joins of the longer way: the first channel's mean is the pivot of the channels' means
-        const double inv_n = 1.0 / len;
-        const double pivot = has ? static_cast<double>(static_cast<float>(x[size_t(lo) * p.C + g * p.cpg])) : 0.0;
+        // as the joins of the longer way: the first channel's mean is the pivot of the means of channels and CTAs
+        const double inv_n = inv_cpg / len;
+        const double pivot = has ? sum_of(g * p.cpg, 0).x : 0.f;
         for (int i = t % across; i < p.cpg && has; i += across) {
-          const int c = g * p.cpg + i;
-          const F2 v = total(c);
-          const double mean = static_cast<double>(v.x) * inv_n, within = static_cast<double>(v.y) - v.x * mean;
-          const double d = static_cast<double>(static_cast<float>(x[size_t(lo) * p.C + c])) + mean - pivot;
-          v0 += d;
-          v1 += (within < 0 ? 0.0 : within) * inv_n + d * d;  // a NaN stays
+#pragma unroll 4
+          for (int k = 0; k < q.cluster; ++k) {  // all on their way at once: a CTA without rows has zeros
+            const uint32_t begin = min(len, k * share), rows = min(len, begin + share) - begin;
+            const F2 v = sum_of(g * p.cpg + i, k);
+            const double d = v.x - pivot;
+            v0 += rows * d;
+            v1 += v.y + rows * d * d;
+          }
         }
         for (int d = across / 2; d > 0; d >>= 1) v0 += __shfl_xor_sync(0xffffffffu, v0, d), v1 += __shfl_xor_sync(0xffffffffu, v1, d);
-        v0 *= inv_cpg, v1 *= inv_cpg;
+        v0 *= inv_n, v1 *= inv_n;
         const double var = v1 - v0 * v0 < 0 || !has ? 0.0 : v1 - v0 * v0;
         if (t % across == 0 && g0 < p.G) {
           const F2 st{has ? static_cast<float>(pivot + v0) : 0.f, 1.f / sqrtf(static_cast<float>(var + static_cast<double>(p.eps)))};
@@ -683,7 +714,8 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_small_kernel(con
       } else {
         for (int i = t % across; i < p.cpg && has; i += across) {
           const int c = g * p.cpg + i;
-          const F2 v = total(c);
+          F2 v = sum_of(c, 0);
+          for (int k = 1; k < q.cluster; ++k) v = add2(v, sum_of(c, k));
           const double w = p.w != nullptr ? load_param(p.w, p.param_dtype, c) : 1.f;
           v0 += w * v.x;
           v1 += w * v.y;
