@@ -25,7 +25,8 @@
 // sizes alone, so results do not depend on the run.
 //
 // fp32 operands are written as sums of bf16 planes (hi + mid + lo, 8 bits each) and multiplied plane by plane: six products
-// (all whose weight is 2^-16 and more) for accurate fp32, three (2^-8 and more) where TF32 is allowed.  bf16 has
+// (all whose weight is 2^-16 and more) for accurate fp32, three (2^-8 and more) where TF32 is allowed.  A plane leaves half a step of
+// eight bits, 2^-8, of what it takes, so that four terms of 2^-24 of a product are left out, or three of 2^-16.  bf16 has
 // fp32's range, so no scaling is needed, and six of them cost what three TF32 products do (half the rate, twice the bytes).
 // The tensor cores cut what they add to an accumulator at its last bit instead of rounding: over a long k that is a bias
 // (2e-8 of the sum for every 16 k; 1e-5 where k was 10^5).  So fp32 leaves the accumulator after each block of 64 k, the small

@@ -796,9 +796,9 @@ int fgb_embedding_backward(const fgb_embedding_call* call, void* stream);
  *   backward  grad_x[r] = weight[g]^T grad_out[r]
  *             grad_weight[g] = sum_r grad_out[r] x[r]^T,   grad_bias[g] = sum_r grad_out[r]
  * fp32 accumulation, the bias added in fp32, one rounding.  fp32 data is
- * multiplied as sums of bf16 planes: FGB_F32_IEEE six products (errors of some
- * 2^-22 of a product), FGB_F32_TF32 three (2^-17); an infinity among fp32
- * operands gives NaN.  Gradients that are null are not computed; grad_bias needs
+ * multiplied as sums of bf16 planes: FGB_F32_IEEE six products (a product is off
+ * by less than 2^-21 of its value), FGB_F32_TF32 three (3 * 2^-16); an infinity
+ * among fp32 operands gives NaN.  Gradients that are null are not computed; grad_bias needs
  * grad_weight.  groups <= fgb_grouped_linear_max_groups(). */
 typedef struct fgb_grouped_linear_call {
   const void* x;           /* [n, ci] */
