@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
   const int half = kPair ? p.bn / 2 : p.bn;  // columns whose operand this CTA holds
   const uint32_t workers = kPair ? gridDim.x / 2u : gridDim.x, worker = kPair ? blockIdx.x / 2u : blockIdx.x;
   volatile uint32_t* abort_flag = &ctl->abort_flag;
-  auto wait = [&](uint64_t* bar, uint32_t parity) { mbar_wait_tries(bar, parity, abort_flag); };
+  auto wait = [&](uint64_t* bar, uint32_t parity) { mbar_wait(bar, parity, abort_flag); };
 
   chain_release();
   if (tid == 0) {

@@ -367,6 +367,31 @@ __global__ void __launch_bounds__(kMbThreads, 1) microbench_kernel(const __grid_
   if (tid == 0 && ctl->abort_flag) report(p.status, FGB_S_WAIT_TIMEOUT);
 }
 
+// A wait on a barrier that nothing completes, and then another one: how long they take, what they say, and how long one
+// try is suspended.  One warp; the waits are bounded.
+__global__ void __launch_bounds__(32) microbench_wait_kernel(int kind, unsigned long long* out, int32_t* status) {
+  __shared__ uint64_t s_bar;
+  __shared__ uint32_t s_abort;
+  if (threadIdx.x == 0) {
+    mbar_init(&s_bar, 1);
+    s_abort = 0;
+    mbar_init_fence();
+  }
+  __syncwarp();
+  if (threadIdx.x != 0) return;
+  auto wait = [&]() { return kind == FGB_MB_WAIT_CLUSTER ? mbar_wait_cluster(&s_bar, 0, &s_abort) : mbar_wait(&s_bar, 0, &s_abort); };
+  constexpr int kTries = 64;
+  const uint64_t t0 = global_timer_ns();
+  for (int i = 0; i < kTries && !mbar_try_wait(&s_bar, 0); ++i) {}  // each behind the answer of the one before, as in a wait
+  const uint64_t t1 = global_timer_ns();
+  const bool first = wait();
+  const uint64_t t2 = global_timer_ns();
+  const bool second = wait();
+  const uint64_t t3 = global_timer_ns();
+  out[0] = t2 - t1, out[1] = t3 - t2, out[2] = (first ? 1u : 0u) + (second ? 2u : 0u), out[3] = (t1 - t0) / kTries;
+  if (s_abort != 0u) report(status, FGB_S_WAIT_TIMEOUT);
+}
+
 }  // namespace
 }  // namespace fgb
 
@@ -453,5 +478,21 @@ extern "C" int fgb_microbench_pipeline(int mode, int stages_a, int stages_b, int
   if (e0) cudaEventDestroy(e0);
   if (e1) cudaEventDestroy(e1);
   if (d_counters) cudaFree(d_counters);
+  return rc;
+}
+
+extern "C" int fgb_microbench_wait(int kind, uint64_t* out, int32_t* status, void* stream) {
+  using namespace fgb;
+  if (!out || !status) return FGB_E_NULL;
+  if (kind != FGB_MB_WAIT_CTA && kind != FGB_MB_WAIT_CLUSTER) return FGB_E_SIZE;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  unsigned long long h[4] = {}, *d = nullptr;
+  int rc = cuda_status(cudaMalloc(&d, sizeof(h)));
+  if (rc != FGB_OK) return rc;
+  rc = cuda_status(launch(microbench_wait_kernel, dim3(1), dim3(32), 0, s, kind, d, status));
+  if (rc == FGB_OK) rc = cuda_status(cudaMemcpyAsync(h, d, sizeof(h), cudaMemcpyDeviceToHost, s));
+  if (rc == FGB_OK) rc = cuda_status(cudaStreamSynchronize(s));
+  cudaFree(d);
+  for (int i = 0; i < 4; ++i) out[i] = h[i];
   return rc;
 }

@@ -54,7 +54,9 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 }
 // Bounded wait.  A wait that is still pending after kWaitNs of wall time gives
 // up, and raises `abort_flag` (shared memory) so that every later wait of the
-// CTA returns at once and the CTA drains quickly.
+// CTA returns at once and the CTA drains quickly.  (The hardware suspends a try
+// while the phase is pending, 4 us where nothing ends it: a number of tries
+// bounds no time, and a wait on its ordinary way seldom comes to the clock.)
 constexpr uint64_t kWaitNs = 1000000000ull;  // 1 s; legitimate waits last microseconds
 __device__ __forceinline__ uint64_t global_timer_ns() {
   uint64_t t;
@@ -129,21 +131,6 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
       }
     }
   }
-}
-
-// Bounded by a number of tries instead of the time: no clock is read on the way.  A try is suspended by the hardware while the
-// phase is pending, for some ten nanoseconds at least, so 2^26 of them are most of a second.
-__device__ __forceinline__ bool mbar_wait_tries(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag) {
-  for (uint32_t i = 1; !mbar_try_wait(bar, parity); ++i) {
-    if ((i & 63u) == 0u) {
-      if (*abort_flag) return false;
-      if (i >= (1u << 26)) {
-        *abort_flag = 1u;
-        return false;
-      }
-    }
-  }
-  return true;
 }
 
 // ------------------------------------------------------------------ proxies / fences

@@ -414,6 +414,18 @@ def microbench_pipeline(mode: int, rows: torch.Tensor, dense: torch.Tensor, iter
     return float(ms.value), [int(c) for c in counters]
 
 
+def microbench_wait(kind: int, device: torch.device):
+    """A barrier wait that nothing ends (``fgb_microbench_wait``; ``kind`` 0: of a CTA, 1: of a cluster).  Returns the nanoseconds of the
+    wait and of the next one, which of them said that the barrier was complete (bits), and the nanoseconds of one try; the
+    status word of the device holds ``S_WAIT_TIMEOUT`` afterwards."""
+    import ctypes
+    out = (ctypes.c_uint64 * 4)()
+    with torch.cuda.device(device):
+        rc = _cabi.lib().fgb_microbench_wait(int(kind), out, status_word(device).data_ptr(), _stream(device))
+    _cabi.check(rc, "fgb_microbench_wait")
+    return tuple(int(v) for v in out)
+
+
 def set_conv_dgrad_relayout(on: bool) -> bool:
     """Force dgrad onto the re-laid-out copy of the weight (the path of the 32-bit types) for every type; returns the
     previous setting.  The default reads 16-bit weights as stored."""

@@ -874,6 +874,16 @@ int fgb_microbench_pipeline(int mode, int stages_a, int stages_b, int iters, int
                             const void* dense, int64_t dense_bytes,
                             float* ms_out, uint64_t* counters, int32_t* status, void* stream);
 
+/* A barrier wait of the kernels that nothing ends, once in one warp: it gives up
+ * after a second, and FGB_S_WAIT_TIMEOUT is recorded in *status.  `kind`: on a
+ * barrier of the CTA's own (CTA), or one that another CTA of the cluster may
+ * arrive on (CLUSTER).  out (host, [4]): nanoseconds of the wait; of a second wait
+ * after it, which returns at once; which of the two said that the barrier was
+ * complete (bits; 0); nanoseconds of one try.  The call synchronises. */
+#define FGB_MB_WAIT_CTA 0
+#define FGB_MB_WAIT_CLUSTER 1
+int fgb_microbench_wait(int kind, uint64_t* out, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
