@@ -91,6 +91,7 @@ struct GroupedSmem {
   uint64_t full[kGrMaxStages], empty[kGrMaxStages];
   uint64_t peer_full[kGrMaxStages];  // pairs: the other CTA has cleared its operands of a stage
   uint64_t acc_full[2], acc_empty[2];
+  uint64_t drained;  // only after a wait that gave up: the products in flight
   uint32_t tmem_base, abort_flag;
 };
 
@@ -313,6 +314,25 @@ __device__ __forceinline__ void store_columns(uint32_t (&acc)[32], uint8_t* stag
   }
 }
 
+// After a wait that gave up: what is in flight is waited for, with a limit of its own.  Not inlined: nothing comes here otherwise.
+// The copies of the last blocks; those of a pair's second CTA count on the leader's barriers, and get a time in which copies end.
+__noinline__ __device__ void drain_copies(GroupedSmem* ctl, uint32_t stages, uint32_t issued, uint32_t rank) {
+  if (rank == 0u) {
+    uint32_t late = 0;
+    for (uint32_t b = issued - min(issued, stages); b != issued; ++b) mbar_wait(&ctl->full[b % stages], b / stages & 1u, &late);
+  } else {
+    for (const uint64_t t0 = global_timer_ns(); global_timer_ns() - t0 < 100000u;) __nanosleep(1000);
+  }
+}
+template <bool kPair>
+__noinline__ __device__ void drain_products(GroupedSmem* ctl) {
+  uint32_t late = 0;
+  const uint32_t bar = smem_u32(&ctl->drained);
+  if constexpr (kPair) umma_commit_pair(cluster_map(bar, 0));
+  else umma_commit(bar);
+  mbar_wait(&ctl->drained, 0, &late);
+}
+
 // kPair: launched as clusters of two CTAs, which work on tiles of 256 rows together: each loads its 128 rows and half of the
 // columns, the first CTA (the leader) issues products over both CTAs' operands, each gets its rows' accumulators.  A CTA loads
 // 32 KB a stage instead of 48 for the same products: with one CTA a tile L2's rate to the SMs was the bound.
@@ -341,7 +361,9 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
   const int half = kPair ? p.bn / 2 : p.bn;  // columns whose operand this CTA holds
   const uint32_t workers = kPair ? gridDim.x / 2u : gridDim.x, worker = kPair ? blockIdx.x / 2u : blockIdx.x;
   volatile uint32_t* abort_flag = &ctl->abort_flag;
-  auto wait = [&](uint64_t* bar, uint32_t parity) { mbar_wait(bar, parity, abort_flag); };
+  // A wait that gives up raises the CTA's abort flag: no load is issued after that, products run on what is there, nothing is
+  // stored, and what is in flight is waited for (again with a limit).
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag); };
 
   chain_release();
   if (tid == 0) {
@@ -354,6 +376,7 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
       mbar_init(&ctl->acc_full[a], 1);
       mbar_init(&ctl->acc_empty[a], kPair ? 2 * kGrEpilogueWarps : kGrEpilogueWarps);
     }
+    mbar_init(&ctl->drained, 1);
     ctl->abort_flag = 0;
     mbar_init_fence();
   }
@@ -395,7 +418,8 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
   if (warp == 8) {
     // ------------------------------------------------------------------ loads
     // One elected lane goes through all blocks of a unit (elect picks the same lane each time).
-    uint32_t s = 0, ph = 0;
+    uint32_t s = 0, ph = 0, issued = 0;
+    bool stopped = false;
     const int G = static_cast<int>(p.ranges.count);
     const uint32_t full_own = smem_u32(&ctl->full[0]), full_leader = kPair ? cluster_map(full_own, 0) : full_own;
     while (walk.next(it)) {
@@ -406,7 +430,10 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
         const int k_end = static_cast<int>(it.to * 64u);
         for (int k0 = static_cast<int>(it.from * 64u); k0 < k_end; k0 += 64) {
           const bool cleared = kMode == kWeight && k0 + 64 > len && (len & 15) != 0;  // see the products
-          wait(&ctl->empty[s], ph ^ 1);
+          if (stopped || !wait(&ctl->empty[s], ph ^ 1)) {
+            stopped = true;
+            break;
+          }
           // Pairs: both CTAs' bytes count on the leader's barrier, so that it has one to wait for -- but for a block that
           // either has to clear rows of first.
           const bool shared = kPair && !cleared;
@@ -439,10 +466,13 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
             }
           }
           if (++s == static_cast<uint32_t>(p.stages)) s = 0, ph ^= 1;
+          ++issued;
         }
       }
       __syncwarp();
     }
+    if (elect_one() && *abort_flag != 0u) drain_copies(ctl, static_cast<uint32_t>(p.stages), issued, rank);
+    __syncwarp();
   } else if (warp == 9) {
     // ------------------------------------------------------------------ products
     // One elected lane goes through all blocks of a unit and carries the ring's and the accumulators' state; the descriptors
@@ -558,6 +588,8 @@ __global__ void __launch_bounds__(kGrThreads, 1) grouped_kernel(const __grid_con
       }
       done += n_blocks;
     }
+    if (leader && elect_one() && *abort_flag != 0u) drain_products<kPair>(ctl);
+    __syncwarp();
   } else {
     // ------------------------------------------------------------------ stores
     const int quarter = warp & 3, group = warp >> 2;
