@@ -16,6 +16,7 @@
 #include "fgb_common.cuh"
 #include "fgb_device.cuh"
 #include "fgb_rows.cuh"
+#include "fgb_sort.cuh"
 
 namespace fgb {
 
@@ -114,6 +115,7 @@ struct EmbInfo {
   uint32_t flags;  // kGoesOn: the run of the last position goes on behind the CTA; kThrough: it began before the CTA, too
 };
 constexpr uint32_t kGoesOn = 1u, kThrough = 2u;
+constexpr uint32_t kNoKey = 0xFFFFFFFFu;  // before the first position and behind the last one
 
 struct EmbGrad {
   const void* g;
@@ -127,47 +129,23 @@ struct EmbGrad {
   float scale;
 };
 
-template <typename T, int kVec>
-__global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const EmbGrad p) {
+// Sums over `count` sorted positions, in shared memory with their keys (s_key[-1] and s_key[count]: the keys before and behind them), of the
+// channels of the packs pack0 .. pack1 - 1: `lanes` groups of `width` threads take a chunk each.  s_head: of each group's chunk the sum of the run
+// that began before it, s_through: whether that run goes on behind it.  slab: for the runs that leave the positions.  The whole CTA calls it.
+template <typename T, int kVec, int kThreads, typename Pos>
+__device__ __forceinline__ void embedding_runs(const EmbGrad& p, const uint32_t* s_key, const Pos* s_pos, float (*s_head)[kThreads], uint8_t* s_through,
+                                               uint32_t count, uint32_t chunk, int pack0, int pack1, int width, float* slab) {
   using Ch = Channels<T, kVec>;
-  extern __shared__ uint32_t s_mem[];
-  __shared__ float s_head[kVec][kEmbThreads];   // of each group's chunk: the sum of the run that began before it
-  __shared__ uint8_t s_through[kEmbThreads];    // and whether that run goes on behind it
-  chain_release();
-  const int packs = p.C / kVec, width = min(kEmbThreads, packs), lanes = kEmbThreads / width;
-  const int cx = threadIdx.x % width, ry = threadIdx.x / width;
-  const uint32_t per_cta = lanes * p.chunk;
-  uint32_t* s_key = s_mem + 1;               // keys of the CTA's positions, one before and one behind them
-  uint32_t* s_pos = s_mem + per_cta + 2;
-  chain_wait();
-  const uint32_t base = blockIdx.x * per_cta;  // < n
-  const uint32_t none = 0xFFFFFFFFu;
-  for (uint32_t i = threadIdx.x; i < per_cta + 2u; i += kEmbThreads) {
-    const uint32_t at = base + i - 1u;  // wraps to 2^32 - 1 ahead of the first
-    uint32_t key = none, pos = 0;
-    if (at < p.n) {
-      pos = static_cast<uint32_t>(__ldg(&p.order[at]));
-      pos = min(pos, p.n - 1u);  // the order is void after a sort that gave up
-      key = static_cast<uint32_t>(__ldg(&p.keys[pos]));
-    }
-    s_mem[i] = key;
-    if (i >= 1u && i <= per_cta) s_pos[i - 1u] = pos;
-  }
-  __syncthreads();
-  const uint32_t count = min(per_cta, p.n - base);  // positions of the CTA
-  const uint32_t b = ry * p.chunk, e = min(b + p.chunk, count);
+  const int lanes = kThreads / width, cx = threadIdx.x % width, ry = threadIdx.x / width;
+  const uint32_t b = ry * chunk, e = min(b + chunk, count);
   const bool active = ry < lanes && b < e;
   const T* g = static_cast<const T*>(p.g);
   T* grad = static_cast<T*>(p.grad);
   auto open_at = [&](uint32_t i) { return s_key[int(i) - 1] == s_key[i]; };  // position i continues a run
-  if (threadIdx.x == 0) {
-    const uint32_t last = s_key[count - 1u];
-    p.info[blockIdx.x] = EmbInfo{last, (s_key[count] == last ? kGoesOn : 0u) | (open_at(0) && s_key[0] == last ? kThrough : 0u)};
-  }
   if (cx == 0 && ry < lanes) s_through[ry] = active && open_at(b) && s_key[b] == s_key[e - 1u] && s_key[e] == s_key[b];
-  for (int c0 = 0; c0 < packs; c0 += width) {
+  for (int c0 = pack0; c0 < pack1; c0 += width) {
     const int c = c0 + cx;
-    const bool mine = active && c < packs;
+    const bool mine = active && c < pack1;
     float acc[kVec];
 #pragma unroll
     for (int i = 0; i < kVec; ++i) acc[i] = 0.f;
@@ -220,7 +198,7 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const EmbGra
     if (mine) {
       const bool from_before = ry == 0 && open_at(0);
       auto collect = [&](float (&sum)[kVec], uint32_t k, int r, bool before) {
-        for (bool more = true; more && r < lanes && r * p.chunk < count; ++r) {
+        for (bool more = true; more && r < lanes && r * chunk < count; ++r) {
 #pragma unroll
           for (int i = 0; i < kVec; ++i) sum[i] += s_head[i][r * width + cx];
           more = s_through[r] != 0;
@@ -234,7 +212,7 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const EmbGra
         }
         // a run that began before the CTA, or goes on behind it
         if (k >= p.rows) return;
-        float* to = p.slab + (size_t(blockIdx.x) * 2 + (before ? 0 : 1)) * p.C + c * kVec;
+        float* to = slab + (before ? 0 : p.C) + c * kVec;
 #pragma unroll
         for (int i = 0; i < kVec; ++i) to[i] = sum[i];
       };
@@ -250,6 +228,38 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const EmbGra
     }
     __syncthreads();
   }
+}
+
+template <typename T, int kVec>
+__global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const EmbGrad p) {
+  extern __shared__ uint32_t s_mem[];
+  __shared__ float s_head[kVec][kEmbThreads];
+  __shared__ uint8_t s_through[kEmbThreads];
+  chain_release();
+  const int packs = p.C / kVec, width = min(kEmbThreads, packs), lanes = kEmbThreads / width;
+  const uint32_t per_cta = lanes * p.chunk;
+  uint32_t* s_key = s_mem + 1;               // keys of the CTA's positions, one before and one behind them
+  uint32_t* s_pos = s_mem + per_cta + 2;
+  chain_wait();
+  const uint32_t base = blockIdx.x * per_cta;  // < n
+  for (uint32_t i = threadIdx.x; i < per_cta + 2u; i += kEmbThreads) {
+    const uint32_t at = base + i - 1u;  // wraps to 2^32 - 1 ahead of the first
+    uint32_t key = kNoKey, pos = 0;
+    if (at < p.n) {
+      pos = static_cast<uint32_t>(__ldg(&p.order[at]));
+      pos = min(pos, p.n - 1u);  // the order is void after a sort that gave up
+      key = static_cast<uint32_t>(__ldg(&p.keys[pos]));
+    }
+    s_mem[i] = key;
+    if (i >= 1u && i <= per_cta) s_pos[i - 1u] = pos;
+  }
+  __syncthreads();
+  const uint32_t count = min(per_cta, p.n - base);  // positions of the CTA
+  if (threadIdx.x == 0) {
+    const uint32_t last = s_key[count - 1u];
+    p.info[blockIdx.x] = EmbInfo{last, (s_key[count] == last ? kGoesOn : 0u) | (s_key[-1] == s_key[0] && s_key[0] == last ? kThrough : 0u)};
+  }
+  embedding_runs<T, kVec, kEmbThreads>(p, s_key, s_pos, s_head, s_through, count, p.chunk, 0, packs, width, p.slab + size_t(blockIdx.x) * 2 * p.C);
 }
 
 // The runs that lie in more than one CTA of the sum kernel: CTA q takes the one that began in that kernel's CTA q and goes
@@ -312,7 +322,166 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_join_kernel(const EmbGr
   }
 }
 
+// ------------------------------------------------------------------ gradient of few positions
+// One launch.  Every CTA sorts all positions by key in its shared memory (stable, 9 bits a pass, as fgb_sort.cu does over tiles).  The first
+// ones take four packs of channels each and add up all runs, so that none leaves a CTA; the others clear the rows that no
+// position holds.  With the seven launches of the other way a call of some rows took 47 us of host time, 38 of them autograd's.
+constexpr int kFewThreads = 512, kFewItems = 8, kFewPositions = kFewThreads * kFewItems, kFewPacks = 4, kFewWarps = kFewThreads / 32;
+constexpr int kFewBitWords = 2048;  // rows that a clearing CTA looks at at a time, in words of bits
+
+struct FewArgs {
+  const void* indices;
+  int wide, passes;
+  int64_t padding;
+  unsigned sum_ctas;
+  int32_t* status;
+  int32_t* mirror;
+};
+
+template <typename T, int kVec>
+__global__ void __launch_bounds__(kFewThreads) embedding_few_kernel(const EmbGrad p, const FewArgs q) {
+  using Ch = Channels<T, kVec>;
+  // counters of the sort [warps][digits]; then the heads of the sums, or the bits of the rows that positions hold
+  __shared__ __align__(16) uint8_t s_shared[16384];
+  __shared__ uint32_t s_mem[kFewPositions + 2];
+  __shared__ uint16_t s_pos[kFewPositions];
+  __shared__ uint32_t s_scan[kFewWarps];
+  __shared__ uint8_t s_through[kFewThreads];
+  static_assert(kFewWarps * kSortDigits * 2 <= 16384 && 8 * kFewThreads * 4 <= 16384 && kFewBitWords * 4 <= 16384 && kSortDigits == kFewThreads);
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  chain_release();
+  chain_wait();
+  const int packs = p.C / kVec;
+  const bool sums = blockIdx.x < q.sum_ctas;
+  // item j of lane l of warp w: position w * 256 + j * 32 + l
+  uint32_t key[kFewItems], pos[kFewItems];
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < kFewItems; ++j) {
+    pos[j] = w * (32 * kFewItems) + j * 32 + lane;
+    key[j] = kNoKey;
+    if (pos[j] < p.n) {
+      const int64_t v = index_at(q.indices, q.wide, pos[j]);
+      const bool in = v >= 0 && v < int64_t(p.rows);
+      bad |= !in;
+      if (in && v != q.padding) key[j] = static_cast<uint32_t>(v);
+    }
+  }
+  if (bad && blockIdx.x == 0u) {
+    report(q.status, FGB_S_BAD_INDEX);
+    mirror_code(q.mirror, FGB_S_BAD_INDEX);
+  }
+  if (!sums) {
+    uint32_t* s_bits = reinterpret_cast<uint32_t*>(s_shared);
+    T* grad = static_cast<T*>(p.grad);
+    const int width = min(kFewThreads, packs), lanes = kFewThreads / width, cx = tid % width, ry = tid / width;
+    const uint32_t ctas = gridDim.x - q.sum_ctas, per = min((p.rows + ctas - 1u) / ctas, kFewBitWords * 32u);
+    for (uint64_t r0 = uint64_t(blockIdx.x - q.sum_ctas) * per; r0 < p.rows; r0 += uint64_t(ctas) * per) {
+      const uint32_t first = static_cast<uint32_t>(r0), rows = min(per, p.rows - first);
+      for (uint32_t i = tid; i < (rows + 31u) / 32u; i += kFewThreads) s_bits[i] = 0u;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kFewItems; ++j) {
+        const uint32_t r = key[j] - first;  // no key: far beyond, first + rows is below 2^31
+        if (key[j] != kNoKey && r < rows) atomicOr(&s_bits[r / 32u], 1u << (r & 31u));
+      }
+      __syncthreads();
+      if (ry < lanes) {
+        for (uint32_t r = ry; r < rows; r += lanes) {
+          if (s_bits[r / 32u] >> (r & 31u) & 1u) continue;
+          for (int c = cx; c < packs; c += width) Ch::store(grad + size_t(first + r) * p.C + c * kVec, typename Ch::Raw{});
+        }
+      }
+      __syncthreads();
+    }
+    return;
+  }
+  uint32_t* s_key = s_mem + 1;
+  uint16_t(*s_cnt)[kSortDigits] = reinterpret_cast<uint16_t(*)[kSortDigits]>(s_shared);
+  uint32_t held = 0;  // positions that have a key
+#pragma unroll
+  for (int j = 0; j < kFewItems; ++j) held += __popc(__ballot_sync(0xffffffffu, key[j] != kNoKey));
+  const uint32_t lt = (1u << lane) - 1u;
+  for (int pass = 0; pass < q.passes; ++pass) {
+    const int shift = pass * kSortDigitBits;
+    for (int i = tid; i < kFewWarps * kSortDigits / 2; i += kFewThreads) reinterpret_cast<uint32_t*>(s_shared)[i] = 0u;
+    __syncthreads();
+    uint32_t rank[kFewItems];
+#pragma unroll
+    for (int j = 0; j < kFewItems; ++j) {  // positions without a key have the largest digit in every pass, and come last
+      const uint32_t d = (key[j] >> shift) & (kSortDigits - 1);
+      const unsigned peers = __match_any_sync(0xffffffffu, d);
+      const int leader = __ffs(peers) - 1;
+      uint32_t before = 0;
+      if (lane == leader) {
+        before = s_cnt[w][d];
+        s_cnt[w][d] = static_cast<uint16_t>(before + __popc(peers));
+      }
+      rank[j] = __shfl_sync(0xffffffffu, before, leader) + __popc(peers & lt);
+      __syncwarp();
+    }
+    __syncthreads();
+    // thread t: digit t
+    uint32_t count = 0;
+#pragma unroll
+    for (int ww = 0; ww < kFewWarps; ++ww) {
+      const uint32_t c = s_cnt[ww][tid];
+      s_cnt[ww][tid] = static_cast<uint16_t>(count);
+      count += c;
+    }
+    uint32_t upto = count;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += o;
+    }
+    if (lane == 31) s_scan[w] = upto;
+    __syncthreads();
+    uint32_t base = upto - count;
+    for (int ww = 0; ww < w; ++ww) base += s_scan[ww];
+#pragma unroll
+    for (int ww = 0; ww < kFewWarps; ++ww) s_cnt[ww][tid] = static_cast<uint16_t>(s_cnt[ww][tid] + base);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kFewItems; ++j) {
+      const uint32_t to = s_cnt[w][(key[j] >> shift) & (kSortDigits - 1)] + rank[j];
+      s_key[to] = key[j], s_pos[to] = static_cast<uint16_t>(pos[j]);
+    }
+    __syncthreads();
+    if (pass + 1 < q.passes) {
+#pragma unroll
+      for (int j = 0; j < kFewItems; ++j) {
+        const uint32_t at = w * (32 * kFewItems) + j * 32 + lane;
+        key[j] = s_key[at], pos[j] = s_pos[at];
+      }
+    }
+  }
+  if (tid == 0) s_key[-1] = kNoKey;
+  if (lane == 0) s_scan[w] = held;
+  __syncthreads();
+  uint32_t count = 0;
+#pragma unroll
+  for (int ww = 0; ww < kFewWarps; ++ww) count += s_scan[ww];
+  if (tid == 0) s_key[count] = kNoKey;  // behind the positions that have a key
+  __syncthreads();
+  const int pack0 = static_cast<int>(blockIdx.x) * kFewPacks, pack1 = min(packs, pack0 + kFewPacks), width = pack1 - pack0;
+  // Long chunks are rows one after the other, short ones heads one after the other that a run through all of them collects
+  const uint32_t lanes = kFewThreads / width;
+  const uint32_t chunk = max(count <= 512u ? 8u : count <= 2048u ? 16u : 32u, (count + lanes - 1u) / lanes);
+  embedding_runs<T, kVec, kFewThreads>(p, s_key, s_pos, reinterpret_cast<float(*)[kFewThreads]>(s_shared), s_through, count, chunk, pack0, pack1, width, nullptr);
+}
+
 // ------------------------------------------------------------------ host side
+static bool emb_few(const fgb_embedding_call& c) { return c.n <= kFewPositions && c.c / row_pack(c.c, elem_bytes(c.dtype)) <= 256; }
+
+template <typename T, int kVec>
+static cudaError_t emb_few_launch(const EmbGrad& a, FewArgs q, cudaStream_t s) {
+  q.sum_ctas = static_cast<unsigned>(ceil_div(a.C / kVec, kFewPacks));
+  // rows are cleared some 16 KB a CTA, by two CTAs an SM at most
+  const int64_t clear = std::min<int64_t>(ceil_div(int64_t(a.rows) * a.C * static_cast<int64_t>(sizeof(T)), 16384), int64_t(device_sm_count()) * 2);
+  return launch_chained(embedding_few_kernel<T, kVec>, dim3(q.sum_ctas + static_cast<unsigned>(clear)), dim3(kFewThreads), 0, s, a, q);
+}
+
 struct EmbPlan {
   int vec, lanes;
   uint32_t chunk, ctas;
@@ -423,6 +592,20 @@ extern "C" int fgb_embedding_backward(const fgb_embedding_call* c, void* stream)
   int32_t* keys = reinterpret_cast<int32_t*>(ws + p.keys_off);
   int64_t* order = reinterpret_cast<int64_t*>(ws + p.order_off);
   const uint32_t n = static_cast<uint32_t>(c->n), rows = static_cast<uint32_t>(c->rows);
+  int key_bits = 1;
+  while (key_bits < 31 && (rows >> key_bits) != 0u) ++key_bits;  // the largest key is `rows`
+  EmbGrad a{};
+  a.g = c->grad_out, a.grad = c->grad_table, a.keys = keys, a.order = order;
+  a.slab = reinterpret_cast<float*>(ws + p.slab_off), a.info = reinterpret_cast<EmbInfo*>(ws + p.info_off);
+  a.n = n, a.rows = rows, a.chunk = p.chunk, a.ctas = p.ctas, a.C = c->c, a.scale = c->scale;
+  if (n > 0 && emb_few(*c)) {
+    const FewArgs q{c->indices, c->index_bits == 64, sort_passes_of(key_bits), c->padding_idx, 0u, c->status, status_mirror(c->status)};
+    cudaError_t e;
+    if (c->dtype == FGB_F16) e = FGB_BY_PACK(__half, p.vec, emb_few_launch)(a, q, s);
+    else if (c->dtype == FGB_BF16) e = FGB_BY_PACK(__nv_bfloat16, p.vec, emb_few_launch)(a, q, s);
+    else e = FGB_BY_PACK(float, p.vec, emb_few_launch)(a, q, s);
+    return e != cudaSuccess ? cuda_status(e) : launch_status();
+  }
   const uint64_t halves = uint64_t(c->rows) * c->c * (elem_bytes(c->dtype) / 2);
   const int64_t units = std::max<int64_t>(c->n, static_cast<int64_t>(halves / 8));
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(ceil_div(units, kEmbThreads), 1), int64_t(device_sm_count()) * 8));
@@ -430,14 +613,8 @@ extern "C" int fgb_embedding_backward(const fgb_embedding_call* c, void* stream)
                                  static_cast<uint16_t*>(c->grad_table), halves, c->status, status_mirror(c->status));
   if (e != cudaSuccess) return cuda_status(e);
   if (n == 0) return launch_status();
-  int key_bits = 1;
-  while (key_bits < 31 && (rows >> key_bits) != 0u) ++key_bits;  // the largest key is `rows`
   rc = fgb_pp_sorted_idx(keys, c->n, key_bits, order, ws + p.sort_off, static_cast<int64_t>(p.sort_bytes), c->status, stream);
   if (rc != FGB_OK) return rc;
-  EmbGrad a{};
-  a.g = c->grad_out, a.grad = c->grad_table, a.keys = keys, a.order = order;
-  a.slab = reinterpret_cast<float*>(ws + p.slab_off), a.info = reinterpret_cast<EmbInfo*>(ws + p.info_off);
-  a.n = n, a.rows = rows, a.chunk = p.chunk, a.ctas = p.ctas, a.C = c->c, a.scale = c->scale;
   if (c->dtype == FGB_F16) e = FGB_BY_PACK(__half, p.vec, emb_sum)(a, p, s);
   else if (c->dtype == FGB_BF16) e = FGB_BY_PACK(__nv_bfloat16, p.vec, emb_sum)(a, p, s);
   else e = FGB_BY_PACK(float, p.vec, emb_sum)(a, p, s);
