@@ -1,1 +1,1 @@
-from . import spconv, utils  # noqa: F401
+from . import embedding, grid_sample, group_norm, grouped_linear, spconv, utils  # noqa: F401

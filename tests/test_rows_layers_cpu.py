@@ -41,6 +41,16 @@ def test_oracle_embedding_is_torchs():
     assert torch.allclose(got, want, rtol=1e-12, atol=1e-12) and (size >= got.abs() - 1e-12).all()
 
 
+def test_layers_are_attributes_of_the_package(lib):
+    """As they are documented, after an import of the package alone."""
+    import os
+    import subprocess
+    import sys
+    code = "import flexgemm_b200.ops as ops; ops.embedding.sparse_embedding, ops.group_norm.sparse_group_norm, ops.grouped_linear.sparse_grouped_linear, " \
+           "ops.utils.sample_offsets, ops.grid_sample.grid_sample_3d"
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+
 def test_group_norm_refuses(lib):
     from flexgemm_b200.ops.group_norm import sparse_group_norm
     x, off = torch.randn(10, 8), torch.tensor([0, 4, 10])
