@@ -18,8 +18,9 @@
 // the next, so slots are unique, those of a sample are consecutive, and nothing has to be planned ahead.
 //
 // Measured (B200): 166000 x 256 fp16 with SiLU, one sample, forward + backward 162 us (floor 65: x and y, x, dy and dx once each; with
-// the second reads of x and dy 104), 39872 x 512 bf16 of four samples 95 us: sums 16, join 6, apply 19, backward 26, 7 and 27.
-// The long way's sums and apply run at 75 to 80 % of the copy rate; a short sample is bound by its chain of latencies.
+// the second reads of x and dy 104), 39872 x 512 bf16 of four samples 95 us: sums 13, join 6, apply 19, backward 26, 7 and 27.
+// Of the copy rate that is 57 and 77 % in the sums and apply of the first, 48 and 67 to 70 % of the second; a short sample is bound by its
+// chain of latencies.
 #include <algorithm>
 
 #include "fgb_common.cuh"
@@ -555,8 +556,8 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas) norm_apply_kernel(con
 // Ragged samples may be long ones in between, and a team would be at one long after all others are done.  Teams leave samples of
 // more than long_rows rows out, and a second launch (kLong) takes them in clusters of kLongCtas CTAs; neighbours, which are often
 // alike, go to different clusters.  us, in one launch / in two (bf16, 96 channels): 2000 samples of 7 rows around one of 50000, forward
-// 2591 / 159, backward 7374 / 321; 2000 samples of 20 rows 14.5 / 16.9 and 28.2 / 31.5.  Lengths that scatter like exp(N(0, 1)) (80000
-// rows of fp32 in 2048 samples, forward + backward): 110 to 162 / 130.
+// 2591 / 132, forward and backward 9965 / 378; 2000 samples of 20 rows 14.5 / 16.9 and 28.2 / 31.5.  Lengths that scatter like exp(N(0, 1)) (80000
+// rows of fp32 in 2048 samples, forward + backward): 110 to 162 / 128.
 constexpr int kLongCtas = 8, kLongClusters = 18;
 struct SmallArgs {
   int team;            // threads of a CTA that take a sample: 32, 64, 128 or 256

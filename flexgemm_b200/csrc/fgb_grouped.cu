@@ -28,8 +28,10 @@
 // (all whose weight is 2^-16 and more) for accurate fp32, three (2^-8 and more) where TF32 is allowed.  A plane leaves half a step of
 // eight bits, 2^-8, of what it takes, so that four terms of 2^-24 of a product are left out, or three of 2^-16.  bf16 has
 // fp32's range, so no scaling is needed, and six of them cost what three TF32 products do (half the rate, twice the bytes).
-// The tensor cores cut what they add to an accumulator at its last bit instead of rounding: over a long k that is a bias
-// (2e-8 of the sum for every 16 k; 1e-5 where k was 10^5).  So fp32 leaves the accumulator after each block of 64 k, the small
+// The tensor cores cut what they add to an accumulator at its last bit instead of rounding: over a long k that is a bias, 5e-8 to 8e-8 of
+// the sum for every 16 k where all terms have one sign (a weight gradient of 6400 / 25600 / 102400 rows that is not cut: 2e-5, 1.3e-4, 3.0e-4
+// low).  16-bit results take that: half a step of fp16 is 4.9e-4, of bf16 3.9e-3, and where tiles are fewer than the CTAs have time for,
+// their parts are added in fp32.  fp32 leaves the accumulator after each block of 64 k, the small
 // products first, the large one last, and the storing warps add the blocks up in registers, rounding to nearest.  A stage has
 // all planes of its block: each is loaded once for the two or three products that it is in.
 #include <algorithm>
@@ -45,7 +47,7 @@ namespace fgb {
 // Measured (B200): 131072 rows of 16 groups, 1024 x 1024 bf16: forward 195 to 210 us, input gradient 211, weight gradient 254 and 21
 // for the join (one cuBLAS product of that size 209, 209, 210; the clock is at the power cap); 166000 of 27, 256 x 256 fp16: 33, 33
 // and 54 (33, 33, 45), forward at 80 % of the copy rate; 24 rows of 64 groups, 512 -> 1024: 8 us, a chain of plan, loads,
-// products and stores (the touched matrices alone take 4).
+// products and stores (the touched matrices alone take 4).  40000 of 4, 256 x 256 fp32: forward 67 us.
 constexpr int kGrThreads = 320;
 constexpr int kGrEpilogueWarps = 8;
 constexpr int kGrMaxStages = 12;
@@ -1023,7 +1025,8 @@ static bool few_rows(const fgb_grouped_linear_call& c) { return c.n <= 16 * c.gr
 static int grouped_plan(const fgb_grouped_linear_call& c, int pass, GroupedPlan& p) {
   const int64_t sms = device_sm_count();
   const int64_t N = c.n, G = c.groups;
-  // fp32: the blocks' sums of a tile are held in 3 x 32 registers, and two stages of three planes in shared memory
+  // fp32: the blocks' sums of a tile are held in 3 x 32 registers, and two stages of three planes in shared memory (a stage has 98304 bytes
+  // at most; beyond some 1400 groups the schedule, 12 bytes each, leaves room for one of those, and loads and products take turns)
   auto most = [&](bool pair) { return !is_f32(c.dtype) ? 256 : pair ? 192 : 96; };
   int64_t blocks, db_units = 0;
   p = GroupedPlan{};

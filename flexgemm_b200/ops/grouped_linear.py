@@ -24,8 +24,8 @@ def sparse_grouped_linear(feats: torch.Tensor, offsets: torch.Tensor, weight: to
 
     Returns:
         [N, Co] of the features' type; sums are float32, the result is rounded once.  float32 follows
-        ``kernels.config.allow_tf32`` at the time a pass runs: a product is off by 3 * 2^-16 of its value at most where it is set,
-        by 2^-21 otherwise (an infinity among float32 inputs gives NaN).  Differentiable (once) in feats, weight and bias.  Offsets that do not
+        ``kernels.config.allow_tf32`` at the time a pass runs: a product is off by 3 * 2^-16 of its value at most where it is set
+        (a term of the bias gradient by 2^-16), by 2^-21 otherwise (an infinity among float32 inputs gives NaN).  Differentiable (once) in feats, weight and bias.  Offsets that do not
         ascend or leave the rows raise from a later call, as every error that the device finds.
     """
     out = _native.ext().grouped_linear(feats, offsets, weight, bias, config.allow_tf32)
