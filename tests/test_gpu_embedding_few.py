@@ -141,3 +141,19 @@ def test_stream_capture_and_two_graphs():
         torch.cuda.synchronize()
         for _, g, scale in graphs:
             assert torch.equal(g, grad(new, table, dy, scale=scale))
+
+
+def test_launches():
+    """A call with gradient of up to 4096 positions is two launches, the lookup and the gradient; the way of many is taken beyond."""
+    from flexgemm_b200 import _cabi
+    from flexgemm_b200.ops.embedding import sparse_embedding
+    count = _cabi.lib().fgb_launch_count
+    def launches(n, C):
+        idx, table, dy = problem(n, 300, C, torch.float32, seed=8)
+        t = table.to(DEV).requires_grad_(True)
+        i, d = idx.to(DEV), dy.to(DEV)
+        before = count()
+        torch.autograd.grad(sparse_embedding(i, t), [t], d)
+        return count() - before
+    assert launches(1, 8) == 2 and launches(2520, 64) == 2 and launches(4096, 1024) == 2
+    assert launches(4097, 8) > 2 and launches(100, 1028) > 2
